@@ -482,6 +482,145 @@ NF_API int nf_router_topk_noalloc(const uint16_t* x_dev, const uint16_t* router_
                                   float routed_scaling, int32_t* topk_idx_dev, float* topk_w_dev, char* msg,
                                   int msg_len, void* stream);
 
+/* ---- verifying drafted tokens: cache, tree attention, log-probabilities ------
+ * The operators of a step that runs several new tokens of every sequence at
+ * once: a chain (a prompt's chunk) or a tree of drafted tokens, of which the
+ * host then keeps one path.  The reference decodes its target model token by
+ * token (TextModel::step, src/text_forward.cpp:625-698); its draft model's
+ * attention (draft_attention, :1216-1289) is the math of nf_kv_write and
+ * nf_tree_attention.  All of them work on caller-owned device buffers of the
+ * current device, enqueue on `stream` and allocate nothing; all but
+ * nf_rope_init may be captured into a CUDA graph.  Every host argument is
+ * checked before any CUDA call; a failed call's message is
+ * nf_kv_last_error() on the same thread.  Device arrays of indices cannot be
+ * checked on the host: a row or sequence whose indices lie outside the
+ * buffers is left out as each call says, and *status_dev (INT32 [1],
+ * optional, cleared by the caller) becomes nonzero. */
+enum { NF_KV_BF16 = 0, NF_KV_E4M3 = 1 };
+enum { NF_DTYPE_F32 = 0, NF_DTYPE_BF16 = 1 };
+/* A layer's cache: keys and values [seqs][kv_heads][max_context][head_dim].
+ * NF_KV_BF16: BF16, scales NULL.  NF_KV_E4M3: E4M3FN codes, and one F32 scale
+ * per row, [seqs][kv_heads][max_context]; a row stands for code * scale.
+ * head_dim 64 or 128; k and v 16-byte aligned; seqs * kv_heads and
+ * max_context below 2^31. */
+typedef struct nf_kv_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int32_t kind; /* NF_KV_BF16 or NF_KV_E4M3 */
+    int32_t seqs, kv_heads, max_context, head_dim;
+} nf_kv_cache;
+/* Message of this thread's last failed call of this section ("" when none). */
+NF_API const char* nf_kv_last_error(void);
+
+/* Rotary positions: pair i of a head's first rotary_dim dims turns by
+ * position * f_i radians, f_i = theta^(-2 i / rotary_dim) scaled as chosen.
+ * The table holds f_i / (2 pi) as 64-bit binary fractions of a turn, so
+ * position * turn[i] modulo 2^64 is the angle of any 31-bit position to
+ * 2^-33 of a turn. */
+enum {
+    NF_ROPE_HALF = 0,       /* pairs (i, i + rotary_dim / 2), rope_heads src/text_forward.cpp:1169-1184 */
+    NF_ROPE_INTERLEAVED = 1 /* pairs (2 i, 2 i + 1) */
+};
+enum {
+    NF_ROPE_PLAIN = 0,
+    NF_ROPE_LINEAR = 1, /* f_i / factor */
+    NF_ROPE_YARN = 2    /* with r_i = original_context f_i / (2 pi) and g_i = clamp((r_i - slow) / (fast - slow), 0, 1):
+                           g_i f_i + (1 - g_i) f_i / factor, the rotated dims multiplied by 0.1 ln(factor) + 1 */
+};
+typedef struct nf_rope {
+    int32_t head_dim, rotary_dim, layout;
+    float magnitude; /* factor on the rotated dims */
+    uint64_t turn[64];
+} nf_rope;
+/* Fills *out (host only, no CUDA call).  rotary_dim even, 0 (no rotation) to
+ * head_dim; theta > 0; factor >= 1; YaRN: original_context > 0 and fast > slow. */
+NF_API int nf_rope_init(nf_rope* out, int head_dim, int rotary_dim, int layout, double theta, int scaling,
+                        double factor, double original_context, double fast, double slow);
+
+/* The rows of a fused q/k/v projection into q and the cache:
+ *   qkv_dev  F32 or BF16 [tokens][row_stride], a row [q | k | v] heads of
+ *            head_dim each; row_stride in elements, rows 16-byte aligned
+ *   q, k     per-head RMSNorm (q_norm_dev / k_norm_dev F32 [head_dim], NULL:
+ *            none; norm_eps), then the rotary position pos_dev INT32
+ *            [tokens] (>= 0)
+ *   q_dev    BF16 [tokens][q_heads][head_dim], 16-byte aligned
+ *   k, v     to row slot_dev[t] of sequence seq_dev[t] (INT32 [tokens]; NULL:
+ *            slot = pos, sequence = t), rounded to BF16, or as E4M3 codes
+ *            with scale = max |x| / 448 (a row of zeros has scale 0; a row
+ *            that holds an infinity or a NaN reads back as NaN)
+ * slot -1 writes no cache row (a padded batch).  A token whose slot, sequence
+ * or position lies outside writes no cache row and a q of NaN, and sets
+ * *status_dev.  No two tokens of a call may name the same row: it would hold
+ * a mixture of both. */
+NF_API int nf_kv_write(const nf_kv_cache* cache, const nf_rope* rope, const void* qkv_dev, int qkv_type,
+                       int64_t row_stride, int tokens, int q_heads, const float* q_norm_dev, const float* k_norm_dev,
+                       float norm_eps, const int32_t* pos_dev, const int32_t* seq_dev, const int32_t* slot_dev,
+                       uint16_t* q_dev, int32_t* status_dev, void* stream);
+
+/* Attention of every sequence's new rows over its cache:
+ *   row r of sequence i (rows row_start_dev[i] .. row_start_dev[i + 1] - 1 of
+ *   q; INT32 [batch + 1], not decreasing) attends to the cached positions
+ *   0 .. prefix_dev[i] - 1 of cache sequence cache_seq_dev[i] (INT32 [batch];
+ *   NULL: i) and to the sequence's own new rows, whose keys and values lie in
+ *   the cache behind the prefix (row j of the sequence at prefix + j):
+ *     mask_dev NULL: rows 0 .. r of the sequence (a chain)
+ *     mask_dev UINT64 [rows][mask_words]: row j when bit j % 64 of word
+ *     j / 64 of row r is set (a tree: a node's ancestors and itself); rows
+ *     from 64 mask_words on are seen by none
+ *   out = softmax(scale q . k) v, with q head h on KV head h / (q_heads /
+ *   kv_heads); a row that sees nothing gives zeros
+ *   q_dev, out_dev  BF16 [rows][q_heads][head_dim], 16-byte aligned
+ *   workspace_dev   nf_tree_attention_workspace(head_dim) bytes, 256-byte
+ *                   aligned: calls in flight at the same time need one each
+ * q_heads a multiple of kv_heads, at most 128 per KV head; mask_words 1 to 64.
+ * Scores, softmax statistics and sums are F32; the probabilities are rounded
+ * to BF16 for the product with the values.  What the cache holds outside the
+ * positions a row sees never reaches the row's result.  Rows behind
+ * row_start_dev[batch] stay as they were; the rows of a sequence whose
+ * prefix, rows or cache sequence lie outside the buffers become NaN, and
+ * *status_dev nonzero (row_start_dev entries are clamped to [0, rows]). */
+NF_API int64_t nf_tree_attention_workspace(int head_dim);
+NF_API int nf_tree_attention(const nf_kv_cache* cache, const uint16_t* q_dev, int rows, int q_heads,
+                             const int32_t* row_start_dev, int batch, const int32_t* prefix_dev,
+                             const int32_t* cache_seq_dev, const uint64_t* mask_dev, int mask_words, float scale,
+                             uint16_t* out_dev, void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev,
+                             void* stream);
+
+/* Log-probabilities of every row of logits (F32 or BF16 [rows][row_stride],
+ * row_stride >= vocab in elements, rows aligned to their type):
+ *   logprob_dev      F32 [rows]: x_target - log sum exp(x), natural
+ *                    logarithms; NaN for a target outside [0, vocab).
+ *                    target_dev INT32 [rows]; both may be NULL
+ *   entropy_dev      F32 [rows] or NULL: -sum p log p
+ *   top_idx_dev      INT32 [rows][top], top_logprob_dev F32 [rows][top]: the
+ *                    `top` greatest logits in falling order, the lower index
+ *                    first among equals (top 0: both NULL; at most 32 and
+ *                    vocab); a NaN logit is taken last, below -infinity
+ * A row with a NaN, or without a logit above -infinity, or with +infinity,
+ * has no distribution: its log-probabilities and entropy are NaN, its top
+ * indices still those of the order above.
+ * workspace_dev: nf_token_logprobs_workspace(rows, vocab, top) bytes, 16-byte
+ * aligned; calls in flight at the same time need one each. */
+NF_API int64_t nf_token_logprobs_workspace(int rows, int64_t vocab, int top);
+NF_API int nf_token_logprobs(const void* logits_dev, int logits_type, int64_t row_stride, int rows, int64_t vocab,
+                             const int32_t* target_dev, int top, float* logprob_dev, float* entropy_dev,
+                             int32_t* top_idx_dev, float* top_logprob_dev, void* workspace_dev,
+                             int64_t workspace_bytes, void* stream);
+
+/* Keeps one path of every sequence's tree: cache row prefix_dev[i] +
+ * path_dev[i][j] of sequence cache_seq_dev[i] (NULL: i) moves to row
+ * prefix_dev[i] + j, for j < path_len_dev[i], in every layer's cache (same
+ * shape and kind; `layers` structs on the host).  path_dev INT32
+ * [batch][max_path]: nodes in rising order, as a child's index is above its
+ * parent's.  A sequence with indices outside the cache, or a path that does
+ * not rise, is left as it was and sets *status_dev.  No two entries of a call
+ * may name the same cache sequence. */
+NF_API int nf_kv_accept(const nf_kv_cache* caches, int layers, const int32_t* prefix_dev, const int32_t* path_dev,
+                        int max_path, const int32_t* path_len_dev, const int32_t* cache_seq_dev, int batch,
+                        int32_t* status_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -47,6 +47,8 @@ EXPORTED = [
     "nf_tp_linear_bf16", "nf_tp_argmax", "nf_tp_result", "nf_tp_sync", "nf_stack_create", "nf_stack_destroy",
     "nf_stack_last_error", "nf_stack_layer_ffn", "nf_stack_bind_bf16", "nf_stack_bind_f32", "nf_stack_finalize",
     "nf_stack_kv_cache", "nf_stack_decode", "nf_stack_sync", "nf_stack_load_kv", "nf_stack_fill_kv",
+    "nf_kv_last_error", "nf_rope_init", "nf_kv_write", "nf_tree_attention_workspace", "nf_tree_attention",
+    "nf_token_logprobs_workspace", "nf_token_logprobs", "nf_kv_accept",
 ]
 STAGES = ["router", "permute", "gate_up", "down", "shared", "combine"]
 
@@ -70,6 +72,23 @@ class StackDesc(ctypes.Structure):
     ]
 
 
+class KvDesc(ctypes.Structure):
+    """nf_kv_cache"""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("kind", ctypes.c_int32), ("seqs", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("max_context", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+    ]
+
+
+class RopeDesc(ctypes.Structure):
+    """nf_rope"""
+    _fields_ = [
+        ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("layout", ctypes.c_int32),
+        ("magnitude", ctypes.c_float), ("turn", ctypes.c_uint64 * 64),
+    ]
+
+
 _lib = None
 
 
@@ -81,7 +100,7 @@ def load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise RuntimeError(f"{LIB_PATH} is missing: build it with python build.py")
     lib = ctypes.CDLL(str(LIB_PATH))
-    P, I32, I64, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+    P, I32, I64, F, D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
     sig = {
         "nf_moe_create": ([ctypes.POINTER(Desc), I32, ctypes.POINTER(P)], I32),
         "nf_moe_destroy": ([P], None),
@@ -134,6 +153,14 @@ def load() -> ctypes.CDLL:
         "nf_stack_sync": ([P, P], I32),
         "nf_stack_load_kv": ([P, I32, P, P], I32),
         "nf_stack_fill_kv": ([P, ctypes.c_uint64], I32),
+        "nf_kv_last_error": ([], ctypes.c_char_p),
+        "nf_rope_init": ([P, I32, I32, I32, D, I32, D, D, D, D], I32),
+        "nf_kv_write": ([P, P, P, I32, I64, I32, I32, P, P, F, P, P, P, P, P, P], I32),
+        "nf_tree_attention_workspace": ([I32], I64),
+        "nf_tree_attention": ([P, P, I32, I32, P, I32, P, P, P, I32, F, P, P, I64, P, P], I32),
+        "nf_token_logprobs_workspace": ([I32, I64, I32], I64),
+        "nf_token_logprobs": ([P, I32, I64, I32, I64, P, I32, P, P, P, P, P, I64, P], I32),
+        "nf_kv_accept": ([P, I32, P, P, I32, P, P, I32, P, P], I32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -850,3 +877,187 @@ class DecoderStack:
 
     def sync(self, stream=0) -> None:
         self._check(self.lib.nf_stack_sync(self.h, stream or None))
+
+
+# ---- verifying drafted tokens: cache, tree attention, log-probabilities --------
+KV_BF16, KV_E4M3 = 0, 1
+DTYPE_F32, DTYPE_BF16 = 0, 1
+ROPE_LAYOUT = dict(half=0, interleaved=1)
+ROPE_SCALING = dict(none=0, linear=1, yarn=2)
+MAX_TOP = 32  # top tokens of one token_logprobs call
+_BF16 = ("torch.bfloat16", "torch.int16", "torch.uint16")
+_CODES = ("torch.float8_e4m3fn", "torch.uint8")
+_I32, _U64 = ("torch.int32",), ("torch.int64", "torch.uint64")
+
+
+def _kv_check(st: int) -> None:
+    if st != NF_OK:
+        raise NfError(st, load().nf_kv_last_error().decode())
+
+
+def _dim(a, axis: int, name: str, rank: int) -> int:
+    """A tensor's extent; the tensor must have `rank` axes."""
+    if len(a.shape) != rank:
+        raise NfError(2, f"{name} has {len(a.shape)} axes; expected {rank}")
+    return a.shape[axis]
+
+
+class KvCache:
+    """A layer's KV cache in CUDA tensors the caller owns (nf_kv_cache): k and
+    v [seqs, kv_heads, context, head_dim], in BF16 (or its bits), or in E4M3
+    (float8_e4m3fn, or its bits as uint8) with F32 scales [seqs, kv_heads,
+    context].  Keeps the tensors alive."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        if isinstance(k, (int, np.ndarray)) or not getattr(k, "is_cuda", False):
+            raise NfError(1, "k is not a CUDA tensor")
+        self.device = dv = k.device.index
+        seqs, heads, context, dim = (_dim(k, i, "k", 4) for i in range(4))
+        kind = KV_BF16 if str(k.dtype) in _BF16 else KV_E4M3
+        types = _BF16 if kind == KV_BF16 else _CODES
+        n = seqs * heads * context
+        if (k_scale is None) != (kind == KV_BF16) or (v_scale is None) != (kind == KV_BF16):
+            raise NfError(1, "an E4M3 cache has scales, a BF16 cache has none")
+        if tuple(v.shape) != tuple(k.shape):
+            raise NfError(2, "k and v differ in shape")
+        self.desc = KvDesc(_dev(k, n * dim, types, "k", dv), _dev(v, n * dim, types, "v", dv),
+                           _dev(k_scale, n, _F32, "k_scale", dv), _dev(v_scale, n, _F32, "v_scale", dv), kind, seqs,
+                           heads, context, dim)
+        self.ref = ctypes.byref(self.desc)
+        self.tensors = (k, v, k_scale, v_scale)
+
+
+class KvCaches:
+    """Several layers' caches of one shape and kind, for kv_accept."""
+
+    def __init__(self, caches):
+        self.caches = list(caches)
+        if not self.caches:
+            raise NfError(1, "no caches")
+        self.device = self.caches[0].device
+        if any(c.device != self.device for c in self.caches):
+            raise NfError(1, "the caches lie on different devices")
+        self.descs = (KvDesc * len(self.caches))(*[c.desc for c in self.caches])
+
+
+class Rope:
+    """Rotary positions (nf_rope): layout "half" or "interleaved"; scaling
+    "none", "linear" or "yarn" (factor, original_context, fast, slow)."""
+
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, layout: str = "half", theta: float = 10000.0,
+                 scaling: str = "none", factor: float = 1.0, original_context: float = 0.0, fast: float = 32.0,
+                 slow: float = 1.0):
+        if layout not in ROPE_LAYOUT or scaling not in ROPE_SCALING:
+            raise NfError(1, f"unknown rotary layout {layout!r} or scaling {scaling!r}")
+        self.desc = RopeDesc()
+        _kv_check(load().nf_rope_init(ctypes.byref(self.desc), head_dim, head_dim if rotary_dim is None else rotary_dim,
+                                      ROPE_LAYOUT[layout], theta, ROPE_SCALING[scaling], factor, original_context,
+                                      fast, slow))
+        self.ref = ctypes.byref(self.desc)
+
+
+def _on_current(device: int, what: str) -> None:
+    if device != _current_device():
+        raise NfError(1, f"{what} is on cuda:{device}, which is not the current device")
+
+
+def kv_write(cache: KvCache, rope: Rope, qkv, q_heads: int, positions, q, *, seqs=None, slots=None, q_norm=None,
+             k_norm=None, eps: float = 1e-5, status=None, stream=0) -> None:
+    """Norms, rotates and stores a fused projection's rows (nf_kv_write): qkv
+    F32 or BF16 [tokens, (q_heads + 2 kv_heads) head_dim], rows of any stride;
+    positions, seqs and slots int32 [tokens]; q BF16 [tokens, q_heads,
+    head_dim] is written, k and v go to the cache."""
+    dv, d = cache.device, cache.desc
+    _on_current(dv, "the cache")
+    tokens, width = _dim(qkv, 0, "qkv", 2), (q_heads + 2 * d.kv_heads) * d.head_dim
+    if qkv.shape[1] != width:
+        raise NfError(2, f"qkv has {qkv.shape[1]} columns; expected {width}")
+    stride = qkv.stride(0) if tokens > 1 else width
+    if not getattr(qkv, "is_cuda", False) or qkv.device.index != dv or (tokens and qkv.stride(1) != 1):
+        raise NfError(1, f"qkv is not on cuda:{dv} with contiguous rows")
+    kind = str(qkv.dtype)
+    if kind not in ("torch.float32", "torch.bfloat16"):
+        raise NfError(1, f"qkv has dtype {qkv.dtype}; expected float32 or bfloat16")
+    if seqs is None and tokens > d.seqs:
+        raise NfError(2, f"{tokens} tokens for a cache of {d.seqs} sequences: pass seqs")
+    _kv_check(load().nf_kv_write(
+        cache.ref, rope.ref, qkv.data_ptr(), DTYPE_F32 if kind == "torch.float32" else DTYPE_BF16, stride, tokens,
+        q_heads, _dev(q_norm, d.head_dim, _F32, "q_norm", dv), _dev(k_norm, d.head_dim, _F32, "k_norm", dv), eps,
+        _dev(positions, tokens, _I32, "positions", dv), _dev(seqs, tokens, _I32, "seqs", dv),
+        _dev(slots, tokens, _I32, "slots", dv), _dev(q, tokens * q_heads * d.head_dim, _BF16, "q", dv),
+        _dev(status, 1, _I32, "status", dv), stream or None))
+
+
+def tree_attention_workspace(head_dim: int) -> int:
+    """Bytes of tree_attention's workspace."""
+    return load().nf_tree_attention_workspace(head_dim)
+
+
+def tree_attention(cache: KvCache, q, row_start, prefix, out, workspace, *, cache_seq=None, mask=None,
+                   scale: float | None = None, status=None, stream=0) -> None:
+    """Attention of new rows over the cache (nf_tree_attention): q and out BF16
+    [rows, q_heads, head_dim]; row_start int32 [batch + 1]; prefix and
+    cache_seq int32 [batch]; mask None (a chain) or 64-bit words [rows,
+    words]; scale None for head_dim ** -0.5; workspace a uint8 tensor of
+    tree_attention_workspace(head_dim) bytes."""
+    dv, d = cache.device, cache.desc
+    _on_current(dv, "the cache")
+    rows, heads, dim = _dim(q, 0, "q", 3), q.shape[1], q.shape[2]
+    if dim != d.head_dim:
+        raise NfError(2, f"q has head_dim {dim}; the cache {d.head_dim}")
+    batch = _dim(row_start, 0, "row_start", 1) - 1
+    if batch < 0:
+        raise NfError(2, "row_start holds no sequence")
+    words = 0 if mask is None else _dim(mask, 1, "mask", 2)
+    _kv_check(load().nf_tree_attention(
+        cache.ref, _dev(q, rows * heads * dim, _BF16, "q", dv), rows, heads,
+        _dev(row_start, batch + 1, _I32, "row_start", dv), batch, _dev(prefix, batch, _I32, "prefix", dv),
+        _dev(cache_seq, batch, _I32, "cache_seq", dv), _dev(mask, rows * words, _U64, "mask", dv), words,
+        dim ** -0.5 if scale is None else scale, _dev(out, rows * heads * dim, _BF16, "out", dv),
+        _dev(workspace, 0, _U8, "workspace", dv), workspace.numel(), _dev(status, 1, _I32, "status", dv),
+        stream or None))
+
+
+def token_logprobs_workspace(rows: int, vocab: int, top: int) -> int:
+    """Bytes of token_logprobs's workspace."""
+    return load().nf_token_logprobs_workspace(rows, vocab, top)
+
+
+def token_logprobs(logits, targets, logprob, entropy, top_idx, top_logprob, workspace, stream=0) -> None:
+    """Log-probabilities of every row of logits (nf_token_logprobs): logits F32
+    or BF16 [rows, vocab], rows of any stride; targets int32 and logprob F32
+    [rows], or both None; entropy F32 [rows] or None; top_idx int32 and
+    top_logprob F32 [rows, top], or both None; workspace a uint8 tensor of
+    token_logprobs_workspace(rows, vocab, top) bytes."""
+    rows, vocab = _dim(logits, 0, "logits", 2), logits.shape[1]
+    if not getattr(logits, "is_cuda", False) or (rows and vocab > 1 and logits.stride(1) != 1):
+        raise NfError(1, "logits is not a CUDA tensor with contiguous rows")
+    dv = logits.device.index
+    _on_current(dv, "logits")
+    kind = str(logits.dtype)
+    if kind not in ("torch.float32", "torch.bfloat16"):
+        raise NfError(1, f"logits has dtype {logits.dtype}; expected float32 or bfloat16")
+    if (top_idx is None) != (top_logprob is None):
+        raise NfError(1, "top_idx and top_logprob go together")
+    top = 0 if top_idx is None else _dim(top_idx, 1, "top_idx", 2)
+    _kv_check(load().nf_token_logprobs(
+        logits.data_ptr(), DTYPE_F32 if kind == "torch.float32" else DTYPE_BF16,
+        logits.stride(0) if rows > 1 else max(1, vocab), rows, vocab, _dev(targets, rows, _I32, "targets", dv), top,
+        _dev(logprob, rows, _F32, "logprob", dv), _dev(entropy, rows, _F32, "entropy", dv),
+        _dev(top_idx, rows * top, _I32, "top_idx", dv), _dev(top_logprob, rows * top, _F32, "top_logprob", dv),
+        _dev(workspace, 0, _U8, "workspace", dv), workspace.numel(), stream or None))
+
+
+def kv_accept(caches: KvCaches, prefix, path, path_len, *, cache_seq=None, status=None, stream=0) -> None:
+    """Moves the accepted paths' cache rows up behind their prefixes in every
+    layer (nf_kv_accept): prefix, path_len and cache_seq int32 [batch], path
+    int32 [batch, max_path] of rising row numbers."""
+    dv = caches.device
+    _on_current(dv, "the cache")
+    batch, longest = _dim(path, 0, "path", 2), path.shape[1]
+    if cache_seq is None and batch > caches.caches[0].desc.seqs:
+        raise NfError(2, f"{batch} paths for a cache of {caches.caches[0].desc.seqs} sequences: pass cache_seq")
+    _kv_check(load().nf_kv_accept(
+        caches.descs, len(caches.caches), _dev(prefix, batch, _I32, "prefix", dv),
+        _dev(path, batch * longest, _I32, "path", dv), longest, _dev(path_len, batch, _I32, "path_len", dv),
+        _dev(cache_seq, batch, _I32, "cache_seq", dv), batch, _dev(status, 1, _I32, "status", dv), stream or None))
