@@ -501,8 +501,8 @@ enum { NF_DTYPE_F32 = 0, NF_DTYPE_BF16 = 1 };
 /* A layer's cache: keys and values [seqs][kv_heads][max_context][head_dim].
  * NF_KV_BF16: BF16, scales NULL.  NF_KV_E4M3: E4M3FN codes, and one F32 scale
  * per row, [seqs][kv_heads][max_context]; a row stands for code * scale.
- * head_dim 64 or 128; k and v 16-byte aligned; seqs * kv_heads and
- * max_context below 2^31. */
+ * head_dim 64 or 128; k and v 16-byte aligned; seqs * kv_heads below
+ * 2^31, max_context at most 2^30. */
 typedef struct nf_kv_cache {
     void* k;
     void* v;

@@ -866,6 +866,22 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t inner_
     return r == CUDA_SUCCESS;
 }
 
+bool make_tmap_kv(CUtensorMap* map, const void* base, bool bf16, uint64_t dim, uint64_t rows, uint64_t heads,
+                  uint32_t box_rows) {
+    PfnEncodeTiled fn = encode_fn();
+    if (!fn) return false;
+    const uint64_t row_bytes = dim * (bf16 ? 2 : 1);
+    cuuint64_t dims[3] = {dim, rows, heads};
+    cuuint64_t strides[2] = {row_bytes, row_bytes * rows};
+    cuuint32_t box[3] = {bf16 ? 64u : static_cast<cuuint32_t>(dim), box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
+                          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS;
+}
+
 bool make_tmap_blocked(CUtensorMap* map, const void* base, uint64_t bytes, uint32_t box_rows) {
     PfnEncodeTiled fn = encode_fn();
     if (!fn || bytes % (BN * 128) != 0 || box_rows == 0 || box_rows > 256) return false;

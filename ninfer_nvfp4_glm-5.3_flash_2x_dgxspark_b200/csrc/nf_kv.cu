@@ -36,7 +36,7 @@ int kv_check_cache(const nf_kv_cache* c) {
     if (c->kind != NF_KV_BF16 && c->kind != NF_KV_E4M3) return kv_fail(NF_ERR_INVALID, "unknown cache kind %d", c->kind);
     if (c->head_dim != 64 && c->head_dim != 128)
         return kv_fail(NF_ERR_UNSUPPORTED, "cache head_dim must be 64 or 128, not %d", c->head_dim);
-    if (c->seqs < 1 || c->kv_heads < 1 || c->max_context < 1 ||
+    if (c->seqs < 1 || c->kv_heads < 1 || c->max_context < 1 || c->max_context > 1 << 30 ||
         static_cast<int64_t>(c->seqs) * c->kv_heads > 0x7fffffffll)
         return kv_fail(NF_ERR_SHAPE, "cache shape [%d][%d][%d]", c->seqs, c->kv_heads, c->max_context);
     if (!c->k || !c->v) return kv_fail(NF_ERR_INVALID, "null cache pointer");

@@ -1,94 +1,1133 @@
 // nf_tree.cu -- nf_tree_attention (include/nf_moe.h): attention of a
 // sequence's new rows, one token, a chain or a tree, over its cached prefix
 // and over one another.
+//
+// The rows of a sequence and KV head are its nodes' q heads of that group, R =
+// nodes * G rows (row = node * G + head): one pass over the keys serves them
+// all.  With c = scale * log2 e, row r and key j:
+//   x = c q_r . k_j (times the key's scale),  m = running max of x,
+//   p = 2^(x - m),  l = sum p,  O = sum p v_j (times the value's scale)
+// and the result is O / l.  Parts of the keys give (m, l, O) each, and
+// O = sum O_i 2^(m_i - m), l = sum l_i 2^(m_i - m) joins them.
 #include "nf_kv.h"
 
 #include "nf_common.cuh"
+#include "nf_gemm_shared.cuh"
 #include "nf_internal.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace nf {
 
 namespace {
 
-constexpr int64_t kWorkBytes = 256;
 constexpr int kStatusBad = NF_DEVERR_BAD_TOKEN;
+constexpr int kKeys = 128;       // keys per tile
+constexpr int kTileRows = 128;   // rows per MMA tile
+constexpr int kItemRows = 256;   // rows per work item: two MMA tiles
+constexpr int kMaxCtas = 148;    // CTAs (one per SM) the workspace has parts for
+constexpr int kThreads = 512;
+constexpr int kConvWarp = 8, kTmaWarp = 12, kMmaWarp = 13, kRowWarp = 14, kScaleWarp = 15;
+constexpr int kParts = 8;        // part descriptors in flight
+constexpr int kBadRing = 16;
+constexpr float kRescale = 8.f;  // the running max may lag the true one by 2^8
 
-// One warp per (row, q head); lane l holds dims l D / 32 ...
+// What joins an item's parts: written by the CTA of its first part.
+struct JoinDesc {
+    int32_t parts;   // 0: nothing to join
+    int32_t rows;    // rows of the item
+    int32_t row0;    // its first row (node * G + head) in the sequence
+    int32_t first;   // the sequence's first row of q
+    int32_t head;    // KV head
+    int32_t pad[3];
+};
+struct Work {
+    JoinDesc* join;  // [kMaxCtas]
+    float2* ml;      // [2 kMaxCtas][kItemRows] (m, l)
+    float* acc;      // [2 kMaxCtas][kItemRows][D]
+};
+constexpr int64_t kJoinBytes = (kMaxCtas * sizeof(JoinDesc) + 255) / 256 * 256;
+constexpr int64_t kMlBytes = 2ll * kMaxCtas * kItemRows * 8;
+
+__host__ __device__ inline Work work_at(void* p) {
+    uint8_t* b = static_cast<uint8_t*>(p);
+    return Work{reinterpret_cast<JoinDesc*>(b), reinterpret_cast<float2*>(b + kJoinBytes),
+                reinterpret_cast<float*>(b + kJoinBytes + kMlBytes)};
+}
+
+struct TreeArgs {
+    const uint16_t* q;
+    uint16_t* out;
+    const int32_t* row_start;
+    const int32_t* prefix;
+    const int32_t* cache_seq;
+    const uint64_t* mask;
+    const float* k_scale;
+    const float* v_scale;
+    const void* v;  // the values once more, for the rare look at single rows
+    void* work;
+    int32_t* status;
+    int rows, nq, nkv, G, batch, seqs, L, words;
+    float c;        // scale * log2(e)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p;
+}
+// 32 lanes x 32 consecutive 32-bit columns
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem, BF16 pairs] * B[smem], K = 16 per instruction
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// MN-major operand with the 128-byte swizzle: rows of 64 elements along N,
+// 8-row groups along K 1024 bytes apart (SBO), further 64 columns `lbo` on.
+__device__ __forceinline__ uint64_t sdesc_sw128_mn(uint32_t saddr, uint32_t lbo) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr >> 4) & 0x3fffu);
+    d |= static_cast<uint64_t>(lbo >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+// ---------------------------------------------------------------------------
+// The work: every (sequence, KV head, up to 256 rows) is an item of ceil(keys
+// / 128) tiles.  An item of up to 128 rows weighs 1 a tile, one of two MMA
+// tiles 2.  The items in order (sequence, head, rows) form one line of weight,
+// which the CTAs cut into equal shares; a tile belongs to the share in which
+// it starts.  One warp walks through the parts of the CTA's share and
+// publishes them to the other roles in a ring of descriptors.
+// ---------------------------------------------------------------------------
+struct Walk {
+    // the sequence
+    int i, first, n, p0, sq, npt;
+    // the part: rows [row0, row0 + rows) of KV head g, tiles [t0, t1) of kt
+    int g, pt, t0, t1, kt, row0, rows, keys;
+    int64_t at, lo, hi;  // weight at the item's start, and the CTA's share
+    bool valid;
+
+    __device__ __forceinline__ bool pair() const { return rows > kTileRows; }
+
+    __device__ __forceinline__ void load(const TreeArgs& a) {
+        first = min(max(__ldg(a.row_start + i), 0), a.rows);
+        n = max(0, min(max(__ldg(a.row_start + i + 1), 0), a.rows) - first);
+        p0 = __ldg(a.prefix + i);
+        sq = a.cache_seq ? __ldg(a.cache_seq + i) : i;
+        npt = (n * a.G + kItemRows - 1) / kItemRows;
+    }
+    __device__ __forceinline__ bool bad(const TreeArgs& a) const {
+        return p0 < 0 || sq < 0 || sq >= a.seqs || p0 > a.L - n;
+    }
+    // shape of item pt of the sequence
+    __device__ __forceinline__ void item(const TreeArgs& a) {
+        row0 = pt * kItemRows;
+        rows = min(kItemRows, n * a.G - row0);
+        keys = p0 + (a.mask ? n : min(n, (row0 + rows - 1) / a.G + 1));
+        kt = (keys + kKeys - 1) / kKeys;
+    }
+    __device__ __forceinline__ int weight() const { return pair() ? 2 * kt : kt; }
+    // weight of the sequence's items of one head
+    __device__ __forceinline__ int64_t head_weight(const TreeArgs& a) {
+        int64_t w = 0;
+        for (pt = 0; pt < npt; ++pt) {
+            item(a);
+            w += weight();
+        }
+        return w;
+    }
+    // the part of the item at (g, pt) inside the share
+    __device__ __forceinline__ void part(const TreeArgs& a) {
+        item(a);
+        const int w = pair() ? 2 : 1;
+        const int64_t end = at + weight();
+        t0 = lo > at ? static_cast<int>((lo - at + w - 1) / w) : 0;
+        t1 = hi < end ? static_cast<int>((hi - at + w - 1) / w) : kt;
+    }
+    __device__ __forceinline__ void next(const TreeArgs& a) {
+        do {
+            at += weight();
+            if (at >= hi) {
+                valid = false;
+                return;
+            }
+            if (++pt == npt) {
+                pt = 0;
+                if (++g == a.nkv) {
+                    g = 0;
+                    do {
+                        ++i;  // at < hi <= total: there is another sequence with items
+                        load(a);
+                    } while (n == 0 || bad(a));
+                }
+            }
+            part(a);
+        } while (t0 >= t1);
+    }
+};
+
+// A part as the roles see it; rows 0 ends the share.
+struct Part {
+    int32_t z;      // cache sequence * KV heads + KV head
+    int32_t t0, t1; // its tiles
+    int32_t p0, n;  // the sequence's prefix and rows
+    int32_t first;  // the sequence's first row of q
+    int32_t row0, rows;  // the item's rows (node * G + head) of the sequence
+    int32_t g;      // KV head
+    int32_t kind;   // bit 0: holds tile 0, bit 1: holds the last tile
+    int32_t pad[2];
+};
+
+// A role's place in the parts, task by task: a tile of a part of up to 128
+// rows is one task, of a larger one two (its two MMA tiles on the same keys).
+struct Task {
+    int idx, z, t, t0, t1, p0, n, sub;
+    bool valid, pair;
+    __device__ __forceinline__ bool fresh() const { return sub == 0; }          // the first task on its keys
+    __device__ __forceinline__ bool done() const { return !pair || sub == 1; }  // the last
+    __device__ __forceinline__ bool tail() const { return (t + 1) * kKeys > p0; }  // holds keys behind the prefix
+};
+
+template <int D, bool FP8>
+struct Geo {
+    static constexpr int kStages = FP8 ? 3 : 4;         // BF16 K or V tiles
+    static constexpr int kRaw = FP8 ? 3 : 0;            // E4M3 K or V tiles as loaded
+    static constexpr int kTileBytes = kKeys * D * 2;    // also a Q tile's
+    static constexpr int kRawBytes = kKeys * D;
+    static constexpr int kHalf = kKeys * 128;           // 64 columns of a tile
+    static constexpr int kQ = 0;
+    static constexpr int kRing = 2 * kTileBytes;
+    static constexpr int kRawAt = kRing + kStages * kTileBytes;
+    static constexpr int kScaleAt = kRawAt + kRaw * kRawBytes;         // [stream][2][K | V][128] floats
+    static constexpr int kMlAt = kScaleAt + (FP8 ? 2 * 2 * 2 * kKeys * 4 : 0);  // [stream][128] (m, l)
+    static constexpr int kPartAt = kMlAt + 2 * kTileRows * 8;
+    static constexpr int kBarAt = kPartAt + kParts * static_cast<int>(sizeof(Part));
+    static constexpr int kBars = 2 + 2 + 2 * kStages + 2 + 2 * (kRaw ? kRaw : 1) + 2 + 2 + 2 + 4 + 4 + 2 * kParts + 3;
+    static constexpr int kSmem = 1024 + kBarAt + kBars * 8 + 64 + kBadRing * 4;
+};
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ CUtensorMap tmk,
+                                                                     const __grid_constant__ CUtensorMap tmv,
+                                                                     const __grid_constant__ TreeArgs a) {
+    using G_ = Geo<D, FP8>;
+    constexpr int NS = G_::kStages, NR = G_::kRaw ? G_::kRaw : 1;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bar = reinterpret_cast<uint64_t*>(sm + G_::kBarAt);
+    uint64_t* q_full = bar;                 // row warp -> MMA, per Q slot
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* kv_full = q_empty + 2;        // TMA (or the converting warps) -> MMA, per stage
+    uint64_t* kv_empty = kv_full + NS;
+    uint64_t* v_ask = kv_empty + NS;        // BF16: MMA -> cleaning warps, a tail tile of V is there
+    uint64_t* v_fixed = v_ask + 1;          // and it is clean
+    uint64_t* raw_full = v_fixed + 1;       // E4M3: TMA -> converting warps
+    uint64_t* raw_empty = raw_full + NR;
+    uint64_t* s_full = raw_empty + NR;      // per stream: scores ready
+    uint64_t* p_full = s_full + 2;          // probabilities ready
+    uint64_t* o_full = p_full + 2;          // a part's products complete
+    uint64_t* sc_full = o_full + 2;         // scales of a task, [stream][2]
+    uint64_t* sc_empty = sc_full + 4;
+    uint64_t* pt_full = sc_empty + 4;       // part descriptors
+    uint64_t* pt_empty = pt_full + kParts;
+    uint64_t* ml_in = pt_empty + kParts;    // the streams' (m, l) exchanged
+    uint64_t* ml_out = ml_in + 1;           // and both outputs read
+    uint64_t* drained = ml_out + 1;         // after a time-out: no product in flight
+    int* s_abort = reinterpret_cast<int*>(drained + 1);
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_abort + 1);
+    int* s_seq = s_abort + 2;
+    int* s_pairs = s_abort + 3;
+    int64_t* s_base = reinterpret_cast<int64_t*>(s_abort + 4);   // weight before the start sequence
+    int64_t* s_total = s_base + 1;
+    int* s_bad = reinterpret_cast<int*>(s_total + 1);            // [kBadRing] per part: a node's value is not finite
+    int64_t* s_warp = reinterpret_cast<int64_t*>(sm + G_::kMlAt);  // scratch of the scan
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&q_full[s], 1);
+            mbar_init(&q_empty[s], 1);
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_full[s], 4);
+            mbar_init(&o_full[s], 1);
+        }
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&kv_full[s], FP8 ? 4 : 1);
+            mbar_init(&kv_empty[s], 1);
+        }
+        mbar_init(v_ask, 1);
+        mbar_init(v_fixed, 4);
+        for (int s = 0; s < NR; ++s) {
+            mbar_init(&raw_full[s], 1);
+            mbar_init(&raw_empty[s], 4);
+        }
+        for (int s = 0; s < 4; ++s) {
+            mbar_init(&sc_full[s], 1);
+            mbar_init(&sc_empty[s], 4);
+        }
+        for (int s = 0; s < kParts; ++s) {
+            mbar_init(&pt_full[s], 1);
+            mbar_init(&pt_empty[s], FP8 ? 15 : 14);  // TMA, MMA, 4 + 8 warps, and the scale warp
+        }
+        mbar_init(ml_in, 8);
+        mbar_init(ml_out, 8);
+        mbar_init(drained, 1);
+        *s_abort = 0;
+        *s_pairs = 0;
+        for (int s = 0; s < kBadRing; ++s) s_bad[s] = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tmk);
+        prefetch_tensormap(&tmv);
+        work_at(a.work).join[blockIdx.x].parts = 0;
+    }
+    if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
+    __syncthreads();
+
+    // ------------------------------------------------------------------ the share
+    // every thread sums the weights of a run of sequences
+    Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
+    Walk w;
+    const int run = (a.batch + kThreads - 1) / kThreads;
+    const int i0 = min(a.batch, static_cast<int>(threadIdx.x) * run), i1 = min(a.batch, i0 + run);
+    int64_t mine = 0;
+    bool pairs = false;
+    for (w.i = i0; w.i < i1; ++w.i) {
+        w.load(a);
+        if (w.n == 0) continue;
+        if (w.bad(a)) {  // its rows become NaN
+            if (a.status) atomicCAS(a.status, 0, kStatusBad);
+            if (w.i % gridDim.x == blockIdx.x)
+                for (int64_t e = 0; e < static_cast<int64_t>(w.n) * a.nq * D; ++e)
+                    a.out[static_cast<int64_t>(w.first) * a.nq * D + e] = 0x7fc0;
+            continue;
+        }
+        mine += w.head_weight(a) * a.nkv;
+        pairs |= w.n * a.G > kTileRows;
+    }
+    if (pairs) *s_pairs = 1;
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+    }
+    if (lane == 31) s_warp[warp] = before;
+    __syncthreads();
+    int64_t total = 0, base = before - mine;
+    for (int k = 0; k < kThreads / 32; ++k) {
+        if (k < warp) base += s_warp[k];
+        total += s_warp[k];
+    }
+    const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(*s_pairs ? 2 : 1));
+    const int64_t lo = per * blockIdx.x, hi = min(total, lo + per);
+    if (mine > 0 && lo >= base && lo < base + mine) {
+        for (w.i = i0; w.i < i1; ++w.i) {
+            w.load(a);
+            if (w.n == 0 || w.bad(a)) continue;
+            const int64_t here = w.head_weight(a) * a.nkv;
+            if (lo < base + here) break;
+            base += here;
+        }
+        *s_seq = w.i;
+        *s_base = base;
+    }
+    __syncthreads();
+    const uint32_t tmem = *s_tmem;
+    volatile int* abort_flag = s_abort;
+    tc_fence_after();
+
+    // A bounded wait.  After a time-out no role waits, loads or multiplies any
+    // more, and every role leaves at its next part.
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+        if (mbar_try_wait(b, parity)) return;
+        const uint64_t start = globaltimer_ns();
+        while (!*abort_flag) {
+            if (mbar_try_wait_sleep(b, parity, 100000u)) return;
+            if (globaltimer_ns() - start > NF_WAIT_BUDGET_NS) {
+                *abort_flag = 1;
+                if (a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
+            }
+        }
+    };
+
+    // The part at k.idx; a role that has finished one hands its descriptor back.
+    auto open = [&](Task& k) {
+        const int r = k.idx % kParts;
+        wait(&pt_full[r], (k.idx / kParts) & 1u);
+        const Part& p = s_part[r];
+        k.valid = !*abort_flag && p.rows > 0;
+        k.pair = p.rows > kTileRows;
+        k.z = p.z;
+        k.t = k.t0 = p.t0;
+        k.t1 = p.t1;
+        k.p0 = p.p0;
+        k.n = p.n;
+        k.sub = 0;
+    };
+    auto begin = [&]() {
+        Task k;
+        k.idx = 0;
+        open(k);
+        return k;
+    };
+    // one task on; true when that ended a part
+    auto step = [&](Task& k) {
+        if (k.pair && k.sub == 0) {
+            k.sub = 1;
+            return false;
+        }
+        k.sub = 0;
+        if (++k.t < k.t1) return false;
+        ++k.idx;
+        open(k);
+        return true;
+    };
+    auto hand_back = [&](int idx) { mbar_arrive(&pt_empty[idx % kParts]); };
+
+    // the softmax warps take over the others' registers: 256 x 184 + 256 x 72 = 512 x 128
+    if (warp >= kConvWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (lo >= hi) {
+        // no share
+    } else if (warp == kTmaWarp) {
+        // ------------------------------------------------------------- loads
+        if (lane == 0) {
+            constexpr int N = FP8 ? NR : NS;
+            uint64_t* full = FP8 ? raw_full : kv_full;
+            uint64_t* empty = FP8 ? raw_empty : kv_empty;
+            int count = 0;
+            auto load = [&](const CUtensorMap* map, const Task& k) {
+                const int s = count % N;
+                if (count >= N) wait(&empty[s], ((count / N) & 1u) ^ 1u);
+                if (*abort_flag) return;
+                if (FP8) {
+                    mbar_arrive_expect_tx(&full[s], G_::kRawBytes);
+                    tma_load_3d(sm + G_::kRawAt + s * G_::kRawBytes, map, &full[s], 0, k.t * kKeys, k.z);
+                } else {
+                    mbar_arrive_expect_tx(&full[s], G_::kTileBytes);
+                    for (int h = 0; h < D / 64; ++h)
+                        tma_load_3d(sm + G_::kRing + s * G_::kTileBytes + h * G_::kHalf, map, &full[s], 64 * h, k.t * kKeys, k.z);
+                }
+                ++count;
+            };
+            Task k = begin(), v = k;
+            // the order in which the products take the tiles: two tiles of K ahead, then V and K in turn
+            for (int u = 0; k.valid || v.valid; ++u) {
+                if (u >= 2) {
+                    if (v.fresh()) load(&tmv, v);
+                    if (step(v)) hand_back(v.idx - 1);
+                }
+                if (k.valid) {
+                    if (k.fresh()) load(&tmk, k);
+                    step(k);
+                }
+            }
+            if (*abort_flag)  // the copies in flight land before the CTA leaves
+                for (int j = max(0, count - N); j < count; ++j) {
+                    const uint64_t t = globaltimer_ns();
+                    while (!mbar_try_wait(&full[j % N], (j / N) & 1u) && globaltimer_ns() - t < NF_WAIT_BUDGET_NS) {
+                    }
+                }
+        }
+    } else if (warp == kMmaWarp) {
+        // ---------------------------------------------------------- products
+        // Task u of the share belongs to stream u & 1.  Its scores are taken
+        // two tasks ahead, behind the product with V of the task before in the
+        // same stream, whose probabilities lie in the scores' columns.
+        const uint32_t id_s = idesc_bf16(kTileRows, kKeys), id_o = idesc_bf16(kTileRows, D) | (1u << 16);
+        const bool leader = elect_one() != 0;
+        int count = 0, k_stage = 0, v_stage = 0, q_at = 0;
+        uint32_t fixed = 0;
+        auto entry = [&]() {  // the next tile of the ring
+            const int s = count % NS;
+            wait(&kv_full[s], (count / NS) & 1u);
+            ++count;
+            return s;
+        };
+        Task k = begin(), v = k;
+        for (uint32_t u = 0; k.valid || v.valid; ++u) {
+            if (u >= 2) {
+                const uint32_t task = u - 2, s = task & 1;
+                const bool clean = !FP8 && v.fresh() && v.tail();
+                if (v.fresh()) v_stage = entry();
+                if (clean && lane == 0) mbar_arrive(v_ask);
+                wait(&p_full[s], (task >> 1) & 1u);
+                if (clean) wait(v_fixed, fixed++ & 1u);
+                tc_fence_after();
+                const bool start = v.pair ? v.t == v.t0 : v.t - v.t0 < 2;
+                const bool last = v.pair ? v.t == v.t1 - 1 : v.t >= v.t1 - 2;
+                if (leader && !*abort_flag) {
+                    const uint64_t vd = sdesc_sw128_mn(smem_u32(sm + G_::kRing + v_stage * G_::kTileBytes), G_::kHalf);
+#pragma unroll
+                    for (int j = 0; j < kKeys / 16; ++j)
+                        mma_bf16_ts(tmem + 256 + s * D, tmem + s * kKeys + j * 8, vd + j * (2048 >> 4), id_o, !(start && j == 0));
+                    if (v.done()) tc_commit(&kv_empty[v_stage]);
+                    if (last) tc_commit(&o_full[s]);
+                }
+                __syncwarp();
+                if (step(v) && lane == 0) hand_back(v.idx - 1);
+            }
+            if (k.valid) {
+                const int slot = (q_at + k.sub) & 1;
+                if (k.t == k.t0) wait(&q_full[slot], ((q_at + k.sub) >> 1) & 1u);
+                if (k.fresh()) k_stage = entry();
+                tc_fence_after();
+                const bool last = k.t == k.t1 - 1;
+                if (leader && !*abort_flag) {
+                    const uint64_t qd = sdesc_sw128(smem_u32(sm + G_::kQ + slot * G_::kTileBytes));
+                    const uint64_t kd = sdesc_sw128(smem_u32(sm + G_::kRing + k_stage * G_::kTileBytes));
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        const uint32_t off = ((j >> 2) * G_::kHalf + (j & 3) * 32) >> 4;
+                        mma_bf16(tmem + (u & 1) * kKeys, qd + off, kd + off, id_s, j != 0);
+                    }
+                    tc_commit(&s_full[u & 1]);
+                    if (k.done()) tc_commit(&kv_empty[k_stage]);
+                    if (last) tc_commit(&q_empty[slot]);
+                }
+                __syncwarp();
+                if (last && k.done()) q_at += k.pair ? 2 : 1;
+                step(k);
+            }
+        }
+        if (*abort_flag && leader) {
+            tc_commit(drained);
+            const uint64_t t = globaltimer_ns();
+            while (!mbar_try_wait(drained, 0) && globaltimer_ns() - t < NF_WAIT_BUDGET_NS) {
+            }
+        }
+    } else if (warp == kRowWarp) {
+        // ----------------------- the walk, and q's rows into swizzled tiles
+        w.valid = true;
+        w.i = *s_seq;
+        w.at = *s_base;
+        w.lo = lo;
+        w.hi = hi;
+        w.load(a);
+        const int64_t head = w.head_weight(a);
+        w.g = static_cast<int>((lo - w.at) / head);
+        w.at += w.g * head;
+        w.pt = 0;
+        w.item(a);
+        while (w.at + w.weight() <= lo) {
+            w.at += w.weight();
+            ++w.pt;
+            w.item(a);
+        }
+        w.part(a);
+        if (w.t0 >= w.t1) w.next(a);
+        int at = 0;
+        for (int idx = 0;; ++idx) {
+            const int r = idx % kParts;
+            if (idx >= kParts) wait(&pt_empty[r], ((idx / kParts) & 1u) ^ 1u);
+            if (lane == 0) {
+                Part p{};
+                if (w.valid) {
+                    p.z = w.sq * a.nkv + w.g;
+                    p.t0 = w.t0;
+                    p.t1 = w.t1;
+                    p.p0 = w.p0;
+                    p.n = w.n;
+                    p.first = w.first;
+                    p.row0 = w.row0;
+                    p.rows = w.rows;
+                    p.g = w.g;
+                    p.kind = (w.t0 == 0) | (w.t1 == w.kt) << 1;
+                    if (p.kind == 1) {  // other CTAs hold the rest: how many parts there are to join
+                        JoinDesc d{};
+                        d.parts = static_cast<int>((w.at + static_cast<int64_t>(w.kt - 1) * (w.pair() ? 2 : 1)) / per) -
+                                  static_cast<int>(blockIdx.x) + 1;
+                        d.rows = w.rows;
+                        d.row0 = w.row0;
+                        d.first = w.first;
+                        d.head = w.g;
+                        work_at(a.work).join[blockIdx.x] = d;
+                    }
+                }
+                s_part[r] = p;
+                mbar_arrive(&pt_full[r]);
+            }
+            __syncwarp();
+            if (!w.valid || *abort_flag) break;
+            for (int sub = 0; sub < (w.pair() ? 2 : 1); ++sub, ++at) {
+                const int slot = at & 1;
+                if (at >= 2) wait(&q_empty[slot], ((at >> 1) & 1u) ^ 1u);
+                const uint32_t dst = smem_u32(sm + G_::kQ + slot * G_::kTileBytes);
+                const int rows = min(kTileRows, w.rows - sub * kTileRows);
+                constexpr int C = D / 8;  // 16-byte chunks of a row
+                for (int e = lane; e < rows * C; e += 32) {
+                    const int r = e / C, ch = e % C, row = w.row0 + sub * kTileRows + r;
+                    const uint16_t* src =
+                        a.q + (static_cast<int64_t>(w.first + row / a.G) * a.nq + w.g * a.G + row % a.G) * D + ch * 8;
+                    const uint32_t to = dst + (ch >> 3) * G_::kHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+                }
+                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[slot]);
+            }
+            w.next(a);
+        }
+    } else if (warp == kScaleWarp) {
+        // ------------------- E4M3: a task's 128 key scales (times c) and value scales
+        if (FP8) {
+            Task k = begin();
+            float ks[4], vs[4];
+            auto fetch = [&]() {
+                const int64_t row = static_cast<int64_t>(k.z) * a.L;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = k.t * kKeys + 32 * e + lane;
+                    const bool in = key < k.p0 + k.n;
+                    ks[e] = in ? __ldg(a.k_scale + row + key) : 0.f;
+                    vs[e] = in ? __ldg(a.v_scale + row + key) : 0.f;
+                }
+            };
+            if (k.valid) fetch();
+            for (uint32_t u = 0; k.valid; ++u) {
+                const uint32_t s = u & 1, b = (u >> 1) & 1, at = 2 * s + b;
+                if (u >= 4) wait(&sc_empty[at], ((u >> 2) & 1u) ^ 1u);
+                float* dst = reinterpret_cast<float*>(sm + G_::kScaleAt) + at * 2 * kKeys;
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    dst[32 * e + lane] = ks[e] * a.c;
+                    if (k.t * kKeys + 32 * e + lane >= k.p0 && !isfinite(vs[e])) {
+                        bad = true;
+                        vs[e] = 0.f;
+                    }
+                    dst[kKeys + 32 * e + lane] = vs[e];
+                }
+                if (bad) s_bad[k.idx % kBadRing] = 1;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_full[at]);
+                if (step(k) && lane == 0) hand_back(k.idx - 1);
+                if (k.valid) fetch();
+            }
+        }
+    } else {
+        // E4M3: every tile to BF16.  BF16: the tail tiles of V, whose keys
+        // behind the sequence's rows, and whose nodes' values that are not
+        // finite, become zero (a zero probability must not meet a NaN).
+        const int tid = threadIdx.x - kConvWarp * 32;
+        int count = 0;
+        uint32_t asked = 0;
+        auto entry = [&](const Task& k, bool is_v) {
+            const bool tail = k.tail();
+            const int end = k.p0 + k.n - k.t * kKeys, node = k.p0 - k.t * kKeys;  // in keys of the tile
+            const int s = count % NS;
+            uint8_t* dst = sm + G_::kRing + s * G_::kTileBytes;
+            if (FP8) {
+                const int r = count % NR;
+                wait(&raw_full[r], (count / NR) & 1u);
+                if (count >= NS) wait(&kv_empty[s], ((count / NS) & 1u) ^ 1u);
+                const uint8_t* src = sm + G_::kRawAt + r * G_::kRawBytes;
+                constexpr int C = D / 16;  // 16-byte chunks of a raw row
+                bool bad = false;
+                uint32_t nan = 0;
+                // chunk e of the raw tile (16 codes) to chunks 2 ch and 2 ch + 1 of its row; the upper half's threads
+                // store the second first, so that eight threads' stores lie in eight bank groups
+                auto put = [&](int e, const uint32_t* y) {
+                    const int row = e / C, ch = e % C, flip = (ch >> 2) & 1;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int col = 2 * ch + (j ^ flip);
+                        const bool up = (j ^ flip) != 0;
+                        *reinterpret_cast<uint4*>(dst + (col >> 3) * G_::kHalf + row * 128 + (((col & 7) ^ (row & 7)) << 4)) =
+                            up ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                };
+                // sign and the 7 exponent and mantissa bits in a BF16's places are the code times 2^-120, subnormal
+                // codes too
+                auto widen = [&](const uint4& x, uint32_t* y) {
+                    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t b = __byte_perm(in[j], 0u, h ? 0x3424 : 0x1404);
+                            const uint32_t t = ((b >> 4) & 0x07f007f0u) | (b & 0x80008000u);
+                            asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y[2 * j + h]) : "r"(t), "r"(0x7b807b80u));  // 2^120
+                        }
+                        nan |= (in[j] & 0x7f7f7f7fu) + 0x01010101u;  // a code 0x7f carries into the sign's place
+                    }
+                };
+#pragma unroll
+                for (int b = 0; b < C; b += 4) {
+                    uint4 x[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4*>(src + ((b + j) * 128 + tid) * 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t y[8];
+                        widen(x[j], y);
+                        put((b + j) * 128 + tid, y);
+                    }
+                }
+                if ((nan & 0x80808080u) != 0 || (is_v && tail)) {
+                    // rare: once more, with NaN codes as NaN, and V's rows behind the sequence and NaN nodes as zeros
+#pragma unroll 1
+                    for (int e = tid; e < C * 128; e += 128) {
+                        const int row = e / C;
+                        const uint4 x = *reinterpret_cast<const uint4*>(src + e * 16);
+                        uint32_t y[8];
+                        nan = 0;
+                        widen(x, y);
+                        const bool node_row = is_v && row >= node && row < end;
+                        const bool zero = (is_v && row >= end) || (node_row && (nan & 0x80808080u));
+                        bad |= node_row && zero;
+                        if (!zero && !(nan & 0x80808080u)) continue;
+                        const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t c2 = in[j >> 1] >> (16 * (j & 1));
+                            if ((c2 & 0x7fu) == 0x7fu) y[j] = (y[j] & 0xffff0000u) | 0x7fc0u;
+                            if ((c2 & 0x7f00u) == 0x7f00u) y[j] = (y[j] & 0xffffu) | 0x7fc00000u;
+                            if (zero) y[j] = 0u;
+                        }
+                        put(e, y);
+                    }
+                }
+                if (bad) s_bad[k.idx % kBadRing] = 1;
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&raw_empty[r]);
+                    mbar_arrive(&kv_full[s]);
+                }
+            } else if (is_v && tail) {
+                wait(v_ask, asked++ & 1u);
+                const int row = tid;
+                bool zero = row >= end;
+                if (row >= node && row < end) {
+                    uint32_t inf = 0;
+#pragma unroll
+                    for (int ch = 0; ch < D / 8; ++ch) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(dst + (ch >> 3) * G_::kHalf + row * 128 +
+                                                                        (((ch & 7) ^ (row & 7)) << 4));
+                        const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)  // an exponent of all ones carries into the sign's place
+                            inf |= ((in[j] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                    }
+                    if (inf) {
+                        zero = true;
+                        s_bad[k.idx % kBadRing] = 1;
+                    }
+                }
+                if (zero)
+#pragma unroll
+                    for (int ch = 0; ch < D / 8; ++ch)
+                        *reinterpret_cast<uint4*>(dst + (ch >> 3) * G_::kHalf + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_fixed);
+            }
+            ++count;
+        };
+        Task k = begin(), v = k;
+        for (int u = 0; k.valid || v.valid; ++u) {
+            if (u >= 2) {
+                if (v.fresh()) entry(v, true);
+                if (step(v) && lane == 0) hand_back(v.idx - 1);
+            }
+            if (k.valid) {
+                if (k.fresh()) entry(k, false);
+                step(k);
+            }
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        // ------------------------------------------- softmax of stream s
+        const int s = warp >> 2, r = threadIdx.x & 127;  // the thread's row of the MMA tile
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+        const uint32_t t_s = tmem + s * kKeys + lanes, t_o = tmem + 256 + s * D + lanes;
+        float2* s_ml = reinterpret_cast<float2*>(sm + G_::kMlAt);
+        uint32_t u0 = 0, mine_n = 0, o_n = 0, ml_n = 0;  // tasks before the part; this stream's tasks and parts; exchanges
+        for (int idx = 0; lo < hi; ++idx) {
+            wait(&pt_full[idx % kParts], (idx / kParts) & 1u);
+            const Part& w = s_part[idx % kParts];
+            if (*abort_flag || w.rows == 0) break;
+            const int p0 = w.p0, n = w.n, t1 = w.t1;
+            const bool pair = w.rows > kTileRows;
+            const int mine0 = static_cast<int>((s ^ u0) & 1);  // pair: which MMA tile; else: the first tile's offset
+            const int row0 = pair ? mine0 * kTileRows : 0;      // first row of the stream in the item
+            const int rows = min(kTileRows, w.rows - row0);
+            const bool active = (warp & 3) * 32 < rows;
+            const int row = w.row0 + row0 + r, node = row / a.G;
+            float m = -INFINITY, l = 0.f;
+            int done = 0;
+            for (int t = w.t0 + (pair ? 0 : mine0); t < t1; t += pair ? 1 : 2, ++mine_n, ++done) {
+                const uint32_t b = mine_n & 1;
+                const float* sc = reinterpret_cast<const float*>(sm + G_::kScaleAt) + (2 * s + b) * 2 * kKeys;
+                wait(&s_full[s], mine_n & 1u);
+                if (FP8) wait(&sc_full[2 * s + b], (mine_n >> 1) & 1u);
+                __syncwarp();
+                if (active) {
+                    tc_fence_after();
+                    const bool tail = (t + 1) * kKeys > p0;
+                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    if (tail) {
+                        const int j0 = t * kKeys - p0;  // node of the tile's first key
+                        auto low = [](int k) { return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u; };
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int j = j0 + 32 * c;
+                            if (!a.mask) {
+                                vis[c] = low(min(n, node + 1) - j);
+                                continue;
+                            }
+                            uint64_t bits = 0;
+                            if (j > -32 && r < rows) {
+                                const uint64_t* mw = a.mask + static_cast<int64_t>(w.first + node) * a.words;
+                                const int wi = j >> 6, sh = j & 63;
+                                if (wi >= 0 && wi < a.words) bits = __ldg(reinterpret_cast<const unsigned long long*>(mw + wi)) >> sh;
+                                if (sh > 32 && wi + 1 >= 0 && wi + 1 < a.words)
+                                    bits |= __ldg(reinterpret_cast<const unsigned long long*>(mw + wi + 1)) << (64 - sh);
+                            }
+                            vis[c] = (static_cast<uint32_t>(bits) & low(n - j)) | low(-j);
+                        }
+                    }
+                    // x = S * factor: the whole row of the tile in registers
+                    float x[kKeys];
+                    uint32_t* xb = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, xb + 32 * c);
+                    tmem_wait_ld();
+                    const uint64_t c2 = f32x2_pack(a.c, a.c);
+#pragma unroll
+                    for (int j = 0; j < kKeys; j += 4) {
+                        uint64_t f0 = c2, f1 = c2;
+                        if (FP8) {
+                            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + j);
+                            f0 = f.x;
+                            f1 = f.y;
+                        }
+                        const uint64_t y0 = mul_f32x2(f32x2_pack(x[j], x[j + 1]), f0);
+                        const uint64_t y1 = mul_f32x2(f32x2_pack(x[j + 2], x[j + 3]), f1);
+                        x[j] = f32x2_lo(y0);
+                        x[j + 1] = f32x2_hi(y0);
+                        x[j + 2] = f32x2_lo(y1);
+                        x[j + 3] = f32x2_hi(y1);
+                    }
+                    if (tail)
+#pragma unroll
+                        for (int j = 0; j < kKeys; ++j) x[j] = (vis[j >> 5] >> (j & 31)) & 1 ? x[j] : -INFINITY;
+                    float mx4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int j = 4; j < kKeys - 4; j += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], x[j + 2 * e], x[j + 2 * e + 1]);
+                    const float mx = fmaxf(max3(max3(mx4[0], x[kKeys - 4], x[kKeys - 3]), mx4[1], mx4[2]),
+                                           max3(mx4[3], x[kKeys - 2], x[kKeys - 1]));
+                    if (__any_sync(0xffffffffu, done == 0 || mx > m + kRescale)) {
+                        const float mn = fmaxf(m, mx);
+                        const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+                        if (done > 0) {
+                            // the products up to the previous task are complete: the scores' commit covers them
+#pragma unroll 1
+                            for (int c = 0; c < D / 16; ++c) {
+                                uint32_t v[16];
+                                tmem_ld16(t_o + 16 * c, v);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
+                                tmem_st16(t_o + 16 * c, v);
+                            }
+                            l *= f;
+                        }
+                        m = mn;
+                    }
+                    const float mu = m == -INFINITY ? 0.f : m;
+                    const uint64_t nm = f32x2_pack(-mu, -mu);
+                    uint64_t sum = 0, sum1 = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int j = 32 * c; j < 32 * c + 32; j += 4) {
+                            const uint64_t y0 = add_f32x2(f32x2_pack(x[j], x[j + 1]), nm);
+                            const uint64_t y1 = add_f32x2(f32x2_pack(x[j + 2], x[j + 3]), nm);
+                            uint64_t p0 = f32x2_pack(ex2(f32x2_lo(y0)), ex2(f32x2_hi(y0)));
+                            uint64_t p1 = f32x2_pack(ex2(f32x2_lo(y1)), ex2(f32x2_hi(y1)));
+                            sum = add_f32x2(sum, p0);
+                            sum1 = add_f32x2(sum1, p1);
+                            if (FP8) {
+                                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + kKeys + j);
+                                p0 = mul_f32x2(p0, f.x);
+                                p1 = mul_f32x2(p1, f.y);
+                            }
+                            pk[(j & 31) >> 1] = bf16x2_hw(f32x2_lo(p0), f32x2_hi(p0));
+                            pk[((j & 31) >> 1) + 1] = bf16x2_hw(f32x2_lo(p1), f32x2_hi(p1));
+                        }
+                        tmem_st16(t_s + 16 * c, pk);
+                    }
+                    sum = add_f32x2(sum, sum1);
+                    l += f32x2_lo(sum) + f32x2_hi(sum);
+                    tmem_wait_st();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&p_full[s]);
+                    if (FP8) mbar_arrive(&sc_empty[2 * s + b]);
+                }
+            }
+            // ------------------------------------------------ the part's end
+            if (done > 0) {
+                wait(&o_full[s], o_n & 1u);
+                ++o_n;
+                __syncwarp();
+                tc_fence_after();
+            }
+            if (s_bad[idx % kBadRing] != 0 && r < rows) {
+                // some node's value is not finite: a row that sees one is NaN
+                const int64_t base_row = static_cast<int64_t>(w.z) * a.L + p0;
+                for (int j = 0; j < n; ++j) {
+                    if (a.mask ? j >= 64 * a.words || !((a.mask[static_cast<int64_t>(w.first + node) * a.words + (j >> 6)] >> (j & 63)) & 1)
+                               : j > node)
+                        continue;
+                    bool bad = FP8 && !isfinite(a.v_scale[base_row + j]);
+                    for (int d = 0; d < D; ++d)
+                        bad |= FP8 ? (static_cast<const uint8_t*>(a.v)[(base_row + j) * D + d] & 0x7f) == 0x7f
+                                   : (static_cast<const uint16_t*>(a.v)[(base_row + j) * D + d] & 0x7f80) == 0x7f80;
+                    if (bad) l = NAN;
+                }
+            }
+            __syncwarp();
+            const bool whole = w.kind == 3;
+            const int slot = 2 * blockIdx.x + (w.kind & 1), cnt = t1 - w.t0;
+            const Work wk = work_at(a.work);
+            float other_m = -INFINITY, other_l = 0.f;
+            if (!pair) {
+                // both streams hold parts of the same rows: exchange (m, l), then each finishes half of the columns
+                s_ml[s * kTileRows + r] = make_float2(m, l);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ml_in);
+                wait(ml_in, ml_n & 1u);
+                __syncwarp();
+                const float2 o = s_ml[(s ^ 1) * kTileRows + r];
+                other_m = o.x;
+                other_l = o.y;
+            }
+            if (active) {
+                const float mt = fmaxf(m, other_m), mu = mt == -INFINITY ? 0.f : mt;
+                const float f0 = m == -INFINITY ? 0.f : ex2(m - mu), f1 = other_m == -INFINITY ? 0.f : ex2(other_m - mu);
+                const float lt = l * f0 + other_l * f1;
+                const bool use0 = done > 0, use1 = !pair && cnt - done > 0;
+                const float inv = lt == 0.f ? 0.f : 1.f / lt;
+                const uint32_t t_other = tmem + 256 + (s ^ 1) * D + lanes;
+                const int irow = row0 + r;  // the thread's row in the item
+                uint16_t* dst = a.out + (static_cast<int64_t>(w.first + node) * a.nq + w.g * a.G + (row - node * a.G)) * D;
+                float* part_o = wk.acc + (static_cast<int64_t>(slot) * kItemRows + irow) * D;
+                for (int c = (pair ? 0 : s * D / 64); c < (pair ? D / 32 : (s + 1) * D / 64); ++c) {
+                    uint32_t v[32];
+                    float o[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = 0.f;
+                    if (use0) {
+                        tmem_ld32(t_o + 32 * c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(v[j]) * f0;
+                    }
+                    if (use1) {
+                        tmem_ld32(t_other + 32 * c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(v[j]), f1, o[j]);
+                    }
+                    if (r < rows) {
+                        if (whole) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) v[j] = bf16x2_hw(o[2 * j] * inv, o[2 * j + 1] * inv);
+#pragma unroll
+                            for (int j = 0; j < 16; j += 4)
+                                *reinterpret_cast<uint4*>(dst + 32 * c + 2 * j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4)
+                                *reinterpret_cast<float4*>(part_o + 32 * c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        }
+                    }
+                }
+                if (!whole && r < rows && (pair || s == 0)) wk.ml[static_cast<int64_t>(slot) * kItemRows + irow] = make_float2(mu, lt);
+            }
+            __syncwarp();
+            tc_fence_before();
+            if (!pair) {  // no product into the streams' outputs before both have read them
+                if (lane == 0) mbar_arrive(ml_out);
+                wait(ml_out, ml_n++ & 1u);
+            }
+            if (r == 0) s_bad[(idx + kBadRing / 2) % kBadRing] = 0;
+            u0 += pair ? 2 * cnt : cnt;
+            __syncwarp();
+            if (lane == 0) hand_back(idx);
+        }
+    }
+    __syncwarp();
+    pdl_trigger();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of items that several CTAs computed, in their order: one
+// warp per row.
 template <int D>
-__global__ void __launch_bounds__(128) tree_attention_kernel(const __grid_constant__ nf_kv_cache c,
-                                                             const uint16_t* __restrict__ q, int rows, int nq,
-                                                             const int32_t* __restrict__ row_start, int batch,
-                                                             const int32_t* __restrict__ prefix,
-                                                             const int32_t* __restrict__ cache_seq,
-                                                             const uint64_t* __restrict__ mask, int words, float scale,
-                                                             uint16_t* __restrict__ out, int32_t* __restrict__ status) {
-    constexpr int E = D / 32;
+__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a) {
+    pdl_wait();
+    const Work wk = work_at(a.work);
+    const int b = blockIdx.x;
+    const JoinDesc d = wk.join[b];
+    if (d.parts == 0) return;
     const int lane = threadIdx.x & 31;
-    const int64_t gw = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (gw >= static_cast<int64_t>(rows) * nq) return;
-    const int r = static_cast<int>(gw / nq), h = static_cast<int>(gw % nq), g = h / (nq / c.kv_heads);
-    // the last sequence that starts at or before row r
-    int i = -1;
-    for (int a = 0; a < batch; ++a)
-        if (r >= row_start[a] && r < row_start[a + 1]) i = a;
-    if (i < 0) return;
-    const int r0 = max(0, row_start[i]), n = min(rows, row_start[i + 1]) - r0;
-    const int p0 = prefix[i], sq = cache_seq ? cache_seq[i] : i;
-    uint16_t* o = out + gw * D + lane * E;
-    if (p0 < 0 || sq < 0 || sq >= c.seqs || n > c.max_context - p0) {
-        if (lane == 0 && status) atomicCAS(status, 0, kStatusBad);
-        for (int e = 0; e < E; ++e) o[e] = 0x7fc0;
-        return;
-    }
-    float qr[E], acc[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; ++e) {
-        qr[e] = bf16_bits_to_f32(q[gw * D + lane * E + e]) * scale;
-        acc[e] = 0.f;
-    }
-    const int64_t base = (static_cast<int64_t>(sq) * c.kv_heads + g) * c.max_context;
-    for (int j = 0; j < p0 + n; ++j) {
-        if (j >= p0) {
-            const int node = j - p0;
-            if (mask ? node >= 64 * words || !((mask[static_cast<int64_t>(r) * words + (node >> 6)] >> (node & 63)) & 1)
-                     : node > r - r0)
-                continue;
+    constexpr int E = D / 32;
+    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < d.rows; r += gridDim.y * 8) {
+        // part 0 lies in slot 2 b + 1, part i > 0 in slot 2 (b + i)
+        auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * b + 1 : 2 * (b + i)) * kItemRows + r; };
+        float m = -INFINITY;
+        bool any = false;
+        for (int i = lane; i < d.parts; i += 32) {
+            const float2 v = wk.ml[slot(i)];
+            if (v.y != 0.f) {  // a part in which the row sees a key
+                m = fmaxf(m, v.x);
+                any = true;
+            }
         }
-        const int64_t at = (base + j) * D + lane * E;
-        float s = 0.f, kf[E], vf[E], vs = 1.f;
-        for (int e = 0; e < E; ++e) {
-            kf[e] = c.kind == NF_KV_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(c.k)[at + e])
-                                         : e4m3_to_f32(static_cast<const uint8_t*>(c.k)[at + e]);
-            vf[e] = c.kind == NF_KV_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(c.v)[at + e])
-                                         : e4m3_to_f32(static_cast<const uint8_t*>(c.v)[at + e]);
-            s = __fmaf_rn(qr[e], kf[e], s);
-        }
-        for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-        if (c.kind == NF_KV_E4M3) {
-            s *= c.k_scale[base + j];
-            vs = c.v_scale[base + j];
-        }
-        const float mn = fmaxf(m, s), corr = m == -INFINITY ? 0.f : expf(m - mn), pr = expf(s - mn);
-        m = mn;
-        l = l * corr + pr;
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * corr + pr * (vf[e] * vs);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        any = __any_sync(0xffffffffu, any);
+        float l = 0.f, acc[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+        if (any)
+#pragma unroll 4
+            for (int i = 0; i < d.parts; ++i) {
+                const float2 v = wk.ml[slot(i)];
+                const float f = v.y != 0.f ? ex2(v.x - m) : 0.f;
+                const float* p = wk.acc + slot(i) * D + lane * E;
+                l += v.y * f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += f == 0.f ? 0.f : p[e] * f;
+            }
+        const int row = d.row0 + r;
+        uint16_t* dst = a.out + (static_cast<int64_t>(d.first + row / a.G) * a.nq + d.head * a.G + row % a.G) * D + lane * E;
+        const float inv = any ? 1.f / l : 0.f;
+        if (E == 4)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(bf16x2_hw(acc[0] * inv, acc[1] * inv), bf16x2_hw(acc[E - 2] * inv, acc[E - 1] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(dst) = bf16x2_hw(acc[0] * inv, acc[1] * inv);
     }
-    for (int e = 0; e < E; ++e) o[e] = f32_to_bf16_bits(l == 0.f ? 0.f : acc[e] / l);
+}
+
+template <int D, bool FP8>
+cudaError_t launch(const nf_kv_cache& c, const TreeArgs& a, cudaStream_t st) {
+    CUtensorMap tmk, tmv;
+    const uint64_t heads = static_cast<uint64_t>(c.seqs) * c.kv_heads;
+    if (!make_tmap_kv(&tmk, c.k, !FP8, D, c.max_context, heads, kKeys) ||
+        !make_tmap_kv(&tmv, c.v, !FP8, D, c.max_context, heads, kKeys))
+        return cudaErrorInvalidValue;
+    static bool attr[kMaxDevices] = {};
+    static int sms[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    constexpr int smem = Geo<D, FP8>::kSmem;
+    if (!attr[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        sms[dev] = gemm_grid_size(dev);
+        attr[dev] = true;
+    }
+    const int grid = std::min(kMaxCtas, sms[dev]);
+    tree_attention_kernel<D, FP8><<<grid, kThreads, smem, st>>>(tmk, tmv, a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_dependent(tree_join_kernel<D>, dim3(grid, 4), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
 cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int rows, int q_heads,
                                   const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* cache_seq,
-                                  const uint64_t* mask, int mask_words, float scale, uint16_t* out, void*,
+                                  const uint64_t* mask, int mask_words, float scale, uint16_t* out, void* work,
                                   int32_t* status, cudaStream_t st) {
     if (rows <= 0 || batch <= 0) return cudaSuccess;
-    const int64_t warps = static_cast<int64_t>(rows) * q_heads;
-    auto kernel = c.head_dim == 128 ? tree_attention_kernel<128> : tree_attention_kernel<64>;
-    kernel<<<static_cast<unsigned>((warps + 3) / 4), 128, 0, st>>>(c, q, rows, q_heads, row_start, batch, prefix,
-                                                                   cache_seq, mask, mask_words, scale, out, status);
-    return cudaGetLastError();
+    TreeArgs a{};
+    a.q = q;
+    a.out = out;
+    a.row_start = row_start;
+    a.prefix = prefix;
+    a.cache_seq = cache_seq;
+    a.mask = mask;
+    a.k_scale = c.k_scale;
+    a.v_scale = c.v_scale;
+    a.v = c.v;
+    a.work = work;
+    a.status = status;
+    a.rows = rows;
+    a.nq = q_heads;
+    a.nkv = c.kv_heads;
+    a.G = q_heads / c.kv_heads;
+    a.batch = batch;
+    a.seqs = c.seqs;
+    a.L = c.max_context;
+    a.words = mask_words;
+    a.c = scale * 1.4426950408889634f;
+    const bool fp8 = c.kind == NF_KV_E4M3;
+    if (c.head_dim == 128) return fp8 ? launch<128, true>(c, a, st) : launch<128, false>(c, a, st);
+    return fp8 ? launch<64, true>(c, a, st) : launch<64, false>(c, a, st);
 }
 
 }  // namespace nf
@@ -97,7 +1136,10 @@ using namespace nf;
 
 extern "C" {
 
-int64_t nf_tree_attention_workspace(int head_dim) { return head_dim == 64 || head_dim == 128 ? kWorkBytes : 0; }
+int64_t nf_tree_attention_workspace(int head_dim) {
+    if (head_dim != 64 && head_dim != 128) return 0;
+    return kJoinBytes + kMlBytes + 2ll * kMaxCtas * kItemRows * head_dim * 4;
+}
 
 int nf_tree_attention(const nf_kv_cache* cache, const uint16_t* q, int rows, int q_heads, const int32_t* row_start,
                       int batch, const int32_t* prefix, const int32_t* cache_seq, const uint64_t* mask, int mask_words,
