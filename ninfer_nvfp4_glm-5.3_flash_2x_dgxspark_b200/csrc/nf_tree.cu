@@ -31,6 +31,7 @@ constexpr int kThreads = 512;
 constexpr int kConvWarp = 8, kTmaWarp = 12, kMmaWarp = 13, kRowWarp = 14, kScaleWarp = 15;
 constexpr int kParts = 8;        // part descriptors in flight
 constexpr int kBadRing = 16;
+constexpr uint64_t kWaitNs = 10000000000ull;  // a row tile's wait can last as long as a whole part
 constexpr float kRescale = 8.f;  // the running max may lag the true one by 2^8
 
 // What joins an item's parts: written by the CTA of its first part.
@@ -76,11 +77,6 @@ __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
 }
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
     uint64_t d;
@@ -178,39 +174,41 @@ struct Walk {
     // weight of the sequence's items of one head
     __device__ __forceinline__ int64_t head_weight(const TreeArgs& a) {
         int64_t w = 0;
+#pragma unroll 1
         for (pt = 0; pt < npt; ++pt) {
             item(a);
             w += weight();
         }
         return w;
     }
-    // the part of the item at (g, pt) inside the share
-    __device__ __forceinline__ void part(const TreeArgs& a) {
-        item(a);
-        const int w = pair() ? 2 : 1;
-        const int64_t end = at + weight();
-        t0 = lo > at ? static_cast<int>((lo - at + w - 1) / w) : 0;
-        t1 = hi < end ? static_cast<int>((hi - at + w - 1) / w) : kt;
-    }
-    __device__ __forceinline__ void next(const TreeArgs& a) {
-        do {
-            at += weight();
-            if (at >= hi) {
-                valid = false;
-                return;
-            }
-            if (++pt == npt) {
-                pt = 0;
-                if (++g == a.nkv) {
-                    g = 0;
-                    do {
-                        ++i;  // at < hi <= total: there is another sequence with items
-                        load(a);
-                    } while (n == 0 || bad(a));
+    // from the item (g, pt) at weight `at` to the first part inside the share, that item's own among them if `here`
+    __device__ __forceinline__ void seek(const TreeArgs& a, bool here) {
+#pragma unroll 1
+        for (;; here = false) {
+            if (!here) {
+                at += weight();
+                if (at >= hi) {
+                    valid = false;
+                    return;
+                }
+                if (++pt == npt) {
+                    pt = 0;
+                    if (++g == a.nkv) {
+                        g = 0;
+#pragma unroll 1
+                        do {
+                            ++i;  // at < hi <= total: there is another sequence with items
+                            load(a);
+                        } while (n == 0 || bad(a));
+                    }
                 }
             }
-            part(a);
-        } while (t0 >= t1);
+            item(a);
+            const int two = pair() ? 1 : 0;  // tile t starts at weight at + (t << two)
+            t0 = lo > at ? static_cast<int>(min(static_cast<int64_t>(kt), (lo - at + two) >> two)) : 0;
+            t1 = static_cast<int>(min(static_cast<int64_t>(kt), (hi - at + two) >> two));
+            if (t0 < t1) return;
+        }
     }
 };
 
@@ -229,12 +227,28 @@ struct Part {
 // A role's place in the parts, task by task: a tile of a part of up to 128
 // rows is one task, of a larger one two (its two MMA tiles on the same keys).
 struct Task {
-    int idx, z, t, t0, t1, p0, n, sub;
-    bool valid, pair;
-    __device__ __forceinline__ bool fresh() const { return sub == 0; }          // the first task on its keys
-    __device__ __forceinline__ bool done() const { return !pair || sub == 1; }  // the last
+    int idx = -1, z = 0, t = 0, t0 = 0, t1 = 0, p0 = 0, n = 0, sub = 0;
+    bool valid = false, pair = false;
+    __device__ __forceinline__ bool fresh() const { return sub == 0; }             // the first task on its keys
+    __device__ __forceinline__ bool done() const { return !pair || sub == 1; }     // the last
+    __device__ __forceinline__ bool ends() const { return t == t1 - 1 && done(); }  // the part's last
     __device__ __forceinline__ bool tail() const { return (t + 1) * kKeys > p0; }  // holds keys behind the prefix
+    __device__ __forceinline__ void next() {
+        if (pair && sub == 0) {
+            sub = 1;
+        } else {
+            sub = 0;
+            ++t;
+        }
+    }
 };
+// What the converting (or cleaning) warps need of a tile.
+struct TileInfo {
+    int32_t what;       // kTileK, kTileV, kTileVTail, or kTileEnd: no more; BF16: the stage, or -1
+    int32_t node, end;  // first key behind the prefix, and behind the sequence's rows, in keys of the tile
+    int32_t idx;        // its part
+};
+enum : int { kTileK = 0, kTileV = 1, kTileVTail = 2, kTileEnd = 3 };
 
 template <int D, bool FP8>
 struct Geo {
@@ -249,7 +263,8 @@ struct Geo {
     static constexpr int kScaleAt = kRawAt + kRaw * kRawBytes;         // [stream][2][K | V][128] floats
     static constexpr int kMlAt = kScaleAt + (FP8 ? 2 * 2 * 2 * kKeys * 4 : 0);  // [stream][128] (m, l)
     static constexpr int kPartAt = kMlAt + 2 * kTileRows * 8;
-    static constexpr int kBarAt = kPartAt + kParts * static_cast<int>(sizeof(Part));
+    static constexpr int kInfoAt = kPartAt + kParts * static_cast<int>(sizeof(Part));
+    static constexpr int kBarAt = kInfoAt + 4 * static_cast<int>(sizeof(TileInfo));
     static constexpr int kBars = 2 + 2 + 2 * kStages + 2 + 2 * (kRaw ? kRaw : 1) + 2 + 2 + 2 + 4 + 4 + 2 * kParts + 3;
     static constexpr int kSmem = 1024 + kBarAt + kBars * 8 + 64 + kBadRing * 4;
 };
@@ -286,8 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     int* s_seq = s_abort + 2;
     int* s_pairs = s_abort + 3;
     int64_t* s_base = reinterpret_cast<int64_t*>(s_abort + 4);   // weight before the start sequence
-    int64_t* s_total = s_base + 1;
-    int* s_bad = reinterpret_cast<int*>(s_total + 1);            // [kBadRing] per part: a node's value is not finite
+    int64_t* s_head = s_base + 1;                                // weight of one of its heads
+    int* s_bad = reinterpret_cast<int*>(s_head + 1);            // [kBadRing] per part: a node's value is not finite
     int64_t* s_warp = reinterpret_cast<int64_t*>(sm + G_::kMlAt);  // scratch of the scan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -315,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         }
         for (int s = 0; s < kParts; ++s) {
             mbar_init(&pt_full[s], 1);
-            mbar_init(&pt_empty[s], FP8 ? 15 : 14);  // TMA, MMA, 4 + 8 warps, and the scale warp
+            mbar_init(&pt_empty[s], FP8 ? 11 : 10);  // TMA, MMA, 8 softmax warps, and the scale warp
         }
         mbar_init(ml_in, 8);
         mbar_init(ml_out, 8);
@@ -334,17 +349,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     // ------------------------------------------------------------------ the share
     // every thread sums the weights of a run of sequences
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
+    TileInfo* s_info = reinterpret_cast<TileInfo*>(sm + G_::kInfoAt);
     Walk w;
     const int run = (a.batch + kThreads - 1) / kThreads;
     const int i0 = min(a.batch, static_cast<int>(threadIdx.x) * run), i1 = min(a.batch, i0 + run);
     int64_t mine = 0;
     bool pairs = false;
+#pragma unroll 1
     for (w.i = i0; w.i < i1; ++w.i) {
         w.load(a);
         if (w.n == 0) continue;
         if (w.bad(a)) {  // its rows become NaN
             if (a.status) atomicCAS(a.status, 0, kStatusBad);
             if (w.i % gridDim.x == blockIdx.x)
+#pragma unroll 1
                 for (int64_t e = 0; e < static_cast<int64_t>(w.n) * a.nq * D; ++e)
                     a.out[static_cast<int64_t>(w.first) * a.nq * D + e] = 0x7fc0;
             continue;
@@ -362,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     if (lane == 31) s_warp[warp] = before;
     __syncthreads();
     int64_t total = 0, base = before - mine;
+#pragma unroll 1
     for (int k = 0; k < kThreads / 32; ++k) {
         if (k < warp) base += s_warp[k];
         total += s_warp[k];
@@ -369,12 +388,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(*s_pairs ? 2 : 1));
     const int64_t lo = per * blockIdx.x, hi = min(total, lo + per);
     if (mine > 0 && lo >= base && lo < base + mine) {
+#pragma unroll 1
         for (w.i = i0; w.i < i1; ++w.i) {
             w.load(a);
             if (w.n == 0 || w.bad(a)) continue;
-            const int64_t here = w.head_weight(a) * a.nkv;
-            if (lo < base + here) break;
-            base += here;
+            const int64_t here = w.head_weight(a);
+            *s_head = here;
+            if (lo < base + here * a.nkv) break;
+            base += here * a.nkv;
         }
         *s_seq = w.i;
         *s_base = base;
@@ -389,17 +410,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     auto wait = [&](uint64_t* b, uint32_t parity) {
         if (mbar_try_wait(b, parity)) return;
         const uint64_t start = globaltimer_ns();
-        while (!*abort_flag) {
-            if (mbar_try_wait_sleep(b, parity, 100000u)) return;
-            if (globaltimer_ns() - start > NF_WAIT_BUDGET_NS) {
-                *abort_flag = 1;
-                if (a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
-            }
+        while (!mbar_try_wait_sleep(b, parity, 100000u)) {
+            if (*abort_flag) return;
+            if (globaltimer_ns() - start > kWaitNs) *abort_flag = 1;
         }
     };
-
-    // The part at k.idx; a role that has finished one hands its descriptor back.
+    // A role's next part; it hands a part's descriptor back when it is through with it.
     auto open = [&](Task& k) {
+        ++k.idx;
         const int r = k.idx % kParts;
         wait(&pt_full[r], (k.idx / kParts) & 1u);
         const Part& p = s_part[r];
@@ -412,25 +430,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         k.n = p.n;
         k.sub = 0;
     };
-    auto begin = [&]() {
-        Task k;
-        k.idx = 0;
-        open(k);
-        return k;
-    };
-    // one task on; true when that ended a part
-    auto step = [&](Task& k) {
-        if (k.pair && k.sub == 0) {
-            k.sub = 1;
-            return false;
-        }
-        k.sub = 0;
-        if (++k.t < k.t1) return false;
-        ++k.idx;
-        open(k);
-        return true;
-    };
     auto hand_back = [&](int idx) { mbar_arrive(&pt_empty[idx % kParts]); };
+    // The order of a share's tiles, the same in every role: the scores are
+    // taken two tasks ahead of the products with V, so K's tiles of tasks 0
+    // and 1 come first, then V's of task u - 2 and K's of task u in turn.
+    auto in_order = [&](auto&& on_v, auto&& on_k) {
+        Task k, v1, v2;
+        k.valid = true;
+#pragma unroll 1
+        for (uint32_t u = 0;; ++u) {
+            if (k.valid && k.t == k.t1) open(k);
+            if (v2.valid) on_v(v2, u - 2);
+            if (k.valid) on_k(k, u);
+            else if (!v1.valid) break;
+            v2 = v1;
+            v1 = k;
+            if (k.valid) k.next();
+        }
+    };
 
     // the softmax warps take over the others' registers: 256 x 184 + 256 x 72 = 512 x 128
     if (warp >= kConvWarp) {
@@ -444,11 +461,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             uint64_t* full = FP8 ? raw_full : kv_full;
             uint64_t* empty = FP8 ? raw_empty : kv_empty;
             int count = 0;
-            auto load = [&](const CUtensorMap* map, const Task& k) {
+            auto load = [&](const CUtensorMap* map, const Task& k, int what) {
                 const int s = count % N;
                 if (count >= N) wait(&empty[s], ((count / N) & 1u) ^ 1u);
                 if (*abort_flag) return;
                 if (FP8) {
+                    s_info[s] = TileInfo{what, k.p0 - k.t * kKeys, k.p0 + k.n - k.t * kKeys, k.idx};
+                    if (what == kTileEnd) {
+                        mbar_arrive(&full[s]);
+                        return;
+                    }
                     mbar_arrive_expect_tx(&full[s], G_::kRawBytes);
                     tma_load_3d(sm + G_::kRawAt + s * G_::kRawBytes, map, &full[s], 0, k.t * kKeys, k.z);
                 } else {
@@ -458,18 +480,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 }
                 ++count;
             };
-            Task k = begin(), v = k;
-            // the order in which the products take the tiles: two tiles of K ahead, then V and K in turn
-            for (int u = 0; k.valid || v.valid; ++u) {
-                if (u >= 2) {
-                    if (v.fresh()) load(&tmv, v);
-                    if (step(v)) hand_back(v.idx - 1);
-                }
-                if (k.valid) {
-                    if (k.fresh()) load(&tmk, k);
-                    step(k);
-                }
-            }
+            in_order(
+                [&](const Task& v, uint32_t) {
+                    if (v.fresh()) load(&tmv, v, v.tail() ? kTileVTail : kTileV);
+                    if (v.ends()) hand_back(v.idx);
+                },
+                [&](const Task& k, uint32_t) {
+                    if (k.fresh()) load(&tmk, k, kTileK);
+                });
+            if (FP8) load(&tmk, Task(), kTileEnd);
             if (*abort_flag)  // the copies in flight land before the CTA leaves
                 for (int j = max(0, count - N); j < count; ++j) {
                     const uint64_t t = globaltimer_ns();
@@ -492,14 +511,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             ++count;
             return s;
         };
-        Task k = begin(), v = k;
-        for (uint32_t u = 0; k.valid || v.valid; ++u) {
-            if (u >= 2) {
-                const uint32_t task = u - 2, s = task & 1;
+        in_order(
+            [&](const Task& v, uint32_t u) {
+                const uint32_t s = u & 1;
                 const bool clean = !FP8 && v.fresh() && v.tail();
                 if (v.fresh()) v_stage = entry();
-                if (clean && lane == 0) mbar_arrive(v_ask);
-                wait(&p_full[s], (task >> 1) & 1u);
+                if (clean && lane == 0) {
+                    s_info[0] = TileInfo{v_stage, v.p0 - v.t * kKeys, v.p0 + v.n - v.t * kKeys, v.idx};
+                    mbar_arrive(v_ask);
+                }
+                wait(&p_full[s], (u >> 1) & 1u);
                 if (clean) wait(v_fixed, fixed++ & 1u);
                 tc_fence_after();
                 const bool start = v.pair ? v.t == v.t0 : v.t - v.t0 < 2;
@@ -513,14 +534,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     if (last) tc_commit(&o_full[s]);
                 }
                 __syncwarp();
-                if (step(v) && lane == 0) hand_back(v.idx - 1);
-            }
-            if (k.valid) {
+                if (v.ends() && lane == 0) hand_back(v.idx);
+            },
+            [&](const Task& k, uint32_t u) {
                 const int slot = (q_at + k.sub) & 1;
                 if (k.t == k.t0) wait(&q_full[slot], ((q_at + k.sub) >> 1) & 1u);
                 if (k.fresh()) k_stage = entry();
                 tc_fence_after();
-                const bool last = k.t == k.t1 - 1;
                 if (leader && !*abort_flag) {
                     const uint64_t qd = sdesc_sw128(smem_u32(sm + G_::kQ + slot * G_::kTileBytes));
                     const uint64_t kd = sdesc_sw128(smem_u32(sm + G_::kRing + k_stage * G_::kTileBytes));
@@ -531,12 +551,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     }
                     tc_commit(&s_full[u & 1]);
                     if (k.done()) tc_commit(&kv_empty[k_stage]);
-                    if (last) tc_commit(&q_empty[slot]);
+                    if (k.t == k.t1 - 1) tc_commit(&q_empty[slot]);
                 }
                 __syncwarp();
-                if (last && k.done()) q_at += k.pair ? 2 : 1;
-                step(k);
-            }
+                if (k.ends()) q_at += k.pair ? 2 : 1;
+            });
+        if (!FP8 && lane == 0) {
+            s_info[0].what = -1;
+            mbar_arrive(v_ask);
         }
         if (*abort_flag && leader) {
             tc_commit(drained);
@@ -548,22 +570,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // ----------------------- the walk, and q's rows into swizzled tiles
         w.valid = true;
         w.i = *s_seq;
-        w.at = *s_base;
         w.lo = lo;
         w.hi = hi;
         w.load(a);
-        const int64_t head = w.head_weight(a);
-        w.g = static_cast<int>((lo - w.at) / head);
-        w.at += w.g * head;
+        w.g = static_cast<int>((lo - *s_base) / *s_head);
+        w.at = *s_base + w.g * *s_head;
         w.pt = 0;
-        w.item(a);
-        while (w.at + w.weight() <= lo) {
-            w.at += w.weight();
-            ++w.pt;
-            w.item(a);
-        }
-        w.part(a);
-        if (w.t0 >= w.t1) w.next(a);
+        w.seek(a, true);
         int at = 0;
         for (int idx = 0;; ++idx) {
             const int r = idx % kParts;
@@ -583,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     p.kind = (w.t0 == 0) | (w.t1 == w.kt) << 1;
                     if (p.kind == 1) {  // other CTAs hold the rest: how many parts there are to join
                         JoinDesc d{};
-                        d.parts = static_cast<int>((w.at + static_cast<int64_t>(w.kt - 1) * (w.pair() ? 2 : 1)) / per) -
+                        d.parts = static_cast<int>((w.at + (static_cast<int64_t>(w.kt - 1) << (w.pair() ? 1 : 0))) / per) -
                                   static_cast<int>(blockIdx.x) + 1;
                         d.rows = w.rows;
                         d.row0 = w.row0;
@@ -615,43 +628,57 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[slot]);
             }
-            w.next(a);
+            w.seek(a, false);
         }
     } else if (warp == kScaleWarp) {
         // ------------------- E4M3: a task's 128 key scales (times c) and value scales
         if (FP8) {
-            Task k = begin();
+            Task k, prev;
             float ks[4], vs[4];
-            auto fetch = [&]() {
-                const int64_t row = static_cast<int64_t>(k.z) * a.L;
+            k.valid = true;
+#pragma unroll 1
+            for (uint32_t u = 0;; ++u) {  // task u's scales are fetched, then those of task u - 1 stored
+                float oks[4], ovs[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int key = k.t * kKeys + 32 * e + lane;
-                    const bool in = key < k.p0 + k.n;
-                    ks[e] = in ? __ldg(a.k_scale + row + key) : 0.f;
-                    vs[e] = in ? __ldg(a.v_scale + row + key) : 0.f;
+                    oks[e] = ks[e];
+                    ovs[e] = vs[e];
                 }
-            };
-            if (k.valid) fetch();
-            for (uint32_t u = 0; k.valid; ++u) {
-                const uint32_t s = u & 1, b = (u >> 1) & 1, at = 2 * s + b;
-                if (u >= 4) wait(&sc_empty[at], ((u >> 2) & 1u) ^ 1u);
-                float* dst = reinterpret_cast<float*>(sm + G_::kScaleAt) + at * 2 * kKeys;
-                bool bad = false;
+                if (k.valid && k.t == k.t1) open(k);
+                if (k.valid) {
+                    const int64_t row = static_cast<int64_t>(k.z) * a.L;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    dst[32 * e + lane] = ks[e] * a.c;
-                    if (k.t * kKeys + 32 * e + lane >= k.p0 && !isfinite(vs[e])) {
-                        bad = true;
-                        vs[e] = 0.f;
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = k.t * kKeys + 32 * e + lane;
+                        const bool in = key < k.p0 + k.n;
+                        ks[e] = in ? __ldg(a.k_scale + row + key) : 0.f;
+                        vs[e] = in ? __ldg(a.v_scale + row + key) : 0.f;
                     }
-                    dst[kKeys + 32 * e + lane] = vs[e];
                 }
-                if (bad) s_bad[k.idx % kBadRing] = 1;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sc_full[at]);
-                if (step(k) && lane == 0) hand_back(k.idx - 1);
-                if (k.valid) fetch();
+                if (u > 0) {
+                    const uint32_t o = u - 1, at = 2 * (o & 1) + ((o >> 1) & 1);
+                    if (o >= 4) wait(&sc_empty[at], ((o >> 2) & 1u) ^ 1u);
+                    float* dst = reinterpret_cast<float*>(sm + G_::kScaleAt) + at * 2 * kKeys;
+                    bool bad = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        dst[32 * e + lane] = oks[e] * a.c;
+                        if (prev.t * kKeys + 32 * e + lane >= prev.p0 && !isfinite(ovs[e])) {
+                            bad = true;
+                            ovs[e] = 0.f;
+                        }
+                        dst[kKeys + 32 * e + lane] = ovs[e];
+                    }
+                    if (bad) s_bad[prev.idx % kBadRing] = 1;
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&sc_full[at]);
+                        if (prev.ends()) hand_back(prev.idx);
+                    }
+                }
+                if (!k.valid) break;
+                prev = k;
+                k.next();
             }
         }
     } else {
@@ -659,16 +686,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // behind the sequence's rows, and whose nodes' values that are not
         // finite, become zero (a zero probability must not meet a NaN).
         const int tid = threadIdx.x - kConvWarp * 32;
-        int count = 0;
-        uint32_t asked = 0;
-        auto entry = [&](const Task& k, bool is_v) {
-            const bool tail = k.tail();
-            const int end = k.p0 + k.n - k.t * kKeys, node = k.p0 - k.t * kKeys;  // in keys of the tile
-            const int s = count % NS;
-            uint8_t* dst = sm + G_::kRing + s * G_::kTileBytes;
+#pragma unroll 1
+        for (int count = 0;; ++count) {
             if (FP8) {
-                const int r = count % NR;
+                const int r = count % NR, s = count % NS;
                 wait(&raw_full[r], (count / NR) & 1u);
+                const TileInfo info = s_info[r];
+                if (*abort_flag || info.what == kTileEnd) break;
+                const bool is_v = info.what != kTileK, tail = info.what == kTileVTail;
+                const int node = info.node, end = info.end;
+                uint8_t* dst = sm + G_::kRing + s * G_::kTileBytes;
                 if (count >= NS) wait(&kv_empty[s], ((count / NS) & 1u) ^ 1u);
                 const uint8_t* src = sm + G_::kRawAt + r * G_::kRawBytes;
                 constexpr int C = D / 16;  // 16-byte chunks of a raw row
@@ -713,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         put((b + j) * 128 + tid, y);
                     }
                 }
-                if ((nan & 0x80808080u) != 0 || (is_v && tail)) {
+                if ((nan & 0x80808080u) != 0 || tail) {
                     // rare: once more, with NaN codes as NaN, and V's rows behind the sequence and NaN nodes as zeros
 #pragma unroll 1
                     for (int e = tid; e < C * 128; e += 128) {
@@ -737,16 +764,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         put(e, y);
                     }
                 }
-                if (bad) s_bad[k.idx % kBadRing] = 1;
+                if (bad) s_bad[info.idx % kBadRing] = 1;
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&raw_empty[r]);
                     mbar_arrive(&kv_full[s]);
                 }
-            } else if (is_v && tail) {
-                wait(v_ask, asked++ & 1u);
-                const int row = tid;
+            } else {
+                wait(v_ask, count & 1u);
+                const TileInfo info = s_info[0];
+                if (*abort_flag || info.what < 0) break;
+                const int row = tid, node = info.node, end = info.end;
+                uint8_t* dst = sm + G_::kRing + info.what * G_::kTileBytes;
                 bool zero = row >= end;
                 if (row >= node && row < end) {
                     uint32_t inf = 0;
@@ -761,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     }
                     if (inf) {
                         zero = true;
-                        s_bad[k.idx % kBadRing] = 1;
+                        s_bad[info.idx % kBadRing] = 1;
                     }
                 }
                 if (zero)
@@ -772,18 +802,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_fixed);
-            }
-            ++count;
-        };
-        Task k = begin(), v = k;
-        for (int u = 0; k.valid || v.valid; ++u) {
-            if (u >= 2) {
-                if (v.fresh()) entry(v, true);
-                if (step(v) && lane == 0) hand_back(v.idx - 1);
-            }
-            if (k.valid) {
-                if (k.fresh()) entry(k, false);
-                step(k);
             }
         }
     }
@@ -1022,6 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag && a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
 }
 
 // Joins the parts of items that several CTAs computed, in their order: one
