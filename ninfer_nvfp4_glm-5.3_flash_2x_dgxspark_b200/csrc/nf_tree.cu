@@ -25,6 +25,7 @@ namespace {
 constexpr int kStatusBad = NF_DEVERR_BAD_TOKEN;
 constexpr int kKeys = 128;       // keys per tile
 constexpr int kTileRows = 128;   // rows per MMA tile
+constexpr int kNarrow = 16;      // up to this many rows, four threads share a row of scores
 constexpr int kItemRows = 256;   // rows per work item: two MMA tiles
 constexpr int kMaxCtas = 148;    // CTAs (one per SM) the workspace has parts for
 constexpr int kThreads = 512;
@@ -111,6 +112,50 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "%15, %16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// 16 lanes x 64 (or 128) consecutive columns as matrix fragments: thread t holds
+// columns 8 i + 2 (t % 4) and + 1 of lane t / 4 in r[4 i], r[4 i + 1] and of
+// lane t / 4 + 8 in r[4 i + 2], r[4 i + 3].
+__device__ __forceinline__ void tmem_ld_frag64(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t* r) {  // 32 columns
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_frag64(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// 16 lanes x 64 columns: thread t's column 4 i + t % 4 of lane t / 4 in r[2 i], of lane t / 4 + 8 in r[2 i + 1].
+__device__ __forceinline__ void tmem_st_pairs64(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -713,20 +758,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             up ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 };
-                // sign and the 7 exponent and mantissa bits in a BF16's places are the code times 2^-120, subnormal
-                // codes too
+                // A code b's sign and 7 exponent and mantissa bits in a BF16's places, 16 b + 240 (b & 128), are the
+                // code times 2^-120, subnormal codes too.  Multiplications, as the logic pipe is the narrower one.
                 auto widen = [&](const uint4& x, uint32_t* y) {
                     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t b = __byte_perm(in[j], 0u, h ? 0x3424 : 0x1404);
-                            const uint32_t t = ((b >> 4) & 0x07f007f0u) | (b & 0x80008000u);
+                            const uint32_t b = __byte_perm(in[j], 0u, h ? 0x4342 : 0x4140);
+                            uint32_t t;
+                            asm("mad.lo.u32 %0, %1, 240, %2;" : "=r"(t) : "r"(b & 0x00800080u), "r"(b * 16u));
                             asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y[2 * j + h]) : "r"(t), "r"(0x7b807b80u));  // 2^120
                         }
-                        nan |= (in[j] & 0x7f7f7f7fu) + 0x01010101u;  // a code 0x7f carries into the sign's place
                     }
+                    // a code 0x7f carries into the sign's place
+                    nan |= ((in[0] & 0x7f7f7f7fu) + 0x01010101u) | ((in[1] & 0x7f7f7f7fu) + 0x01010101u);
+                    nan |= ((in[2] & 0x7f7f7f7fu) + 0x01010101u) | ((in[3] & 0x7f7f7f7fu) + 0x01010101u);
                 };
 #pragma unroll
                 for (int b = 0; b < C; b += 4) {
@@ -822,9 +870,48 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const int mine0 = static_cast<int>((s ^ u0) & 1);  // pair: which MMA tile; else: the first tile's offset
             const int row0 = pair ? mine0 * kTileRows : 0;      // first row of the stream in the item
             const int rows = min(kTileRows, w.rows - row0);
-            const bool active = (warp & 3) * 32 < rows;
+            const bool active = (warp & 3) * 32 < rows, narrow = w.rows <= kNarrow;
             const int row = w.row0 + row0 + r, node = row / a.G;
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f, m2 = -INFINITY, l2 = 0.f;  // (m2, l2): a narrow part's second row
+            // which keys of tile t a node's row sees
+            auto visible = [&](int node, bool valid, int t, uint32_t* vis) {
+                const int j0 = t * kKeys - p0;  // node of the tile's first key
+                auto low = [](int k) { return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u; };
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int j = j0 + 32 * c;
+                    if (!a.mask) {
+                        vis[c] = low(min(n, node + 1) - j);
+                        continue;
+                    }
+                    uint64_t bits = 0;
+                    if (j > -32 && valid) {
+                        const unsigned long long* mw =
+                            reinterpret_cast<const unsigned long long*>(a.mask) + static_cast<int64_t>(w.first + node) * a.words;
+                        const int wi = j >> 6, sh = j & 63;
+                        if (wi >= 0 && wi < a.words) bits = __ldg(mw + wi) >> sh;
+                        if (sh > 32 && wi + 1 >= 0 && wi + 1 < a.words) bits |= __ldg(mw + wi + 1) << (64 - sh);
+                    }
+                    vis[c] = (static_cast<uint32_t>(bits) & low(n - j)) | low(-j);
+                }
+            };
+            // whether the node sees a row whose value is not finite (some node's is)
+            auto poisoned = [&](int node) {
+                const int64_t base_row = static_cast<int64_t>(w.z) * a.L + p0;
+#pragma unroll 1
+                for (int j = 0; j < n; ++j) {
+                    if (a.mask ? j >= 64 * a.words || !((a.mask[static_cast<int64_t>(w.first + node) * a.words + (j >> 6)] >> (j & 63)) & 1)
+                               : j > node)
+                        continue;
+                    bool bad = FP8 && !isfinite(a.v_scale[base_row + j]);
+#pragma unroll 1
+                    for (int d = 0; d < D; ++d)
+                        bad |= FP8 ? (static_cast<const uint8_t*>(a.v)[(base_row + j) * D + d] & 0x7f) == 0x7f
+                                   : (static_cast<const uint16_t*>(a.v)[(base_row + j) * D + d] & 0x7f80) == 0x7f80;
+                    if (bad) return true;
+                }
+                return false;
+            };
             int done = 0;
             for (int t = w.t0 + (pair ? 0 : mine0); t < t1; t += pair ? 1 : 2, ++mine_n, ++done) {
                 const uint32_t b = mine_n & 1;
@@ -832,31 +919,94 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 wait(&s_full[s], mine_n & 1u);
                 if (FP8) wait(&sc_full[2 * s + b], (mine_n >> 1) & 1u);
                 __syncwarp();
-                if (active) {
+                const bool tail = (t + 1) * kKeys > p0;
+                if (narrow && active) {
+                    // thread t of the warp: every fourth pair of columns of rows t / 4 and t / 4 + 8
                     tc_fence_after();
-                    const bool tail = (t + 1) * kKeys > p0;
-                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-                    if (tail) {
-                        const int j0 = t * kKeys - p0;  // node of the tile's first key
-                        auto low = [](int k) { return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u; };
+                    const bool two = rows > 8;
+                    uint32_t v[64], pk[32];
+                    tmem_ld_frag64(t_s, v);
+                    tmem_ld_frag64(t_s + 64, v + 32);
+                    tmem_wait_ld();
+                    float mnew[2], fac[2];
+                    bool grow = done == 0;
+                    const float* sq = sc + 2 * (lane & 3);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int j = j0 + 32 * c;
-                            if (!a.mask) {
-                                vis[c] = low(min(n, node + 1) - j);
-                                continue;
-                            }
-                            uint64_t bits = 0;
-                            if (j > -32 && r < rows) {
-                                const uint64_t* mw = a.mask + static_cast<int64_t>(w.first + node) * a.words;
-                                const int wi = j >> 6, sh = j & 63;
-                                if (wi >= 0 && wi < a.words) bits = __ldg(reinterpret_cast<const unsigned long long*>(mw + wi)) >> sh;
-                                if (sh > 32 && wi + 1 >= 0 && wi + 1 < a.words)
-                                    bits |= __ldg(reinterpret_cast<const unsigned long long*>(mw + wi + 1)) << (64 - sh);
-                            }
-                            vis[c] = (static_cast<uint32_t>(bits) & low(n - j)) | low(-j);
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == 1 && !two) break;
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint64_t f = FP8 ? *reinterpret_cast<const uint64_t*>(sq + 8 * i) : f32x2_pack(a.c, a.c);
+                            const uint64_t y = mul_f32x2(f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), f);
+                            v[4 * i + 2 * h] = __float_as_uint(f32x2_lo(y));
+                            v[4 * i + 2 * h + 1] = __float_as_uint(f32x2_hi(y));
                         }
+                        if (tail) {
+                            uint32_t vis[4];
+                            const int r2 = (lane >> 2) + 8 * h;
+                            visible((w.row0 + r2) / a.G, r2 < rows, t, vis);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    if (!((vis[i >> 2] >> (8 * (i & 3) + 2 * (lane & 3) + e)) & 1)) v[4 * i + 2 * h + e] = 0xff800000u;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            mx = max3(mx, __uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                        const float old = h ? m2 : m;
+                        mnew[h] = fmaxf(old, mx);
+                        grow |= mx > old + kRescale;
+                        fac[h] = old == -INFINITY ? 0.f : ex2(old - mnew[h]);
                     }
+                    if (__any_sync(0xffffffffu, grow)) {
+                        if (!two) fac[1] = 0.f;
+                        if (done > 0) {
+#pragma unroll 1
+                            for (int c = 0; c < D / 64; ++c) {
+                                uint32_t o[32];
+                                tmem_ld_frag64(t_o + 64 * c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fac[(j >> 1) & 1]);
+                                tmem_st_frag64(t_o + 64 * c, o);
+                            }
+                            l *= fac[0];
+                            l2 *= fac[1];
+                        }
+                        m = mnew[0];
+                        if (two) m2 = mnew[1];
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == 1 && !two) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) pk[2 * i + 1] = 0u;
+                            break;
+                        }
+                        const float mh = h ? m2 : m, mu = mh == -INFINITY ? 0.f : mh;
+                        const uint64_t nm = f32x2_pack(-mu, -mu);
+                        uint64_t sum = 0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint64_t y = add_f32x2(f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), nm);
+                            uint64_t pr = f32x2_pack(ex2(f32x2_lo(y)), ex2(f32x2_hi(y)));
+                            sum = add_f32x2(sum, pr);
+                            if (FP8) pr = mul_f32x2(pr, *reinterpret_cast<const uint64_t*>(sq + kKeys + 8 * i));
+                            pk[2 * i + h] = bf16x2_hw(f32x2_lo(pr), f32x2_hi(pr));
+                        }
+                        (h ? l2 : l) += f32x2_lo(sum) + f32x2_hi(sum);  // this thread's columns; joined at the part's end
+                    }
+                    tmem_st_pairs64(t_s, pk);
+                    tmem_wait_st();
+                    tc_fence_before();
+                } else if (active) {
+                    tc_fence_after();
+                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    if (tail) visible(node, r < rows, t, vis);
                     // x = S * factor: the whole row of the tile in registers
                     float x[kKeys];
                     uint32_t* xb = reinterpret_cast<uint32_t*>(x);
@@ -949,37 +1099,92 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 __syncwarp();
                 tc_fence_after();
             }
-            if (s_bad[idx % kBadRing] != 0 && r < rows) {
-                // some node's value is not finite: a row that sees one is NaN
-                const int64_t base_row = static_cast<int64_t>(w.z) * a.L + p0;
-                for (int j = 0; j < n; ++j) {
-                    if (a.mask ? j >= 64 * a.words || !((a.mask[static_cast<int64_t>(w.first + node) * a.words + (j >> 6)] >> (j & 63)) & 1)
-                               : j > node)
-                        continue;
-                    bool bad = FP8 && !isfinite(a.v_scale[base_row + j]);
-                    for (int d = 0; d < D; ++d)
-                        bad |= FP8 ? (static_cast<const uint8_t*>(a.v)[(base_row + j) * D + d] & 0x7f) == 0x7f
-                                   : (static_cast<const uint16_t*>(a.v)[(base_row + j) * D + d] & 0x7f80) == 0x7f80;
-                    if (bad) l = NAN;
-                }
+            if (narrow && active) {
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                l2 += __shfl_xor_sync(0xffffffffu, l2, 1);
+                l2 += __shfl_xor_sync(0xffffffffu, l2, 2);
+            }
+            if (s_bad[idx % kBadRing] != 0) {
+                const int ra = narrow ? lane >> 2 : r;
+                if (active && ra < rows && poisoned((w.row0 + row0 + ra) / a.G)) l = NAN;
+                if (narrow && active && ra + 8 < rows && poisoned((w.row0 + ra + 8) / a.G)) l2 = NAN;
             }
             __syncwarp();
             const bool whole = w.kind == 3;
             const int slot = 2 * blockIdx.x + (w.kind & 1), cnt = t1 - w.t0;
             const Work wk = work_at(a.work);
-            float other_m = -INFINITY, other_l = 0.f;
+            float other_m = -INFINITY, other_l = 0.f, other_m2 = -INFINITY, other_l2 = 0.f;
             if (!pair) {
                 // both streams hold parts of the same rows: exchange (m, l), then each finishes half of the columns
-                s_ml[s * kTileRows + r] = make_float2(m, l);
+                const int ra = narrow ? lane >> 2 : r;
+                if (!narrow || active) {
+                    s_ml[s * kTileRows + ra] = make_float2(m, l);
+                    if (narrow) s_ml[s * kTileRows + ra + 8] = make_float2(m2, l2);
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ml_in);
                 wait(ml_in, ml_n & 1u);
                 __syncwarp();
-                const float2 o = s_ml[(s ^ 1) * kTileRows + r];
+                const float2 o = s_ml[(s ^ 1) * kTileRows + ra];
                 other_m = o.x;
                 other_l = o.y;
+                if (narrow) {
+                    const float2 o2 = s_ml[(s ^ 1) * kTileRows + ra + 8];
+                    other_m2 = o2.x;
+                    other_l2 = o2.y;
+                }
             }
-            if (active) {
+            if (narrow && active) {
+                const bool use0 = done > 0, use1 = cnt - done > 0;
+                float f0[2], f1[2], lt[2], mu[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float a0 = h ? m2 : m, a1 = h ? other_m2 : other_m, mt = fmaxf(a0, a1);
+                    mu[h] = mt == -INFINITY ? 0.f : mt;
+                    f0[h] = a0 == -INFINITY ? 0.f : ex2(a0 - mu[h]);
+                    f1[h] = a1 == -INFINITY ? 0.f : ex2(a1 - mu[h]);
+                    lt[h] = (h ? l2 : l) * f0[h] + (h ? other_l2 : other_l) * f1[h];
+                }
+                // D / 2 columns for each stream, 32 at a time
+#pragma unroll 1
+                for (int c = s * D / 2; c < (s + 1) * D / 2; c += 32) {
+                    uint32_t v[16];
+                    float o[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] = 0.f;
+                    if (use0) {
+                        tmem_ld_frag32(t_o + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __uint_as_float(v[j]) * f0[(j >> 1) & 1];
+                    }
+                    if (use1) {
+                        tmem_ld_frag32(tmem + 256 + (s ^ 1) * D + lanes + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = fmaf(__uint_as_float(v[j]), f1[(j >> 1) & 1], o[j]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int ra = (lane >> 2) + 8 * h, rr = w.row0 + ra, nd = rr / a.G;
+                        if (ra >= rows) continue;
+                        const float inv = lt[h] == 0.f ? 0.f : 1.f / lt[h];
+                        const int col = c + 2 * (lane & 3);
+                        uint16_t* dst = a.out + (static_cast<int64_t>(w.first + nd) * a.nq + w.g * a.G + (rr - nd * a.G)) * D + col;
+                        float* part_o = wk.acc + (static_cast<int64_t>(slot) * kItemRows + ra) * D + col;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x0 = o[4 * i + 2 * h], x1 = o[4 * i + 2 * h + 1];
+                            if (whole) *reinterpret_cast<uint32_t*>(dst + 8 * i) = bf16x2_hw(x0 * inv, x1 * inv);
+                            else *reinterpret_cast<float2*>(part_o + 8 * i) = make_float2(x0, x1);
+                        }
+                        if (!whole && s == 0 && (lane & 3) == 0)
+                            wk.ml[static_cast<int64_t>(slot) * kItemRows + ra] = make_float2(mu[h], lt[h]);
+                    }
+                }
+            }
+            if (active && !narrow) {
                 const float mt = fmaxf(m, other_m), mu = mt == -INFINITY ? 0.f : mt;
                 const float f0 = m == -INFINITY ? 0.f : ex2(m - mu), f1 = other_m == -INFINITY ? 0.f : ex2(other_m - mu);
                 const float lt = l * f0 + other_l * f1;
