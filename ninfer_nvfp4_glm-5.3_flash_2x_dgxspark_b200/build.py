@@ -28,8 +28,8 @@ LIB = HERE / "lib" / "libnf_moe.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = ["nf_kernels.cu", "nf_gemm.cu", "nf_gemm2.cu", "nf_moe.cu", "nf_noalloc.cu", "nf_ep.cu", "nf_tp.cu", "nf_attn.cu",
-              "nf_stack.cu", "nf_kv.cu", "nf_tree.cu", "nf_logprobs.cu"]
-HEADERS = ["nf_handle.h", "nf_common.cuh", "nf_internal.h", "nf_nccl.h", "nf_gemm_shared.cuh", "nf_kv.h"]
+              "nf_stack.cu", "nf_kv.cu", "nf_tree.cu", "nf_tree_few.cu", "nf_logprobs.cu"]
+HEADERS = ["nf_handle.h", "nf_common.cuh", "nf_internal.h", "nf_nccl.h", "nf_gemm_shared.cuh", "nf_kv.h", "nf_tree.cuh"]
 
 
 def _newer(out: Path, inputs: list[Path]) -> bool:

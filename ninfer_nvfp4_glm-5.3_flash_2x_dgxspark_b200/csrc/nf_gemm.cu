@@ -867,7 +867,7 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t inner_
 }
 
 bool make_tmap_kv(CUtensorMap* map, const void* base, bool bf16, uint64_t dim, uint64_t rows, uint64_t heads,
-                  uint32_t box_rows) {
+                  uint32_t box_rows, bool swizzle_bytes) {
     PfnEncodeTiled fn = encode_fn();
     if (!fn) return false;
     const uint64_t row_bytes = dim * (bf16 ? 2 : 1);
@@ -877,7 +877,9 @@ bool make_tmap_kv(CUtensorMap* map, const void* base, bool bf16, uint64_t dim, u
     cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
                           const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          bf16 || (swizzle_bytes && dim == 128) ? CU_TENSOR_MAP_SWIZZLE_128B
+                          : swizzle_bytes                          ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                   : CU_TENSOR_MAP_SWIZZLE_NONE,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }

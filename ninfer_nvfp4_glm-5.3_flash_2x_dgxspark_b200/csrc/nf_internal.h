@@ -155,10 +155,10 @@ cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t
 bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t inner_elems, uint64_t rows,
                   uint32_t box_inner, uint32_t box_rows);
 // A KV cache as a 3-D tensor [heads][rows][dim]: BF16 with boxes of 64 elements
-// x box_rows rows and the 128-byte swizzle, or bytes with unswizzled boxes of
-// whole rows.
+// x box_rows rows and the 128-byte swizzle, or bytes with boxes of whole rows
+// (64 or 128 bytes), unswizzled or with the row's own swizzle.
 bool make_tmap_kv(CUtensorMap* map, const void* base, bool bf16, uint64_t dim, uint64_t rows, uint64_t heads,
-                  uint32_t box_rows);
+                  uint32_t box_rows, bool swizzle_bytes = false);
 // B in box order as a 2-D byte tensor [bytes / 128 rows, 128] with 256-row
 // boxes and 128-byte swizzle: box i is the 32 KB block i.
 bool make_tmap_blocked(CUtensorMap* map, const void* base, uint64_t bytes, uint32_t box_rows = 256);

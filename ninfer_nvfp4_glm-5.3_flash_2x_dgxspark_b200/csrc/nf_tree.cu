@@ -2,18 +2,12 @@
 // sequence's new rows, one token, a chain or a tree, over its cached prefix
 // and over one another.
 //
-// The rows of a sequence and KV head are its nodes' q heads of that group, R =
-// nodes * G rows (row = node * G + head): one pass over the keys serves them
-// all.  With c = scale * log2 e, row r and key j:
-//   x = c q_r . k_j (times the key's scale),  m = running max of x,
-//   p = 2^(x - m),  l = sum p,  O = sum p v_j (times the value's scale)
-// and the result is O / l.  Parts of the keys give (m, l, O) each, and
-// O = sum O_i 2^(m_i - m), l = sum l_i 2^(m_i - m) joins them.
-#include "nf_kv.h"
-
-#include "nf_common.cuh"
-#include "nf_gemm_shared.cuh"
-#include "nf_internal.h"
+// The kernel for many rows.  A tile of 128 keys is multiplied with 128 rows on
+// the 5th-generation tensor cores, scores and outputs in TMEM, in two streams
+// that take turns: while one stream's scores go through the softmax, the other
+// stream's products run.  An item of more than 128 rows gives each stream its
+// own 128 rows over the same tiles; a smaller one gives them every other tile.
+#include "nf_tree.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -22,63 +16,12 @@ namespace nf {
 
 namespace {
 
-constexpr int kStatusBad = NF_DEVERR_BAD_TOKEN;
 constexpr int kKeys = 128;       // keys per tile
-constexpr int kTileRows = 128;   // rows per MMA tile
-constexpr int kNarrow = 16;      // up to this many rows, four threads share a row of scores
-constexpr int kItemRows = 256;   // rows per work item: two MMA tiles
-constexpr int kMaxCtas = 148;    // CTAs (one per SM) the workspace has parts for
 constexpr int kThreads = 512;
 constexpr int kConvWarp = 8, kTmaWarp = 12, kMmaWarp = 13, kRowWarp = 14, kScaleWarp = 15;
-constexpr int kParts = 8;        // part descriptors in flight
 constexpr int kBadRing = 16;
-constexpr uint64_t kWaitNs = 10000000000ull;  // a row tile's wait can last as long as a whole part
 constexpr float kRescale = 8.f;  // the running max may lag the true one by 2^8
 
-// What joins an item's parts: written by the CTA of its first part.
-struct JoinDesc {
-    int32_t parts;   // 0: nothing to join
-    int32_t rows;    // rows of the item
-    int32_t row0;    // its first row (node * G + head) in the sequence
-    int32_t first;   // the sequence's first row of q
-    int32_t head;    // KV head
-    int32_t pad[3];
-};
-struct Work {
-    JoinDesc* join;  // [kMaxCtas]
-    float2* ml;      // [2 kMaxCtas][kItemRows] (m, l)
-    float* acc;      // [2 kMaxCtas][kItemRows][D]
-};
-constexpr int64_t kJoinBytes = (kMaxCtas * sizeof(JoinDesc) + 255) / 256 * 256;
-constexpr int64_t kMlBytes = 2ll * kMaxCtas * kItemRows * 8;
-
-__host__ __device__ inline Work work_at(void* p) {
-    uint8_t* b = static_cast<uint8_t*>(p);
-    return Work{reinterpret_cast<JoinDesc*>(b), reinterpret_cast<float2*>(b + kJoinBytes),
-                reinterpret_cast<float*>(b + kJoinBytes + kMlBytes)};
-}
-
-struct TreeArgs {
-    const uint16_t* q;
-    uint16_t* out;
-    const int32_t* row_start;
-    const int32_t* prefix;
-    const int32_t* cache_seq;
-    const uint64_t* mask;
-    const float* k_scale;
-    const float* v_scale;
-    const void* v;  // the values once more, for the rare look at single rows
-    void* work;
-    int32_t* status;
-    int rows, nq, nkv, G, batch, seqs, L, words;
-    float c;        // scale * log2(e)
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -88,6 +31,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+__device__ __forceinline__ void f16x2_to_f32(uint32_t v, float& lo, float& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(v));
 }
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t p;
@@ -114,50 +62,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-// 16 lanes x 64 (or 128) consecutive columns as matrix fragments: thread t holds
-// columns 8 i + 2 (t % 4) and + 1 of lane t / 4 in r[4 i], r[4 i + 1] and of
-// lane t / 4 + 8 in r[4 i + 2], r[4 i + 3].
-__device__ __forceinline__ void tmem_ld_frag64(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t* r) {  // 32 columns
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st_frag64(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-// 16 lanes x 64 columns: thread t's column 4 i + t % 4 of lane t / 4 in r[2 i], of lane t / 4 + 8 in r[2 i + 1].
-__device__ __forceinline__ void tmem_st_pairs64(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D[tmem] (+)= A[tmem, BF16 pairs] * B[smem], K = 16 per instruction
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
@@ -179,95 +83,6 @@ __device__ __forceinline__ uint64_t sdesc_sw128_mn(uint32_t saddr, uint32_t lbo)
     d |= static_cast<uint64_t>(2u) << 61;
     return d;
 }
-
-// ---------------------------------------------------------------------------
-// The work: every (sequence, KV head, up to 256 rows) is an item of ceil(keys
-// / 128) tiles.  An item of up to 128 rows weighs 1 a tile, one of two MMA
-// tiles 2.  The items in order (sequence, head, rows) form one line of weight,
-// which the CTAs cut into equal shares; a tile belongs to the share in which
-// it starts.  One warp walks through the parts of the CTA's share and
-// publishes them to the other roles in a ring of descriptors.
-// ---------------------------------------------------------------------------
-struct Walk {
-    // the sequence
-    int i, first, n, p0, sq, npt;
-    // the part: rows [row0, row0 + rows) of KV head g, tiles [t0, t1) of kt
-    int g, pt, t0, t1, kt, row0, rows, keys;
-    int64_t at, lo, hi;  // weight at the item's start, and the CTA's share
-    bool valid;
-
-    __device__ __forceinline__ bool pair() const { return rows > kTileRows; }
-
-    __device__ __forceinline__ void load(const TreeArgs& a) {
-        first = min(max(__ldg(a.row_start + i), 0), a.rows);
-        n = max(0, min(max(__ldg(a.row_start + i + 1), 0), a.rows) - first);
-        p0 = __ldg(a.prefix + i);
-        sq = a.cache_seq ? __ldg(a.cache_seq + i) : i;
-        npt = (n * a.G + kItemRows - 1) / kItemRows;
-    }
-    __device__ __forceinline__ bool bad(const TreeArgs& a) const {
-        return p0 < 0 || sq < 0 || sq >= a.seqs || p0 > a.L - n;
-    }
-    // shape of item pt of the sequence
-    __device__ __forceinline__ void item(const TreeArgs& a) {
-        row0 = pt * kItemRows;
-        rows = min(kItemRows, n * a.G - row0);
-        keys = p0 + (a.mask ? n : min(n, (row0 + rows - 1) / a.G + 1));
-        kt = (keys + kKeys - 1) / kKeys;
-    }
-    __device__ __forceinline__ int weight() const { return pair() ? 2 * kt : kt; }
-    // weight of the sequence's items of one head
-    __device__ __forceinline__ int64_t head_weight(const TreeArgs& a) {
-        int64_t w = 0;
-#pragma unroll 1
-        for (pt = 0; pt < npt; ++pt) {
-            item(a);
-            w += weight();
-        }
-        return w;
-    }
-    // from the item (g, pt) at weight `at` to the first part inside the share, that item's own among them if `here`
-    __device__ __forceinline__ void seek(const TreeArgs& a, bool here) {
-#pragma unroll 1
-        for (;; here = false) {
-            if (!here) {
-                at += weight();
-                if (at >= hi) {
-                    valid = false;
-                    return;
-                }
-                if (++pt == npt) {
-                    pt = 0;
-                    if (++g == a.nkv) {
-                        g = 0;
-#pragma unroll 1
-                        do {
-                            ++i;  // at < hi <= total: there is another sequence with items
-                            load(a);
-                        } while (n == 0 || bad(a));
-                    }
-                }
-            }
-            item(a);
-            const int two = pair() ? 1 : 0;  // tile t starts at weight at + (t << two)
-            t0 = lo > at ? static_cast<int>(min(static_cast<int64_t>(kt), (lo - at + two) >> two)) : 0;
-            t1 = static_cast<int>(min(static_cast<int64_t>(kt), (hi - at + two) >> two));
-            if (t0 < t1) return;
-        }
-    }
-};
-
-// A part as the roles see it; rows 0 ends the share.
-struct Part {
-    int32_t z;      // cache sequence * KV heads + KV head
-    int32_t t0, t1; // its tiles
-    int32_t p0, n;  // the sequence's prefix and rows
-    int32_t first;  // the sequence's first row of q
-    int32_t row0, rows;  // the item's rows (node * G + head) of the sequence
-    int32_t g;      // KV head
-    int32_t kind;   // bit 0: holds tile 0, bit 1: holds the last tile
-    int32_t pad[2];
-};
 
 // A role's place in the parts, task by task: a tile of a part of up to 128
 // rows is one task, of a larger one two (its two MMA tiles on the same keys).
@@ -343,12 +158,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     uint64_t* drained = ml_out + 1;         // after a time-out: no product in flight
     int* s_abort = reinterpret_cast<int*>(drained + 1);
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_abort + 1);
-    int* s_seq = s_abort + 2;
-    int* s_pairs = s_abort + 3;
-    int64_t* s_base = reinterpret_cast<int64_t*>(s_abort + 4);   // weight before the start sequence
-    int64_t* s_head = s_base + 1;                                // weight of one of its heads
-    int* s_bad = reinterpret_cast<int*>(s_head + 1);            // [kBadRing] per part: a node's value is not finite
-    int64_t* s_warp = reinterpret_cast<int64_t*>(sm + G_::kMlAt);  // scratch of the scan
+    int* s_bad = s_abort + 2; // [kBadRing] per part: a node's value is not finite
+    __shared__ ShareScratch s_share;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -381,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         mbar_init(ml_out, 8);
         mbar_init(drained, 1);
         *s_abort = 0;
-        *s_pairs = 0;
+        s_share.pairs = 0;
         for (int s = 0; s < kBadRing; ++s) s_bad[s] = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmk);
@@ -391,61 +202,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
     __syncthreads();
 
-    // ------------------------------------------------------------------ the share
-    // every thread sums the weights of a run of sequences
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
     TileInfo* s_info = reinterpret_cast<TileInfo*>(sm + G_::kInfoAt);
-    Walk w;
-    const int run = (a.batch + kThreads - 1) / kThreads;
-    const int i0 = min(a.batch, static_cast<int>(threadIdx.x) * run), i1 = min(a.batch, i0 + run);
-    int64_t mine = 0;
-    bool pairs = false;
-#pragma unroll 1
-    for (w.i = i0; w.i < i1; ++w.i) {
-        w.load(a);
-        if (w.n == 0) continue;
-        if (w.bad(a)) {  // its rows become NaN
-            if (a.status) atomicCAS(a.status, 0, kStatusBad);
-            if (w.i % gridDim.x == blockIdx.x)
-#pragma unroll 1
-                for (int64_t e = 0; e < static_cast<int64_t>(w.n) * a.nq * D; ++e)
-                    a.out[static_cast<int64_t>(w.first) * a.nq * D + e] = 0x7fc0;
-            continue;
-        }
-        mine += w.head_weight(a) * a.nkv;
-        pairs |= w.n * a.G > kTileRows;
-    }
-    if (pairs) *s_pairs = 1;
-    int64_t before = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += up;
-    }
-    if (lane == 31) s_warp[warp] = before;
-    __syncthreads();
-    int64_t total = 0, base = before - mine;
-#pragma unroll 1
-    for (int k = 0; k < kThreads / 32; ++k) {
-        if (k < warp) base += s_warp[k];
-        total += s_warp[k];
-    }
-    const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(*s_pairs ? 2 : 1));
-    const int64_t lo = per * blockIdx.x, hi = min(total, lo + per);
-    if (mine > 0 && lo >= base && lo < base + mine) {
-#pragma unroll 1
-        for (w.i = i0; w.i < i1; ++w.i) {
-            w.load(a);
-            if (w.n == 0 || w.bad(a)) continue;
-            const int64_t here = w.head_weight(a);
-            *s_head = here;
-            if (lo < base + here * a.nkv) break;
-            base += here * a.nkv;
-        }
-        *s_seq = w.i;
-        *s_base = base;
-    }
-    __syncthreads();
+    using ItemWalk = Walk<kItemRows, kKeys>;
+    const Share share = find_share<D, kThreads, ItemWalk>(a, s_share);
+    const bool idle = share.lo >= share.hi;
     const uint32_t tmem = *s_tmem;
     volatile int* abort_flag = s_abort;
     tc_fence_after();
@@ -497,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     // the softmax warps take over the others' registers: 256 x 184 + 256 x 72 = 512 x 128
     if (warp >= kConvWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (lo >= hi) {
+    if (idle) {
         // no share
     } else if (warp == kTmaWarp) {
         // ------------------------------------------------------------- loads
@@ -613,44 +374,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         }
     } else if (warp == kRowWarp) {
         // ----------------------- the walk, and q's rows into swizzled tiles
-        w.valid = true;
-        w.i = *s_seq;
-        w.lo = lo;
-        w.hi = hi;
-        w.load(a);
-        w.g = static_cast<int>((lo - *s_base) / *s_head);
-        w.at = *s_base + w.g * *s_head;
-        w.pt = 0;
-        w.seek(a, true);
+        ItemWalk w;
+        w.start(a, share, s_share);
         int at = 0;
         for (int idx = 0;; ++idx) {
             const int r = idx % kParts;
             if (idx >= kParts) wait(&pt_empty[r], ((idx / kParts) & 1u) ^ 1u);
             if (lane == 0) {
-                Part p{};
-                if (w.valid) {
-                    p.z = w.sq * a.nkv + w.g;
-                    p.t0 = w.t0;
-                    p.t1 = w.t1;
-                    p.p0 = w.p0;
-                    p.n = w.n;
-                    p.first = w.first;
-                    p.row0 = w.row0;
-                    p.rows = w.rows;
-                    p.g = w.g;
-                    p.kind = (w.t0 == 0) | (w.t1 == w.kt) << 1;
-                    if (p.kind == 1) {  // other CTAs hold the rest: how many parts there are to join
-                        JoinDesc d{};
-                        d.parts = static_cast<int>((w.at + (static_cast<int64_t>(w.kt - 1) << (w.pair() ? 1 : 0))) / per) -
-                                  static_cast<int>(blockIdx.x) + 1;
-                        d.rows = w.rows;
-                        d.row0 = w.row0;
-                        d.first = w.first;
-                        d.head = w.g;
-                        work_at(a.work).join[blockIdx.x] = d;
-                    }
-                }
-                s_part[r] = p;
+                s_part[r] = w.describe(a, share);
                 mbar_arrive(&pt_full[r]);
             }
             __syncwarp();
@@ -745,7 +476,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 const uint8_t* src = sm + G_::kRawAt + r * G_::kRawBytes;
                 constexpr int C = D / 16;  // 16-byte chunks of a raw row
                 bool bad = false;
-                uint32_t nan = 0;
                 // chunk e of the raw tile (16 codes) to chunks 2 ch and 2 ch + 1 of its row; the upper half's threads
                 // store the second first, so that eight threads' stores lie in eight bank groups
                 auto put = [&](int e, const uint32_t* y) {
@@ -758,23 +488,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             up ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 };
-                // A code b's sign and 7 exponent and mantissa bits in a BF16's places, 16 b + 240 (b & 128), are the
-                // code times 2^-120, subnormal codes too.  Multiplications, as the logic pipe is the narrower one.
+                // exact, a NaN as a NaN: E4M3 -> F16 -> F32 -> BF16
                 auto widen = [&](const uint4& x, uint32_t* y) {
                     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t b = __byte_perm(in[j], 0u, h ? 0x4342 : 0x4140);
-                            uint32_t t;
-                            asm("mad.lo.u32 %0, %1, 240, %2;" : "=r"(t) : "r"(b & 0x00800080u), "r"(b * 16u));
-                            asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y[2 * j + h]) : "r"(t), "r"(0x7b807b80u));  // 2^120
+                            float lo, hi;
+                            f16x2_to_f32(e4m3x2_to_f16x2(h ? in[j] >> 16 : in[j]), lo, hi);
+                            y[2 * j + h] = bf16x2_hw(lo, hi);
                         }
-                    }
-                    // a code 0x7f carries into the sign's place
-                    nan |= ((in[0] & 0x7f7f7f7fu) + 0x01010101u) | ((in[1] & 0x7f7f7f7fu) + 0x01010101u);
-                    nan |= ((in[2] & 0x7f7f7f7fu) + 0x01010101u) | ((in[3] & 0x7f7f7f7fu) + 0x01010101u);
                 };
 #pragma unroll
                 for (int b = 0; b < C; b += 4) {
@@ -788,28 +512,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         put((b + j) * 128 + tid, y);
                     }
                 }
-                if ((nan & 0x80808080u) != 0 || tail) {
-                    // rare: once more, with NaN codes as NaN, and V's rows behind the sequence and NaN nodes as zeros
+                if (tail) {
+                    // V's rows behind the sequence, and a node's chunks that hold a NaN, become zeros
 #pragma unroll 1
                     for (int e = tid; e < C * 128; e += 128) {
                         const int row = e / C;
                         const uint4 x = *reinterpret_cast<const uint4*>(src + e * 16);
-                        uint32_t y[8];
-                        nan = 0;
-                        widen(x, y);
-                        const bool node_row = is_v && row >= node && row < end;
-                        const bool zero = (is_v && row >= end) || (node_row && (nan & 0x80808080u));
-                        bad |= node_row && zero;
-                        if (!zero && !(nan & 0x80808080u)) continue;
+                        uint32_t y[8] = {};
                         const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                        uint32_t nan = 0;  // a code 0x7f carries into the sign's place
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const uint32_t c2 = in[j >> 1] >> (16 * (j & 1));
-                            if ((c2 & 0x7fu) == 0x7fu) y[j] = (y[j] & 0xffff0000u) | 0x7fc0u;
-                            if ((c2 & 0x7f00u) == 0x7f00u) y[j] = (y[j] & 0xffffu) | 0x7fc00000u;
-                            if (zero) y[j] = 0u;
-                        }
-                        put(e, y);
+                        for (int j = 0; j < 4; ++j) nan |= ((in[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                        const bool nan_node = nan != 0 && row >= node && row < end;
+                        bad |= nan_node;
+                        if (row >= end || nan_node) put(e, y);
                     }
                 }
                 if (bad) s_bad[info.idx % kBadRing] = 1;
@@ -861,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         const uint32_t t_s = tmem + s * kKeys + lanes, t_o = tmem + 256 + s * D + lanes;
         float2* s_ml = reinterpret_cast<float2*>(sm + G_::kMlAt);
         uint32_t u0 = 0, mine_n = 0, o_n = 0, ml_n = 0;  // tasks before the part; this stream's tasks and parts; exchanges
-        for (int idx = 0; lo < hi; ++idx) {
+        for (int idx = 0; !idle; ++idx) {
             wait(&pt_full[idx % kParts], (idx / kParts) & 1u);
             const Part& w = s_part[idx % kParts];
             if (*abort_flag || w.rows == 0) break;
@@ -870,48 +586,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const int mine0 = static_cast<int>((s ^ u0) & 1);  // pair: which MMA tile; else: the first tile's offset
             const int row0 = pair ? mine0 * kTileRows : 0;      // first row of the stream in the item
             const int rows = min(kTileRows, w.rows - row0);
-            const bool active = (warp & 3) * 32 < rows, narrow = w.rows <= kNarrow;
+            const bool active = (warp & 3) * 32 < rows;
             const int row = w.row0 + row0 + r, node = row / a.G;
-            float m = -INFINITY, l = 0.f, m2 = -INFINITY, l2 = 0.f;  // (m2, l2): a narrow part's second row
-            // which keys of tile t a node's row sees
-            auto visible = [&](int node, bool valid, int t, uint32_t* vis) {
-                const int j0 = t * kKeys - p0;  // node of the tile's first key
-                auto low = [](int k) { return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u; };
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int j = j0 + 32 * c;
-                    if (!a.mask) {
-                        vis[c] = low(min(n, node + 1) - j);
-                        continue;
-                    }
-                    uint64_t bits = 0;
-                    if (j > -32 && valid) {
-                        const unsigned long long* mw =
-                            reinterpret_cast<const unsigned long long*>(a.mask) + static_cast<int64_t>(w.first + node) * a.words;
-                        const int wi = j >> 6, sh = j & 63;
-                        if (wi >= 0 && wi < a.words) bits = __ldg(mw + wi) >> sh;
-                        if (sh > 32 && wi + 1 >= 0 && wi + 1 < a.words) bits |= __ldg(mw + wi + 1) << (64 - sh);
-                    }
-                    vis[c] = (static_cast<uint32_t>(bits) & low(n - j)) | low(-j);
-                }
-            };
-            // whether the node sees a row whose value is not finite (some node's is)
-            auto poisoned = [&](int node) {
-                const int64_t base_row = static_cast<int64_t>(w.z) * a.L + p0;
-#pragma unroll 1
-                for (int j = 0; j < n; ++j) {
-                    if (a.mask ? j >= 64 * a.words || !((a.mask[static_cast<int64_t>(w.first + node) * a.words + (j >> 6)] >> (j & 63)) & 1)
-                               : j > node)
-                        continue;
-                    bool bad = FP8 && !isfinite(a.v_scale[base_row + j]);
-#pragma unroll 1
-                    for (int d = 0; d < D; ++d)
-                        bad |= FP8 ? (static_cast<const uint8_t*>(a.v)[(base_row + j) * D + d] & 0x7f) == 0x7f
-                                   : (static_cast<const uint16_t*>(a.v)[(base_row + j) * D + d] & 0x7f80) == 0x7f80;
-                    if (bad) return true;
-                }
-                return false;
-            };
+            float m = -INFINITY, l = 0.f;
             int done = 0;
             for (int t = w.t0 + (pair ? 0 : mine0); t < t1; t += pair ? 1 : 2, ++mine_n, ++done) {
                 const uint32_t b = mine_n & 1;
@@ -920,93 +597,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 if (FP8) wait(&sc_full[2 * s + b], (mine_n >> 1) & 1u);
                 __syncwarp();
                 const bool tail = (t + 1) * kKeys > p0;
-                if (narrow && active) {
-                    // thread t of the warp: every fourth pair of columns of rows t / 4 and t / 4 + 8
-                    tc_fence_after();
-                    const bool two = rows > 8;
-                    uint32_t v[64], pk[32];
-                    tmem_ld_frag64(t_s, v);
-                    tmem_ld_frag64(t_s + 64, v + 32);
-                    tmem_wait_ld();
-                    float mnew[2], fac[2];
-                    bool grow = done == 0;
-                    const float* sq = sc + 2 * (lane & 3);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h == 1 && !two) break;
-                        float mx = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint64_t f = FP8 ? *reinterpret_cast<const uint64_t*>(sq + 8 * i) : f32x2_pack(a.c, a.c);
-                            const uint64_t y = mul_f32x2(f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), f);
-                            v[4 * i + 2 * h] = __float_as_uint(f32x2_lo(y));
-                            v[4 * i + 2 * h + 1] = __float_as_uint(f32x2_hi(y));
-                        }
-                        if (tail) {
-                            uint32_t vis[4];
-                            const int r2 = (lane >> 2) + 8 * h;
-                            visible((w.row0 + r2) / a.G, r2 < rows, t, vis);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                    if (!((vis[i >> 2] >> (8 * (i & 3) + 2 * (lane & 3) + e)) & 1)) v[4 * i + 2 * h + e] = 0xff800000u;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            mx = max3(mx, __uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1]));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float old = h ? m2 : m;
-                        mnew[h] = fmaxf(old, mx);
-                        grow |= mx > old + kRescale;
-                        fac[h] = old == -INFINITY ? 0.f : ex2(old - mnew[h]);
-                    }
-                    if (__any_sync(0xffffffffu, grow)) {
-                        if (!two) fac[1] = 0.f;
-                        if (done > 0) {
-#pragma unroll 1
-                            for (int c = 0; c < D / 64; ++c) {
-                                uint32_t o[32];
-                                tmem_ld_frag64(t_o + 64 * c, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fac[(j >> 1) & 1]);
-                                tmem_st_frag64(t_o + 64 * c, o);
-                            }
-                            l *= fac[0];
-                            l2 *= fac[1];
-                        }
-                        m = mnew[0];
-                        if (two) m2 = mnew[1];
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h == 1 && !two) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) pk[2 * i + 1] = 0u;
-                            break;
-                        }
-                        const float mh = h ? m2 : m, mu = mh == -INFINITY ? 0.f : mh;
-                        const uint64_t nm = f32x2_pack(-mu, -mu);
-                        uint64_t sum = 0;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint64_t y = add_f32x2(f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), nm);
-                            uint64_t pr = f32x2_pack(ex2(f32x2_lo(y)), ex2(f32x2_hi(y)));
-                            sum = add_f32x2(sum, pr);
-                            if (FP8) pr = mul_f32x2(pr, *reinterpret_cast<const uint64_t*>(sq + kKeys + 8 * i));
-                            pk[2 * i + h] = bf16x2_hw(f32x2_lo(pr), f32x2_hi(pr));
-                        }
-                        (h ? l2 : l) += f32x2_lo(sum) + f32x2_hi(sum);  // this thread's columns; joined at the part's end
-                    }
-                    tmem_st_pairs64(t_s, pk);
-                    tmem_wait_st();
-                    tc_fence_before();
-                } else if (active) {
+                if (active) {
                     tc_fence_after();
                     uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-                    if (tail) visible(node, r < rows, t, vis);
+                    if (tail)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) vis[c] = visible(a, w.first + node, node, n, t * kKeys + 32 * c - p0, r < rows);
                     // x = S * factor: the whole row of the tile in registers
                     float x[kKeys];
                     uint32_t* xb = reinterpret_cast<uint32_t*>(x);
@@ -1099,92 +695,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 __syncwarp();
                 tc_fence_after();
             }
-            if (narrow && active) {
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                l2 += __shfl_xor_sync(0xffffffffu, l2, 1);
-                l2 += __shfl_xor_sync(0xffffffffu, l2, 2);
-            }
-            if (s_bad[idx % kBadRing] != 0) {
-                const int ra = narrow ? lane >> 2 : r;
-                if (active && ra < rows && poisoned((w.row0 + row0 + ra) / a.G)) l = NAN;
-                if (narrow && active && ra + 8 < rows && poisoned((w.row0 + ra + 8) / a.G)) l2 = NAN;
-            }
+            if (s_bad[idx % kBadRing] != 0 && r < rows && poisoned<D, FP8>(a, w.z, p0, n, w.first, node)) l = NAN;
             __syncwarp();
             const bool whole = w.kind == 3;
             const int slot = 2 * blockIdx.x + (w.kind & 1), cnt = t1 - w.t0;
             const Work wk = work_at(a.work);
-            float other_m = -INFINITY, other_l = 0.f, other_m2 = -INFINITY, other_l2 = 0.f;
+            float other_m = -INFINITY, other_l = 0.f;
             if (!pair) {
                 // both streams hold parts of the same rows: exchange (m, l), then each finishes half of the columns
-                const int ra = narrow ? lane >> 2 : r;
-                if (!narrow || active) {
-                    s_ml[s * kTileRows + ra] = make_float2(m, l);
-                    if (narrow) s_ml[s * kTileRows + ra + 8] = make_float2(m2, l2);
-                }
+                s_ml[s * kTileRows + r] = make_float2(m, l);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ml_in);
                 wait(ml_in, ml_n & 1u);
                 __syncwarp();
-                const float2 o = s_ml[(s ^ 1) * kTileRows + ra];
+                const float2 o = s_ml[(s ^ 1) * kTileRows + r];
                 other_m = o.x;
                 other_l = o.y;
-                if (narrow) {
-                    const float2 o2 = s_ml[(s ^ 1) * kTileRows + ra + 8];
-                    other_m2 = o2.x;
-                    other_l2 = o2.y;
-                }
             }
-            if (narrow && active) {
-                const bool use0 = done > 0, use1 = cnt - done > 0;
-                float f0[2], f1[2], lt[2], mu[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float a0 = h ? m2 : m, a1 = h ? other_m2 : other_m, mt = fmaxf(a0, a1);
-                    mu[h] = mt == -INFINITY ? 0.f : mt;
-                    f0[h] = a0 == -INFINITY ? 0.f : ex2(a0 - mu[h]);
-                    f1[h] = a1 == -INFINITY ? 0.f : ex2(a1 - mu[h]);
-                    lt[h] = (h ? l2 : l) * f0[h] + (h ? other_l2 : other_l) * f1[h];
-                }
-                // D / 2 columns for each stream, 32 at a time
-#pragma unroll 1
-                for (int c = s * D / 2; c < (s + 1) * D / 2; c += 32) {
-                    uint32_t v[16];
-                    float o[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) o[j] = 0.f;
-                    if (use0) {
-                        tmem_ld_frag32(t_o + c, v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __uint_as_float(v[j]) * f0[(j >> 1) & 1];
-                    }
-                    if (use1) {
-                        tmem_ld_frag32(tmem + 256 + (s ^ 1) * D + lanes + c, v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = fmaf(__uint_as_float(v[j]), f1[(j >> 1) & 1], o[j]);
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int ra = (lane >> 2) + 8 * h, rr = w.row0 + ra, nd = rr / a.G;
-                        if (ra >= rows) continue;
-                        const float inv = lt[h] == 0.f ? 0.f : 1.f / lt[h];
-                        const int col = c + 2 * (lane & 3);
-                        uint16_t* dst = a.out + (static_cast<int64_t>(w.first + nd) * a.nq + w.g * a.G + (rr - nd * a.G)) * D + col;
-                        float* part_o = wk.acc + (static_cast<int64_t>(slot) * kItemRows + ra) * D + col;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x0 = o[4 * i + 2 * h], x1 = o[4 * i + 2 * h + 1];
-                            if (whole) *reinterpret_cast<uint32_t*>(dst + 8 * i) = bf16x2_hw(x0 * inv, x1 * inv);
-                            else *reinterpret_cast<float2*>(part_o + 8 * i) = make_float2(x0, x1);
-                        }
-                        if (!whole && s == 0 && (lane & 3) == 0)
-                            wk.ml[static_cast<int64_t>(slot) * kItemRows + ra] = make_float2(mu[h], lt[h]);
-                    }
-                }
-            }
-            if (active && !narrow) {
+            if (active) {
                 const float mt = fmaxf(m, other_m), mu = mt == -INFINITY ? 0.f : mt;
                 const float f0 = m == -INFINITY ? 0.f : ex2(m - mu), f1 = other_m == -INFINITY ? 0.f : ex2(other_m - mu);
                 const float lt = l * f0 + other_l * f1;
@@ -1297,28 +825,23 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
 }
 
 template <int D, bool FP8>
-cudaError_t launch(const nf_kv_cache& c, const TreeArgs& a, cudaStream_t st) {
+cudaError_t launch_many(const nf_kv_cache& c, const TreeArgs& a, int grid, cudaStream_t st) {
     CUtensorMap tmk, tmv;
     const uint64_t heads = static_cast<uint64_t>(c.seqs) * c.kv_heads;
     if (!make_tmap_kv(&tmk, c.k, !FP8, D, c.max_context, heads, kKeys) ||
         !make_tmap_kv(&tmv, c.v, !FP8, D, c.max_context, heads, kKeys))
         return cudaErrorInvalidValue;
     static bool attr[kMaxDevices] = {};
-    static int sms[kMaxDevices] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
     constexpr int smem = Geo<D, FP8>::kSmem;
     if (!attr[dev]) {
         const cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
-        sms[dev] = gemm_grid_size(dev);
         attr[dev] = true;
     }
-    const int grid = std::min(kMaxCtas, sms[dev]);
     tree_attention_kernel<D, FP8><<<grid, kThreads, smem, st>>>(tmk, tmv, a);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    return launch_dependent(tree_join_kernel<D>, dim3(grid, 4), dim3(256), 0, st, a);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -1349,9 +872,21 @@ cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int r
     a.L = c.max_context;
     a.words = mask_words;
     a.c = scale * 1.4426950408889634f;
-    const bool fp8 = c.kind == NF_KV_E4M3;
-    if (c.head_dim == 128) return fp8 ? launch<128, true>(c, a, st) : launch<128, false>(c, a, st);
-    return fp8 ? launch<64, true>(c, a, st) : launch<64, false>(c, a, st);
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    static int sms[kMaxDevices] = {};
+    if (!sms[dev]) sms[dev] = std::min(kMaxCtas, gemm_grid_size(dev));
+    const int grid = sms[dev];
+    const bool fp8 = c.kind == NF_KV_E4M3, wide = c.head_dim == 128;
+    // by the rows of an average item; either kernel is right for every item
+    const bool few = static_cast<int64_t>(rows) * a.G <= static_cast<int64_t>(kFewRows) * batch;
+    cudaError_t e = few   ? launch_tree_few(c, a, grid, st)
+                    : fp8 ? (wide ? launch_many<128, true>(c, a, grid, st) : launch_many<64, true>(c, a, grid, st))
+                          : (wide ? launch_many<128, false>(c, a, grid, st) : launch_many<64, false>(c, a, grid, st));
+    if (e == cudaSuccess)
+        e = wide ? launch_dependent(tree_join_kernel<128>, dim3(grid, 4), dim3(256), 0, st, a)
+                 : launch_dependent(tree_join_kernel<64>, dim3(grid, 4), dim3(256), 0, st, a);
+    return e;
 }
 
 }  // namespace nf
