@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     }
     if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
     __syncthreads();
+    pdl_trigger();  // the join's blocks may wait for this grid beside it
 
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
     TileInfo* s_info = reinterpret_cast<TileInfo*>(sm + G_::kInfoAt);
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 wait(&raw_full[r], (count / NR) & 1u);
                 const TileInfo info = s_info[r];
                 if (*abort_flag || info.what == kTileEnd) break;
-                const bool is_v = info.what != kTileK, tail = info.what == kTileVTail;
+                const bool tail = info.what == kTileVTail;
                 const int node = info.node, end = info.end;
                 uint8_t* dst = sm + G_::kRing + s * G_::kTileBytes;
                 if (count >= NS) wait(&kv_empty[s], ((count / NS) & 1u) ^ 1u);
@@ -768,7 +769,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         }
     }
     __syncwarp();
-    pdl_trigger();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -879,8 +879,9 @@ cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int r
     const int grid = sms[dev];
     const bool fp8 = c.kind == NF_KV_E4M3, wide = c.head_dim == 128;
     // by the rows of an average item; either kernel is right for every item
-    const bool few = static_cast<int64_t>(rows) * a.G <= static_cast<int64_t>(kFewRows) * batch;
-    cudaError_t e = few   ? launch_tree_few(c, a, grid, st)
+    const int64_t all = static_cast<int64_t>(rows) * a.G;
+    const int nt = all <= 8ll * batch ? 1 : all <= static_cast<int64_t>(kFewRows) * batch ? 2 : 0;
+    cudaError_t e = nt    ? launch_tree_few(c, a, nt, grid, st)
                     : fp8 ? (wide ? launch_many<128, true>(c, a, grid, st) : launch_many<64, true>(c, a, grid, st))
                           : (wide ? launch_many<128, false>(c, a, grid, st) : launch_many<64, false>(c, a, grid, st));
     if (e == cudaSuccess)
