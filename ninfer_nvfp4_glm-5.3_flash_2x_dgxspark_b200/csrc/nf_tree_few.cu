@@ -3,10 +3,11 @@
 //
 // The work is the cache's bytes: 8 rows do 16 (BF16) or 32 (E4M3) flops a
 // byte, a fraction of what the tensor cores could.  So the keys only have to
-// stream: one warp issues TMA tiles of 64 keys into a ring, and the others
-// take 16 keys of a tile each (groups of four warps take tiles in turn), with
-// their own running maximum, sum and output in registers, and join at the
-// part's end.  Both products are taken transposed, S^T = K Q^T and O^T = V^T
+// stream: one warp issues TMA tiles of 64 keys into a ring, and eight warps
+// take 32 keys of a tile each (pairs of warps take tiles in turn), with their
+// own running maximum, sum and output in registers.  Two more warps bring the
+// next part's q into fragments' order and join the eight warps' outputs of the
+// part before, so that the others go from part to part without a stop.  Both products are taken transposed, S^T = K Q^T and O^T = V^T
 // P^T, so that the keys and the head's dims fill the 16 rows of the m16n8k16
 // tiles and the 8 columns are the rows of q.  E4M3 codes become F16 in
 // registers, one conversion for two codes and nothing written back to shared
@@ -25,18 +26,22 @@ constexpr int kKeys = 64;     // keys per tile
 // NT: column tiles of 8 rows (1 or 2).
 template <int D, bool FP8, int NT>
 struct Geo {
-    static constexpr int kWarps = 16 / NT;      // consuming warps
-    static constexpr int kGroups = kWarps / 4;  // which take tiles in turn
-    static constexpr int kThreads = 32 * (kWarps + 1);
+    static constexpr int kWarps = 8;            // consuming warps
+    static constexpr int kGroups = kWarps / 2;  // which take tiles in turn
+    static constexpr int kAux = 2;              // warps for q and the join
+    static constexpr int kThreads = 32 * (kWarps + 1 + kAux);
     static constexpr int kRows = 8 * NT;
     static constexpr int kPitch = D + 8;        // floats of an output row in shared memory
     static constexpr int kTileBytes = kKeys * D * (FP8 ? 1 : 2);  // K or V
-    static constexpr int kStages = FP8 ? 8 : 4;
+    static constexpr int kStages = (FP8 ? 10 : 5) - (NT - 1) * (FP8 ? 2 : 1);
     static constexpr int kOutAt = kStages * 2 * kTileBytes;             // [warp][row][D] floats
     static constexpr int kMlAt = kOutAt + kWarps * kRows * kPitch * 4;  // [warp][row] (m, l)
-    static constexpr int kPartAt = kMlAt + kWarps * kRows * 8;
+    static constexpr int kQPitch = 2 * D + 16;  // bytes of a row of q
+    static constexpr int kQAt = kMlAt + kWarps * kRows * 8;             // [2][row] q as F16 or BF16
+    static constexpr int kCqAt = kQAt + 2 * kRows * kQPitch;            // [2][row] factors
+    static constexpr int kPartAt = kCqAt + 2 * kRows * 4;
     static constexpr int kBarAt = kPartAt + kParts * static_cast<int>(sizeof(Part));
-    static constexpr int kSmem = 1024 + kBarAt + (2 * kStages + 2 * kParts + 2) * 8 + 32;
+    static constexpr int kSmem = 1024 + kBarAt + (2 * kStages + 2 * kParts + 6) * 8 + 32;
 };
 
 // d = a (16 x 16, row) * b (16 x 8, col) + d, F16 in, F32 accumulate
@@ -89,21 +94,27 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
     uint64_t* pt_empty = pt_full + kParts;
     uint64_t* x_in = pt_empty + kParts;  // every warp's share of a part is in shared memory
     uint64_t* x_out = x_in + 1;          // and has been read
-    int* s_abort = reinterpret_cast<int*>(x_out + 1);
+    uint64_t* q_full = x_out + 1;        // [2] a part's q
+    uint64_t* q_empty = q_full + 2;
+    int* s_abort = reinterpret_cast<int*>(q_empty + 2);
     int* s_bad = s_abort + 1;            // [4], of the part in turn: a drafted row's value is not finite
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 4);
+            mbar_init(&empty[s], 2);
         }
         for (int s = 0; s < kParts; ++s) {
             mbar_init(&pt_full[s], 1);
-            mbar_init(&pt_empty[s], kWarps);
+            mbar_init(&pt_empty[s], kWarps + G_::kAux);
         }
         mbar_init(x_in, kWarps);
-        mbar_init(x_out, kWarps);
+        mbar_init(x_out, G_::kAux);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&q_full[s], G_::kAux);
+            mbar_init(&q_empty[s], kWarps);
+        }
         *s_abort = 0;
         for (int s = 0; s < 4; ++s) s_bad[s] = 0;
         s_share.pairs = 0;
@@ -173,82 +184,157 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                 while (!mbar_try_wait(&full[j % NS], (j / NS) & 1u) && globaltimer_ns() - t < NF_WAIT_BUDGET_NS) {
                 }
             }
+    } else if (warp > kWarps) {
+        // ------------------------------------------------ q, and the join
+        const int tid = threadIdx.x - 32 * (kWarps + 1);
+        constexpr int kCount = 32 * G_::kAux, C = D / 8;  // 16-byte chunks of a row of q
+        const float* s_out = reinterpret_cast<const float*>(sm + G_::kOutAt);
+        const float2* s_ml = reinterpret_cast<const float2*>(sm + G_::kMlAt);
+#pragma unroll 1
+        for (int idx = 0;; ++idx) {
+            wait(&pt_full[idx % kParts], (idx / kParts) & 1u);
+            const bool more = !*abort_flag && s_part[idx % kParts].rows > 0;
+            if (more) {
+                const Part& w = s_part[idx % kParts];
+                const int b = idx & 1;
+                if (idx >= 2) wait(&q_empty[b], ((idx >> 1) & 1u) ^ 1u);
+#pragma unroll
+                for (int e = tid; e < kRows * C; e += kCount) {
+                    const int r = e / C, ch = e % C, row = w.row0 + r, node = row / a.G;
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (r < w.rows)
+                        v = *reinterpret_cast<const uint4*>(
+                            a.q + (static_cast<int64_t>(w.first + node) * a.nq + w.g * a.G + (row - node * a.G)) * D + 8 * ch);
+                    float mine = a.c;
+                    if (FP8) {
+                        // the row's largest exponent to 2^0: what F16 then loses is below 2^-24 of the row's maximum
+                        uint32_t in[4] = {v.x, v.y, v.z, v.w}, top = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top = max(top, max(in[k] & 0x7f80u, (in[k] >> 16) & 0x7f80u));
+#pragma unroll
+                        for (int o = 1; o < C; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const int ex = top == 0 || top == 0x7f80u ? 127 : min(static_cast<int>(top >> 7), 253);
+                        const float down = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+                        mine = a.c * __uint_as_float(static_cast<uint32_t>(ex) << 23);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            in[k] = pack_f16x2(__uint_as_float(in[k] << 16) * down, __uint_as_float(in[k] & 0xffff0000u) * down);
+                        v = make_uint4(in[0], in[1], in[2], in[3]);
+                    }
+                    *reinterpret_cast<uint4*>(sm + G_::kQAt + (b * kRows + r) * G_::kQPitch + 16 * ch) = v;
+                    if (ch == 0) reinterpret_cast<float*>(sm + G_::kCqAt)[b * kRows + r] = mine;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[b]);
+            }
+            if (idx > 0) {
+                // the part before: four dims of a row a thread
+                const int at = idx - 1;
+                const Part& w = s_part[at % kParts];
+                wait(x_in, at & 1u);
+                if (tid == 0) s_bad[(at + 2) & 3] = 0;
+                const int rows = w.rows;
+                const bool whole = w.kind == 3;
+                const int slot = 2 * blockIdx.x + (w.kind & 1);
+                const Work wk = work_at(a.work);
+#pragma unroll 1
+                for (int e = tid; e < rows * (D / 4); e += kCount) {
+                    const int r = e / (D / 4), d = e % (D / 4) * 4;
+                    float2 ml[kWarps];
+                    float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+                    for (int k = 0; k < kWarps; ++k) {
+                        ml[k] = s_ml[k * kRows + r];
+                        mt = fmaxf(mt, ml[k].x);
+                    }
+                    const float mu = mt == -INFINITY ? 0.f : mt;
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int k = 0; k < kWarps; ++k) {
+                        const float4 x = *reinterpret_cast<const float4*>(s_out + (k * kRows + r) * kPitch + d);
+                        const float g = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ex2(ml[k].x - mu);
+                        lt += ml[k].y * g;
+                        acc.x += g == 0.f ? 0.f : x.x * g;
+                        acc.y += g == 0.f ? 0.f : x.y * g;
+                        acc.z += g == 0.f ? 0.f : x.z * g;
+                        acc.w += g == 0.f ? 0.f : x.w * g;
+                    }
+                    const int row = w.row0 + r, nd = row / a.G;
+                    if (s_bad[at & 3] && poisoned<D, FP8>(a, w.z, w.p0, w.n, w.first, nd)) lt = NAN;
+                    if (whole) {
+                        const float iv = lt == 0.f ? 0.f : 1.f / lt;
+                        uint16_t* dst = a.out + (static_cast<int64_t>(w.first + nd) * a.nq + w.g * a.G + (row - nd * a.G)) * D + d;
+                        *reinterpret_cast<uint2*>(dst) =
+                            make_uint2(bf16x2_hw(acc.x * iv, acc.y * iv), bf16x2_hw(acc.z * iv, acc.w * iv));
+                    } else {
+                        const int64_t to = static_cast<int64_t>(slot) * kItemRows + r;
+                        *reinterpret_cast<float4*>(wk.acc + to * D + d) = acc;
+                        if (d == 0) wk.ml[to] = make_float2(mu, lt);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(x_out);
+                    mbar_arrive(&pt_empty[at % kParts]);
+                }
+            }
+            if (!more) break;
+        }
     } else {
-        // ------------------------------------------------ 16 keys of a tile
+        // ------------------------------------------------ 32 keys of a tile
         // Fragment coordinates: of S^T and O^T a thread holds rows 2 t4, 2 t4 + 1 of a column tile for keys (dims)
         // grp and grp + 8.
         const int grp = lane >> 2, t4 = lane & 3;
         const int mi = lane >> 3, mr = lane & 7;  // ldmatrix: the lane's matrix and row
-        const int key0 = 16 * (warp & 3);         // the warp's keys of a tile
+        const int key0 = 32 * (warp & 1);         // the warp's keys of a tile
         float* s_out = reinterpret_cast<float*>(sm + G_::kOutAt);
         float2* s_ml = reinterpret_cast<float2*>(sm + G_::kMlAt);
         uint32_t pos0 = 0;  // tiles before the part
-        // q's fragments, row 8 c + grp of column tile c.  Step s of the product covers dims 16 s .. + 15; with E4M3 a
-        // thread's codes are four neighbours, so its slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9 stand for dims 4 t .. 4 t + 3.
-        uint32_t qb[NT][D / 16][2];
-        auto load_q = [&](const Part& w) {
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-                const int r = 8 * c + grp, row = w.row0 + r, node = row / a.G;
-                const uint16_t* q = a.q + (static_cast<int64_t>(w.first + node) * a.nq + w.g * a.G + (row - node * a.G)) * D;
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s) {
-                    uint2 v = make_uint2(0u, 0u);
-                    if (r < w.rows) {
-                        if (FP8) v = *reinterpret_cast<const uint2*>(q + 16 * s + 4 * t4);
-                        else v = make_uint2(*reinterpret_cast<const uint32_t*>(q + 16 * s + 2 * t4),
-                                            *reinterpret_cast<const uint32_t*>(q + 16 * s + 2 * t4 + 8));
-                    }
-                    qb[c][s][0] = v.x;
-                    qb[c][s][1] = v.y;
-                }
-            }
+        wait(&pt_full[0], 0);
+        // E4M3: the scales of the warp's next 32 keys, one a lane
+        float ksc = 0.f, vsc = 0.f;
+        auto fetch = [&](const Part& w, int t) {
+            const int key = t * kKeys + key0 + lane;
+            const bool in = t < w.t1 && key < w.p0 + w.n;
+            const int64_t at = static_cast<int64_t>(w.z) * a.L + key;
+            ksc = in ? __ldg(a.k_scale + at) : 0.f;
+            vsc = in ? __ldg(a.v_scale + at) : 0.f;
         };
+        // a part's first tile of this warp: every kGroups-th in the order of all tiles
+        auto first_tile = [&](const Part& w) { return w.t0 + static_cast<int>(((warp >> 1) - pos0) % G_::kGroups); };
+        if (FP8 && !*abort_flag) fetch(s_part[0], first_tile(s_part[0]));
 #pragma unroll 1
         for (int idx = 0;; ++idx) {
             const Part& w = s_part[idx % kParts];
-            if (idx == 0) {
-                wait(&pt_full[0], 0);
-                if (!*abort_flag && w.rows > 0) load_q(w);
-            }
             if (*abort_flag || w.rows == 0) break;
             const int rows = w.rows, t1 = w.t1, first = w.first, p0 = w.p0, n = w.n, end = p0 + n;
-            // this warp's tiles: every kGroups-th
-            const int t_first = w.t0 + static_cast<int>(((warp >> 2) - pos0) % G_::kGroups);
-            const int64_t zrow = static_cast<int64_t>(w.z) * a.L;
-            // E4M3: lanes 0-15 hold the scales of the warp's 16 keys, lanes 16-31 the values' scales
-            float sc = 0.f;
-            auto fetch = [&](int t) {
-                const int key = t * kKeys + key0 + (lane & 15);
-                return key < end ? __ldg((lane < 16 ? a.k_scale : a.v_scale) + zrow + key) : 0.f;
-            };
-            if (FP8 && t_first < t1) sc = fetch(t_first);
+            const int t_first = first_tile(w);
+            // q's fragments, row 8 c + grp of column tile c.  Step s of the product covers dims 16 s .. + 15; with E4M3
+            // a thread's codes are four neighbours, so its slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9 stand for dims 4 t .. + 3.
+            uint32_t qb[NT][D / 16][2];
             float cq[NT][2];
+            wait(&q_full[idx & 1], (idx >> 1) & 1u);
+            __syncwarp();
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
-                float mine = a.c;
-                if (FP8) {
-                    // the row's largest exponent to 2^0: what F16 then loses is below 2^-24 of the row's maximum
-                    uint32_t top = 0;
+                const uint8_t* q = sm + G_::kQAt + ((idx & 1) * kRows + 8 * c + grp) * G_::kQPitch;
 #pragma unroll
-                    for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) top = max(top, max(qb[c][s][e] & 0x7f80u, (qb[c][s][e] >> 16) & 0x7f80u));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const int e = top == 0 || top == 0x7f80u ? 127 : min(static_cast<int>(top >> 7), 253);
-                    const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-                    mine = a.c * __uint_as_float(static_cast<uint32_t>(e) << 23);
-#pragma unroll
-                    for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-                        for (int f = 0; f < 2; ++f)
-                            qb[c][s][f] = pack_f16x2(__uint_as_float(qb[c][s][f] << 16) * down,
-                                                     __uint_as_float(qb[c][s][f] & 0xffff0000u) * down);
+                for (int s = 0; s < D / 16; ++s) {
+                    if (FP8) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(q + 32 * s + 8 * t4);
+                        qb[c][s][0] = v.x;
+                        qb[c][s][1] = v.y;
+                    } else {
+                        qb[c][s][0] = *reinterpret_cast<const uint32_t*>(q + 32 * s + 4 * t4);
+                        qb[c][s][1] = *reinterpret_cast<const uint32_t*>(q + 32 * s + 4 * t4 + 16);
+                    }
                 }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) cq[c][e] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t4 + e));
+                const float2 f = *reinterpret_cast<const float2*>(sm + G_::kCqAt + ((idx & 1) * kRows + 8 * c + 2 * t4) * 4);
+                cq[c][0] = f.x;
+                cq[c][1] = f.y;
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_empty[idx & 1]);
             float o[NT][D / 16][4];
 #pragma unroll
             for (int c = 0; c < NT; ++c)
@@ -271,87 +357,92 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
             for (int t = t_first; t < t1; t += G_::kGroups) {
                 const uint32_t pos = pos0 + static_cast<uint32_t>(t - w.t0);
                 const int s = static_cast<int>(pos % NS);
-                const float my = sc;
-                if (FP8 && t + G_::kGroups < t1) sc = fetch(t + G_::kGroups);
+                const float my_k = ksc, my_v = vsc;
+                if (FP8) fetch(w, t + G_::kGroups);
                 wait(&full[s], (pos / NS) & 1u);
                 __syncwarp();
                 const int k0 = t * kKeys + key0;  // the warp's first key
                 if (k0 < end) {
                     const uint32_t kt = smem_u32(sm + s * 2 * G_::kTileBytes), vt = kt + G_::kTileBytes;
-                    const bool tail = k0 + 16 > p0;
-                    // ---- S^T: two chains of products for each column tile
+                    const bool tail = k0 + 32 > p0;
+                    // ---- S^T of 16 keys (b), twice
                     float x[NT][2][4];
 #pragma unroll
                     for (int c = 0; c < NT; ++c)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[c][0][e] = x[c][1][e] = 0.f;
-                    const int key = key0 + 8 * (mi & 1) + mr;
 #pragma unroll
-                    for (int i = 0; i < D / 16; i += FP8 ? 2 : 1) {
-                        uint32_t b[4];
-                        if (FP8) {
-                            // 16-byte chunks i and i + 1 (a step's 16 codes) of keys 0-7 and 8-15
-                            const uint32_t ch = i + (mi >> 1);
-                            ldsm_x4(kt + key * D + ((D == 128 ? ch ^ (key & 7) : ch ^ ((key >> 1) & 3)) << 4), b);
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t a0 = e4m3x2_to_f16x2(b[2 * e]), a2 = e4m3x2_to_f16x2(b[2 * e] >> 16);
-                                const uint32_t a1 = e4m3x2_to_f16x2(b[2 * e + 1]), a3 = e4m3x2_to_f16x2(b[2 * e + 1] >> 16);
-#pragma unroll
-                                for (int c = 0; c < NT; ++c) mma_f16(x[c][e], a0, a1, a2, a3, qb[c][i + e][0], qb[c][i + e][1]);
-                            }
-                        } else {
-                            const int ch = 2 * i + (mi >> 1);
-                            ldsm_x4(kt + (ch >> 3) * kKeys * 128 + key * 128 + (((ch & 7) ^ (key & 7)) << 4), b);
-#pragma unroll
-                            for (int c = 0; c < NT; ++c) mma_16816(x[c][i & 1], b[0], b[1], b[2], b[3], qb[c][i][0], qb[c][i][1]);
-                        }
-                    }
-                    // ---- x = c q . k; element e: key grp + 8 (e / 2), row 2 t4 + (e & 1)
-                    float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
-                    if (FP8)
+                    for (int i = 0; i < D / 16; i += FP8 ? 2 : 1)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            ks[h] = __shfl_sync(0xffffffffu, my, grp + 8 * h);
-                            vs[h] = __shfl_sync(0xffffffffu, my, 16 + grp + 8 * h);
+                            const int key = key0 + 16 * h + 8 * (mi & 1) + mr;
+                            uint32_t b[4];
+                            if (FP8) {
+                                // 16-byte chunks i and i + 1 (a step's 16 codes) of keys 0-7 and 8-15
+                                const uint32_t ch = i + (mi >> 1);
+                                ldsm_x4(kt + key * D + ((D == 128 ? ch ^ (key & 7) : ch ^ ((key >> 1) & 3)) << 4), b);
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const uint32_t a0 = e4m3x2_to_f16x2(b[2 * e]), a2 = e4m3x2_to_f16x2(b[2 * e] >> 16);
+                                    const uint32_t a1 = e4m3x2_to_f16x2(b[2 * e + 1]), a3 = e4m3x2_to_f16x2(b[2 * e + 1] >> 16);
+#pragma unroll
+                                    for (int c = 0; c < NT; ++c) mma_f16(x[c][h], a0, a1, a2, a3, qb[c][i + e][0], qb[c][i + e][1]);
+                                }
+                            } else {
+                                const int ch = 2 * i + (mi >> 1);
+                                ldsm_x4(kt + (ch >> 3) * kKeys * 128 + key * 128 + (((ch & 7) ^ (key & 7)) << 4), b);
+#pragma unroll
+                                for (int c = 0; c < NT; ++c) mma_16816(x[c][h], b[0], b[1], b[2], b[3], qb[c][i][0], qb[c][i][1]);
+                            }
+                        }
+                    // ---- x = c q . k; element (h, e): key 16 h + grp + 8 (e / 2), row 2 t4 + (e & 1)
+                    float ks[4] = {1.f, 1.f, 1.f, 1.f}, vs[4] = {1.f, 1.f, 1.f, 1.f};
+                    if (FP8)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            ks[h] = __shfl_sync(0xffffffffu, my_k, grp + 8 * h);
+                            vs[h] = __shfl_sync(0xffffffffu, my_v, grp + 8 * h);
                             if (tail && k0 + grp + 8 * h >= p0 && !isfinite(vs[h])) {
                                 bad = true;
                                 vs[h] = 0.f;
                             }
                         }
-                    uint32_t pb[NT][2];
+                    uint32_t pb[NT][4];
                     bool scale = false;
                     float f[NT][2];
 #pragma unroll
                     for (int c = 0; c < NT; ++c) {
-                        float p[4];
+                        float p[4][2];  // [key grp + 8 h][row]
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) p[e] = (x[c][0][e] + x[c][1][e]) * (ks[e >> 1] * cq[c][e & 1]);
+                        for (int h = 0; h < 4; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) p[h][e] = x[c][h >> 1][2 * (h & 1) + e] * (ks[h] * cq[c][e]);
                         if (tail)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const int r = 8 * c + 2 * t4 + e, node = (w.row0 + r) / a.G;
-                                const uint32_t vis = visible(a, first + node, node, n, k0 - p0, r < rows);
-                                if (!((vis >> grp) & 1u)) p[e] = -INFINITY;
-                                if (!((vis >> (grp + 8)) & 1u)) p[2 + e] = -INFINITY;
+                                const uint32_t vis = visible(a, first + node, node, n, k0 - p0, r < rows) >> grp;
+#pragma unroll
+                                for (int h = 0; h < 4; ++h)
+                                    if (!((vis >> (8 * h)) & 1u)) p[h][e] = -INFINITY;
                             }
                         // ---- the rows' running maximum, sum and weights
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float mx = fmaxf(p[e], p[2 + e]);
+                            float mx = fmaxf(fmaxf(p[0][e], p[1][e]), fmaxf(p[2][e], p[3][e]));
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                             const float mn = fmaxf(m[c][e], mx), mu = mn == -INFINITY ? 0.f : mn;
                             f[c][e] = m[c][e] == -INFINITY ? 0.f : ex2(m[c][e] - mu);
                             m[c][e] = mn;
-                            p[e] = ex2(p[e] - mu);
-                            p[2 + e] = ex2(p[2 + e] - mu);
-                            l[c][e] = l[c][e] * f[c][e] + (p[e] + p[2 + e]);
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) p[h][e] = ex2(p[h][e] - mu);
+                            l[c][e] = l[c][e] * f[c][e] + ((p[0][e] + p[1][e]) + (p[2][e] + p[3][e]));
                             if (FP8) {
-                                p[e] *= vs[0];
-                                p[2 + e] *= vs[1];
-                                float wm = fmaxf(fabsf(p[e]), fabsf(p[2 + e]));
+#pragma unroll
+                                for (int h = 0; h < 4; ++h) p[h][e] *= vs[h];
+                                float wm = fmaxf(fmaxf(fabsf(p[0][e]), fabsf(p[1][e])), fmaxf(fabsf(p[2][e]), fabsf(p[3][e])));
                                 wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 4));
                                 wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 8));
                                 wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 16));
@@ -363,14 +454,14 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                                     f[c][e] *= fminf(to / inv[c][e], 1.7e38f);
                                     inv[c][e] = to;
                                 }
-                                p[e] *= inv[c][e];
-                                p[2 + e] *= inv[c][e];
+#pragma unroll
+                                for (int h = 0; h < 4; ++h) p[h][e] *= inv[c][e];
                             }
                             scale |= f[c][e] != 1.f;
                         }
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            pb[c][h] = transpose8(FP8 ? pack_f16x2(p[2 * h], p[2 * h + 1]) : pack_bf16x2(p[2 * h], p[2 * h + 1]));
+                        for (int h = 0; h < 4; ++h)
+                            pb[c][h] = transpose8(FP8 ? pack_f16x2(p[h][0], p[h][1]) : pack_bf16x2(p[h][0], p[h][1]));
                     }
                     if (__any_sync(0xffffffffu, scale))
 #pragma unroll
@@ -379,35 +470,41 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                             for (int i = 0; i < D / 16; ++i)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) o[c][i][e] *= f[c][e & 1];
-                    // ---- O^T += V^T P^T over the warp's 16 keys
-                    const int kk = k0 + 2 * t4;
+                    // ---- O^T += V^T P^T over the warp's keys
 #pragma unroll
-                    for (int i = 0; i < D / 16; i += FP8 ? 2 : 1) {
-                        uint32_t b[4];
-                        if (FP8) {
-                            // chunks i and i + 1 of keys 0-7 and 8-15, pairs of codes transposed: a register holds dims
-                            // 2 grp and 2 grp + 1 (the tile's rows grp and grp + 8) of keys 2 t4 and 2 t4 + 1
-                            const uint32_t ch = i + (mi >> 1);
-                            ldsm_x4_t(vt + key * D + ((D == 128 ? ch ^ (key & 7) : ch ^ ((key >> 1) & 3)) << 4), b);
+                    for (int h = 0; h < 2; ++h) {
+                        const int kk = k0 + 16 * h + 2 * t4;
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t lo = __byte_perm(b[2 * e], 0u, 0x3120), hi = __byte_perm(b[2 * e + 1], 0u, 0x3120);
-                                uint32_t v[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi),
-                                                 e4m3x2_to_f16x2(hi >> 16)};
+                        for (int i = 0; i < D / 16; i += FP8 ? 2 : 1) {
+                            uint32_t b[4];
+                            if (FP8) {
+                                // chunks i and i + 1 of keys 0-7 and 8-15, pairs of codes transposed: a register holds
+                                // dims 2 grp and 2 grp + 1 (the tile's rows grp and grp + 8) of keys 2 t4 and 2 t4 + 1
+                                const uint32_t ch = i + (mi >> 1);
+                                const int key = key0 + 16 * h + 8 * (mi & 1) + mr;
+                                ldsm_x4_t(vt + key * D + ((D == 128 ? ch ^ (key & 7) : ch ^ ((key >> 1) & 3)) << 4), b);
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const uint32_t lo = __byte_perm(b[2 * e], 0u, 0x3120), hi = __byte_perm(b[2 * e + 1], 0u, 0x3120);
+                                    uint32_t v[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi),
+                                                     e4m3x2_to_f16x2(hi >> 16)};
+                                    if (tail)
+#pragma unroll
+                                        for (int g = 0; g < 4; ++g) v[g] = clean<FP8>(v[g], kk + 8 * (g >> 1), p0, end, bad);
+#pragma unroll
+                                    for (int c = 0; c < NT; ++c)
+                                        mma_f16(o[c][i + e], v[0], v[1], v[2], v[3], pb[c][2 * h], pb[c][2 * h + 1]);
+                                }
+                            } else {
+                                const int key = key0 + 16 * h + 8 * (mi >> 1) + mr, ch = 2 * i + (mi & 1);
+                                ldsm_x4_t(vt + (ch >> 3) * kKeys * 128 + key * 128 + (((ch & 7) ^ (key & 7)) << 4), b);
                                 if (tail)
 #pragma unroll
-                                    for (int h = 0; h < 4; ++h) v[h] = clean<FP8>(v[h], kk + 8 * (h >> 1), p0, end, bad);
+                                    for (int g = 0; g < 4; ++g) b[g] = clean<FP8>(b[g], kk + 8 * (g >> 1), p0, end, bad);
 #pragma unroll
-                                for (int c = 0; c < NT; ++c) mma_f16(o[c][i + e], v[0], v[1], v[2], v[3], pb[c][0], pb[c][1]);
+                                for (int c = 0; c < NT; ++c)
+                                    mma_16816(o[c][i], b[0], b[1], b[2], b[3], pb[c][2 * h], pb[c][2 * h + 1]);
                             }
-                        } else {
-                            const int vkey = key0 + 8 * (mi >> 1) + mr, ch = 2 * i + (mi & 1);
-                            ldsm_x4_t(vt + (ch >> 3) * kKeys * 128 + vkey * 128 + (((ch & 7) ^ (vkey & 7)) << 4), b);
-                            if (tail)
-#pragma unroll
-                                for (int h = 0; h < 4; ++h) b[h] = clean<FP8>(b[h], kk + 8 * (h >> 1), p0, end, bad);
-#pragma unroll
-                            for (int c = 0; c < NT; ++c) mma_16816(o[c][i], b[0], b[1], b[2], b[3], pb[c][0], pb[c][1]);
                         }
                     }
                 }
@@ -415,7 +512,13 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                 if (lane == 0) mbar_arrive(&empty[s]);
             }
             pos0 += static_cast<uint32_t>(t1 - w.t0);
-            // ---- the warps' outputs to shared memory, once all have read the part before's
+            {
+                // the next part's first scales are on their way meanwhile
+                const int r = (idx + 1) % kParts;
+                wait(&pt_full[r], ((idx + 1) / kParts) & 1u);
+                if (FP8 && !*abort_flag) fetch(s_part[r], first_tile(s_part[r]));
+            }
+            // ---- the warp's output to shared memory, once the part before's has been read
             if (bad) s_bad[idx & 3] = 1;
             if (idx > 0) wait(x_out, (idx - 1) & 1u);
             __syncwarp();
@@ -443,56 +546,8 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                     }
                 }
             __syncwarp();
-            if (lane == 0) mbar_arrive(x_in);
-            // the next part's q is on its way meanwhile
-            {
-                const int r = (idx + 1) % kParts;
-                wait(&pt_full[r], ((idx + 1) / kParts) & 1u);
-                if (!*abort_flag && s_part[r].rows > 0) load_q(s_part[r]);
-            }
-            wait(x_in, idx & 1u);
-            __syncwarp();
-            // ---- and joined, four dims of a row a thread
-            if (threadIdx.x == 0) s_bad[(idx + 2) & 3] = 0;
-            const bool whole = w.kind == 3;
-            const int slot = 2 * blockIdx.x + (w.kind & 1);
-            const Work wk = work_at(a.work);
-#pragma unroll 1
-            for (int e = threadIdx.x; e < rows * (D / 4); e += 32 * kWarps) {
-                const int r = e / (D / 4), d = e % (D / 4) * 4;
-                float mt = -INFINITY, lt = 0.f;
-#pragma unroll
-                for (int k = 0; k < kWarps; ++k) mt = fmaxf(mt, s_ml[k * kRows + r].x);
-                const float mu = mt == -INFINITY ? 0.f : mt;
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                for (int k = 0; k < kWarps; ++k) {
-                    const float2 v = s_ml[k * kRows + r];
-                    const float4 x = *reinterpret_cast<const float4*>(s_out + (k * kRows + r) * kPitch + d);
-                    const float g = v.x == -INFINITY && v.y == 0.f ? 0.f : ex2(v.x - mu);
-                    lt += v.y * g;
-                    if (g != 0.f) {
-                        acc.x = fmaf(x.x, g, acc.x);
-                        acc.y = fmaf(x.y, g, acc.y);
-                        acc.z = fmaf(x.z, g, acc.z);
-                        acc.w = fmaf(x.w, g, acc.w);
-                    }
-                }
-                const int row = w.row0 + r, nd = row / a.G;
-                if (s_bad[idx & 3] && poisoned<D, FP8>(a, w.z, p0, n, first, nd)) lt = NAN;
-                if (whole) {
-                    const float iv = lt == 0.f ? 0.f : 1.f / lt;
-                    uint16_t* dst = a.out + (static_cast<int64_t>(first + nd) * a.nq + w.g * a.G + (row - nd * a.G)) * D + d;
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(bf16x2_hw(acc.x * iv, acc.y * iv), bf16x2_hw(acc.z * iv, acc.w * iv));
-                } else {
-                    const int64_t at = static_cast<int64_t>(slot) * kItemRows + r;
-                    *reinterpret_cast<float4*>(wk.acc + at * D + d) = acc;
-                    if (d == 0) wk.ml[at] = make_float2(mu, lt);
-                }
-            }
-            __syncwarp();
             if (lane == 0) {
-                mbar_arrive(x_out);
+                mbar_arrive(x_in);
                 mbar_arrive(&pt_empty[idx % kParts]);
             }
         }
