@@ -58,20 +58,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Clears the 16-bit halves of a pair of keys (k, k + 1) that lie behind the
-// sequence, or that are not finite in a drafted row (which is noted).
-template <bool FP8>
-__device__ __forceinline__ uint32_t clean(uint32_t v, int k, int node, int end, bool& bad) {
-    constexpr uint32_t kExp = FP8 ? 0x7c00u : 0x7f80u;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const bool inf = ((v >> (16 * h)) & kExp) == kExp && k + h >= node && k + h < end;
-        bad |= inf;
-        if (inf || k + h >= end) v &= h ? 0x0000ffffu : 0xffff0000u;
-    }
-    return v;
-}
-
 // An 8 x 8 matrix of 16-bit values held as fragments, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
@@ -365,6 +351,32 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                 if (k0 < end) {
                     const uint32_t kt = smem_u32(sm + s * 2 * G_::kTileBytes), vt = kt + G_::kTileBytes;
                     const bool tail = k0 + 32 > p0;
+                    if (__builtin_expect(tail, 0)) {
+                        // V's rows behind the sequence, and drafted rows that are not finite (which is noted), become
+                        // zeros: a zero probability must not meet a NaN.  A lane has a key's row.
+                        const int row = key0 + lane, at = k0 + lane;
+                        uint8_t* v = sm + s * 2 * G_::kTileBytes + G_::kTileBytes;
+                        constexpr int kRowBytes = D * (FP8 ? 1 : 2), kBox = FP8 ? kRowBytes : 128;
+                        bool zero = at >= end;
+                        if (at >= p0 && at < end)
+#pragma unroll 1
+                            for (int c = 0; c < kRowBytes / 16; ++c) {  // chunks in any order: the swizzle stays in the row
+                                const uint4 x = *reinterpret_cast<const uint4*>(v + c * 16 / kBox * (kKeys * kBox) + row * kBox + c * 16 % kBox);
+                                const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)  // an exponent of all ones (E4M3: 0x7f) carries into the sign's place
+                                    zero |= FP8 ? (((in[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0
+                                                : (((in[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
+                            }
+                        if (zero) {
+                            bad |= at < end;
+#pragma unroll 1
+                            for (int c = 0; c < kRowBytes / 16; ++c)
+                                *reinterpret_cast<uint4*>(v + c * 16 / kBox * (kKeys * kBox) + row * kBox + c * 16 % kBox) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async();  // before TMA writes here again
+                        __syncwarp();
+                    }
                     // ---- S^T of 16 keys (b), twice
                     float x[NT][2][4];
 #pragma unroll
@@ -417,7 +429,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                         for (int h = 0; h < 4; ++h)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) p[h][e] = x[c][h >> 1][2 * (h & 1) + e] * (ks[h] * cq[c][e]);
-                        if (tail)
+                        if (__builtin_expect(tail, 0))
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const int r = 8 * c + 2 * t4 + e, node = (w.row0 + r) / a.G;
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                                 wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 16));
                                 ref[c][e] = fmaxf(ref[c][e] * f[c][e], wm);
                                 const float top = ref[c][e] * inv[c][e];
-                                if (ref[c][e] > 0.f && !(top >= 0.0625f && top <= 32768.f)) {
+                                if (__builtin_expect(ref[c][e] > 0.f && !(top >= 0.0625f && top <= 32768.f), 0)) {
                                     const int ex = min(max(258 - static_cast<int>(__float_as_uint(ref[c][e]) >> 23), 7), 247);
                                     const float to = __uint_as_float(static_cast<uint32_t>(ex) << 23);
                                     f[c][e] *= fminf(to / inv[c][e], 1.7e38f);
@@ -463,7 +475,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                         for (int h = 0; h < 4; ++h)
                             pb[c][h] = transpose8(FP8 ? pack_f16x2(p[h][0], p[h][1]) : pack_bf16x2(p[h][0], p[h][1]));
                     }
-                    if (__any_sync(0xffffffffu, scale))
+                    if (__builtin_expect(__any_sync(0xffffffffu, scale), 0))
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -473,7 +485,6 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                     // ---- O^T += V^T P^T over the warp's keys
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int kk = k0 + 16 * h + 2 * t4;
 #pragma unroll
                         for (int i = 0; i < D / 16; i += FP8 ? 2 : 1) {
                             uint32_t b[4];
@@ -486,11 +497,8 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
                                     const uint32_t lo = __byte_perm(b[2 * e], 0u, 0x3120), hi = __byte_perm(b[2 * e + 1], 0u, 0x3120);
-                                    uint32_t v[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi),
-                                                     e4m3x2_to_f16x2(hi >> 16)};
-                                    if (tail)
-#pragma unroll
-                                        for (int g = 0; g < 4; ++g) v[g] = clean<FP8>(v[g], kk + 8 * (g >> 1), p0, end, bad);
+                                    const uint32_t v[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi),
+                                                           e4m3x2_to_f16x2(hi >> 16)};
 #pragma unroll
                                     for (int c = 0; c < NT; ++c)
                                         mma_f16(o[c][i + e], v[0], v[1], v[2], v[3], pb[c][2 * h], pb[c][2 * h + 1]);
@@ -498,9 +506,6 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                             } else {
                                 const int key = key0 + 16 * h + 8 * (mi >> 1) + mr, ch = 2 * i + (mi & 1);
                                 ldsm_x4_t(vt + (ch >> 3) * kKeys * 128 + key * 128 + (((ch & 7) ^ (key & 7)) << 4), b);
-                                if (tail)
-#pragma unroll
-                                    for (int g = 0; g < 4; ++g) b[g] = clean<FP8>(b[g], kk + 8 * (g >> 1), p0, end, bad);
 #pragma unroll
                                 for (int c = 0; c < NT; ++c)
                                     mma_16816(o[c][i], b[0], b[1], b[2], b[3], pb[c][2 * h], pb[c][2 * h + 1]);
