@@ -501,19 +501,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             y[2 * j + h] = bf16x2_hw(lo, hi);
                         }
                 };
+#pragma unroll 1
+                for (int b = 0; b < C; b += 2) {
+                    uint4 x[2];
 #pragma unroll
-                for (int b = 0; b < C; b += 4) {
-                    uint4 x[4];
+                    for (int j = 0; j < 2; ++j) x[j] = *reinterpret_cast<const uint4*>(src + ((b + j) * 128 + tid) * 16);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4*>(src + ((b + j) * 128 + tid) * 16);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 2; ++j) {
                         uint32_t y[8];
                         widen(x[j], y);
                         put((b + j) * 128 + tid, y);
                     }
                 }
-                if (tail) {
+                if (__builtin_expect(tail, 0)) {
                     // V's rows behind the sequence, and a node's chunks that hold a NaN, become zeros
 #pragma unroll 1
                     for (int e = tid; e < C * 128; e += 128) {
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 if (active) {
                     tc_fence_after();
                     uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-                    if (tail)
+                    if (__builtin_expect(tail, 0))
 #pragma unroll
                         for (int c = 0; c < 4; ++c) vis[c] = visible(a, w.first + node, node, n, t * kKeys + 32 * c - p0, r < rows);
                     // x = S * factor: the whole row of the tile in registers
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         x[j + 2] = f32x2_lo(y1);
                         x[j + 3] = f32x2_hi(y1);
                     }
-                    if (tail)
+                    if (__builtin_expect(tail, 0))
 #pragma unroll
                         for (int j = 0; j < kKeys; ++j) x[j] = (vis[j >> 5] >> (j & 31)) & 1 ? x[j] : -INFINITY;
                     float mx4[4] = {x[0], x[1], x[2], x[3]};
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], x[j + 2 * e], x[j + 2 * e + 1]);
                     const float mx = fmaxf(max3(max3(mx4[0], x[kKeys - 4], x[kKeys - 3]), mx4[1], mx4[2]),
                                            max3(mx4[3], x[kKeys - 2], x[kKeys - 1]));
-                    if (__any_sync(0xffffffffu, done == 0 || mx > m + kRescale)) {
+                    if (__builtin_expect(__any_sync(0xffffffffu, done == 0 || mx > m + kRescale), 0)) {
                         const float mn = fmaxf(m, mx);
                         const float f = m == -INFINITY ? 0.f : ex2(m - mn);
                         if (done > 0) {
