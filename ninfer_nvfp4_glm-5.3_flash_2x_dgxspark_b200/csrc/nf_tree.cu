@@ -44,23 +44,59 @@ __device__ __forceinline__ uint32_t elect_one() {
 }
 // 32 lanes x 32 consecutive 32-bit columns
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, "
+                 "%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+
+  // 16 lanes x 128 columns as matrix fragments: thread t holds columns 8 i + 2 (t % 4) and + 1 of lane t / 4 in r[4 i] and
+// r[4 i + 1], and of lane t / 4 + 8 in r[4 i + 2] and r[4 i + 3].
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, "
+                 "%51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+                   "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+                   "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+                   "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+                   "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr)
+                 : "memory");
+}
+// The same of 16 columns.
+__device__ __forceinline__ void tmem_ld_frag16(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_frag16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// 16 lanes x 64 columns: thread t's column 4 i + t % 4 of lane t / 4 in r[2 i], of lane t / 4 + 8 in r[2 i + 1].
+__device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+                 "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, "
+                 "%31, %32};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                   "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+                   "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+                   "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D[tmem] (+)= A[tmem, BF16 pairs] * B[smem], K = 16 per instruction
@@ -192,7 +228,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         mbar_init(ml_out, 8);
         mbar_init(drained, 1);
         *s_abort = 0;
-        s_share.pairs = 0;
         for (int s = 0; s < kBadRing; ++s) s_bad[s] = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmk);
@@ -206,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
     TileInfo* s_info = reinterpret_cast<TileInfo*>(sm + G_::kInfoAt);
     using ItemWalk = Walk<kItemRows, kKeys>;
-    const Share share = find_share<D, kThreads, ItemWalk>(a, s_share);
+    const Share share = find_share<D, kThreads, 2, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;
     const uint32_t tmem = *s_tmem;
     volatile int* abort_flag = s_abort;
@@ -589,100 +624,122 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const int rows = min(kTileRows, w.rows - row0);
             const bool active = (warp & 3) * 32 < rows;
             const int row = w.row0 + row0 + r, node = row / a.G;
-            float m = -INFINITY, l = 0.f;
+            // A thread holds a quarter of the columns of rows lane / 4 and + 8 of either half (16 lanes) of the warp's
+            // rows, as matrix fragments: so it needs 32 of a tile's 128 scales.  The half at hand's (max, sum) and the
+            // other's change places.
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, mo[2] = {-INFINITY, -INFINITY}, lo[2] = {0.f, 0.f};
+            const int mine_rows = rows - (warp & 3) * 32;  // rows of this warp
             int done = 0;
             for (int t = w.t0 + (pair ? 0 : mine0); t < t1; t += pair ? 1 : 2, ++mine_n, ++done) {
                 const uint32_t b = mine_n & 1;
-                const float* sc = reinterpret_cast<const float*>(sm + G_::kScaleAt) + (2 * s + b) * 2 * kKeys;
+                const float* sc = reinterpret_cast<const float*>(sm + G_::kScaleAt) + (2 * s + b) * 2 * kKeys + 2 * (lane & 3);
                 wait(&s_full[s], mine_n & 1u);
                 if (FP8) wait(&sc_full[2 * s + b], (mine_n >> 1) & 1u);
                 __syncwarp();
+                tc_fence_after();
                 const bool tail = (t + 1) * kKeys > p0;
-                if (active) {
-                    tc_fence_after();
-                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-                    if (__builtin_expect(tail, 0))
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) vis[c] = visible(a, w.first + node, node, n, t * kKeys + 32 * c - p0, r < rows);
-                    // x = S * factor: the whole row of the tile in registers
-                    float x[kKeys];
-                    uint32_t* xb = reinterpret_cast<uint32_t*>(x);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, xb + 32 * c);
-                    tmem_wait_ld();
-                    const uint64_t c2 = f32x2_pack(a.c, a.c);
-#pragma unroll
-                    for (int j = 0; j < kKeys; j += 4) {
-                        uint64_t f0 = c2, f1 = c2;
-                        if (FP8) {
-                            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + j);
-                            f0 = f.x;
-                            f1 = f.y;
-                        }
-                        const uint64_t y0 = mul_f32x2(f32x2_pack(x[j], x[j + 1]), f0);
-                        const uint64_t y1 = mul_f32x2(f32x2_pack(x[j + 2], x[j + 3]), f1);
-                        x[j] = f32x2_lo(y0);
-                        x[j + 1] = f32x2_hi(y0);
-                        x[j + 2] = f32x2_lo(y1);
-                        x[j + 3] = f32x2_hi(y1);
-                    }
-                    if (__builtin_expect(tail, 0))
-#pragma unroll
-                        for (int j = 0; j < kKeys; ++j) x[j] = (vis[j >> 5] >> (j & 31)) & 1 ? x[j] : -INFINITY;
-                    float mx4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                    for (int j = 4; j < kKeys - 4; j += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], x[j + 2 * e], x[j + 2 * e + 1]);
-                    const float mx = fmaxf(max3(max3(mx4[0], x[kKeys - 4], x[kKeys - 3]), mx4[1], mx4[2]),
-                                           max3(mx4[3], x[kKeys - 2], x[kKeys - 1]));
-                    if (__builtin_expect(__any_sync(0xffffffffu, done == 0 || mx > m + kRescale), 0)) {
-                        const float mn = fmaxf(m, mx);
-                        const float f = m == -INFINITY ? 0.f : ex2(m - mn);
-                        if (done > 0) {
-                            // the products up to the previous task are complete: the scores' commit covers them
 #pragma unroll 1
-                            for (int c = 0; c < D / 16; ++c) {
-                                uint32_t v[16];
-                                tmem_ld16(t_o + 16 * c, v);
-                                tmem_wait_ld();
+                for (int half = 0; half < 2; ++half) {
+                    if (mine_rows > 16 * half) {
+                        const uint32_t lane0 = static_cast<uint32_t>(half) << 20;
+                        uint32_t v[64];
+                        tmem_ld_frag(t_s + lane0, v);
+                        tmem_wait_ld();
+                        // x = S * factor
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
-                                tmem_st16(t_o + 16 * c, v);
+                        for (int i = 0; i < 16; ++i) {
+                            const uint64_t f = FP8 ? *reinterpret_cast<const uint64_t*>(sc + 8 * i) : f32x2_pack(a.c, a.c);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint64_t y = mul_f32x2(
+                                    f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), f);
+                                v[4 * i + 2 * h] = __float_as_uint(f32x2_lo(y));
+                                v[4 * i + 2 * h + 1] = __float_as_uint(f32x2_hi(y));
                             }
-                            l *= f;
                         }
-                        m = mn;
-                    }
-                    const float mu = m == -INFINITY ? 0.f : m;
-                    const uint64_t nm = f32x2_pack(-mu, -mu);
-                    uint64_t sum = 0, sum1 = 0;
+                        if (__builtin_expect(tail, 0)) {
+                            const int ra = (warp & 3) * 32 + 16 * half + (lane >> 2);  // the thread's first row
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t pk[16];
+                            for (int h = 0; h < 2; ++h) {
+                                const int nd = (w.row0 + row0 + ra + 8 * h) / a.G;
 #pragma unroll
-                        for (int j = 32 * c; j < 32 * c + 32; j += 4) {
-                            const uint64_t y0 = add_f32x2(f32x2_pack(x[j], x[j + 1]), nm);
-                            const uint64_t y1 = add_f32x2(f32x2_pack(x[j + 2], x[j + 3]), nm);
-                            uint64_t p0 = f32x2_pack(ex2(f32x2_lo(y0)), ex2(f32x2_hi(y0)));
-                            uint64_t p1 = f32x2_pack(ex2(f32x2_lo(y1)), ex2(f32x2_hi(y1)));
-                            sum = add_f32x2(sum, p0);
-                            sum1 = add_f32x2(sum1, p1);
-                            if (FP8) {
-                                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + kKeys + j);
-                                p0 = mul_f32x2(p0, f.x);
-                                p1 = mul_f32x2(p1, f.y);
+                                for (int c = 0; c < 4; ++c) {
+                                    const uint32_t vis = visible(a, w.first + nd, nd, n, t * kKeys + 32 * c - p0, ra + 8 * h < rows) >>
+                                                         (2 * (lane & 3));
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                        for (int e = 0; e < 2; ++e)
+                                            if (!((vis >> (8 * i + e)) & 1u)) v[16 * c + 4 * i + 2 * h + e] = 0xff800000u;
+                                }
                             }
-                            pk[(j & 31) >> 1] = bf16x2_hw(f32x2_lo(p0), f32x2_hi(p0));
-                            pk[((j & 31) >> 1) + 1] = bf16x2_hw(f32x2_lo(p1), f32x2_hi(p1));
                         }
-                        tmem_st16(t_s + 16 * c, pk);
+                        float mn[2], f[2];
+                        bool grow = done == 0;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float mx[2] = {__uint_as_float(v[2 * h]), __uint_as_float(v[4 + 2 * h])};
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                mx[i & 1] = max3(mx[i & 1], __uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1]));
+                            float x = fmaxf(mx[0], mx[1]);
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                            mn[h] = fmaxf(m[h], x);
+                            grow |= x > m[h] + kRescale;
+                        }
+                        if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                f[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn[h]);
+                                m[h] = mn[h];
+                                l[h] *= f[h];
+                            }
+                            // the products up to the previous task are complete: the scores' commit covers them
+                            if (done > 0)
+#pragma unroll 1
+                                for (int c = 0; c < D; c += 16) {
+                                    uint32_t o[8];
+                                    tmem_ld_frag16(t_o + lane0 + c, o);
+                                    tmem_wait_ld();
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f[(k >> 1) & 1]);
+                                    tmem_st_frag16(t_o + lane0 + c, o);
+                                }
+                        }
+                        uint32_t pk[32];
+                        const float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
+                        const uint64_t nm[2] = {f32x2_pack(-mu0, -mu0), f32x2_pack(-mu1, -mu1)};
+                        uint64_t sum[2] = {0, 0};
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            uint64_t g = 0;
+                            if (FP8) g = *reinterpret_cast<const uint64_t*>(sc + kKeys + 8 * i);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint64_t y = add_f32x2(
+                                    f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), nm[h]);
+                                uint64_t pr = f32x2_pack(ex2(f32x2_lo(y)), ex2(f32x2_hi(y)));
+                                sum[h] = add_f32x2(sum[h], pr);
+                                if (FP8) pr = mul_f32x2(pr, g);
+                                pk[2 * i + h] = bf16x2_hw(f32x2_lo(pr), f32x2_hi(pr));
+                            }
+                        }
+                        tmem_st_pairs(t_s + lane0, pk);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) l[h] += f32x2_lo(sum[h]) + f32x2_hi(sum[h]);  // of the thread's columns
                     }
-                    sum = add_f32x2(sum, sum1);
-                    l += f32x2_lo(sum) + f32x2_hi(sum);
-                    tmem_wait_st();
-                    tc_fence_before();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float tm = m[h], tl = l[h];
+                        m[h] = mo[h];
+                        l[h] = lo[h];
+                        mo[h] = tm;
+                        lo[h] = tl;
+                    }
                 }
+                tmem_wait_st();
+                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&p_full[s]);
@@ -696,7 +753,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 __syncwarp();
                 tc_fence_after();
             }
-            if (s_bad[idx % kBadRing] != 0 && r < rows && poisoned<D, FP8>(a, w.z, p0, n, w.first, node)) l = NAN;
+            // from the fragments' rows to the thread's own, r
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                float x = h < 2 ? l[h & 1] : lo[h & 1];
+                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                if ((lane & 3) == 0)
+                    s_ml[s * kTileRows + (warp & 3) * 32 + 8 * h + (lane >> 2)] = make_float2(h < 2 ? m[h & 1] : mo[h & 1], x);
+            }
+            __syncwarp();
+            const float mr = s_ml[s * kTileRows + r].x;
+            float lr = s_ml[s * kTileRows + r].y;
+            if (s_bad[idx % kBadRing] != 0 && r < rows && poisoned<D, FP8>(a, w.z, p0, n, w.first, node)) {
+                lr = NAN;
+                s_ml[s * kTileRows + r].y = lr;
+            }
             __syncwarp();
             const bool whole = w.kind == 3;
             const int slot = 2 * blockIdx.x + (w.kind & 1), cnt = t1 - w.t0;
@@ -704,8 +776,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             float other_m = -INFINITY, other_l = 0.f;
             if (!pair) {
                 // both streams hold parts of the same rows: exchange (m, l), then each finishes half of the columns
-                s_ml[s * kTileRows + r] = make_float2(m, l);
-                __syncwarp();
                 if (lane == 0) mbar_arrive(ml_in);
                 wait(ml_in, ml_n & 1u);
                 __syncwarp();
@@ -714,9 +784,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 other_l = o.y;
             }
             if (active) {
-                const float mt = fmaxf(m, other_m), mu = mt == -INFINITY ? 0.f : mt;
-                const float f0 = m == -INFINITY ? 0.f : ex2(m - mu), f1 = other_m == -INFINITY ? 0.f : ex2(other_m - mu);
-                const float lt = l * f0 + other_l * f1;
+                const float mt = fmaxf(mr, other_m), mu = mt == -INFINITY ? 0.f : mt;
+                const float f0 = mr == -INFINITY ? 0.f : ex2(mr - mu), f1 = other_m == -INFINITY ? 0.f : ex2(other_m - mu);
+                const float lt = lr * f0 + other_l * f1;
                 const bool use0 = done > 0, use1 = !pair && cnt - done > 0;
                 const float inv = lt == 0.f ? 0.f : 1.f / lt;
                 const uint32_t t_other = tmem + 256 + (s ^ 1) * D + lanes;
@@ -776,52 +846,116 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     if (threadIdx.x == 0 && *abort_flag && a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
 }
 
-// Joins the parts of items that several CTAs computed, in their order: one
-// warp per row.
+// Joins the parts of items that several CTAs computed, in their order: four
+// rows a warp, so that sixteen loads are on their way at a time.
+constexpr int kJoinRows = 32;  // rows of a block
 template <int D>
 __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a) {
     pdl_wait();
     const Work wk = work_at(a.work);
     const int b = blockIdx.x;
     const JoinDesc d = wk.join[b];
-    if (d.parts == 0) return;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * 4;
+    if (d.parts == 0 || r0 >= d.rows) return;
     constexpr int E = D / 32;
-    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < d.rows; r += gridDim.y * 8) {
-        // part 0 lies in slot 2 b + 1, part i > 0 in slot 2 (b + i)
-        auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * b + 1 : 2 * (b + i)) * kItemRows + r; };
-        float m = -INFINITY;
-        bool any = false;
-        for (int i = lane; i < d.parts; i += 32) {
-            const float2 v = wk.ml[slot(i)];
-            if (v.y != 0.f) {  // a part in which the row sees a key
-                m = fmaxf(m, v.x);
-                any = true;
-            }
-        }
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        any = __any_sync(0xffffffffu, any);
-        float l = 0.f, acc[E];
+    // part 0 lies in slot 2 b + 1, part i > 0 in slot 2 (b + i)
+    auto slot = [&](int i, int r) { return static_cast<int64_t>(i == 0 ? 2 * b + 1 : 2 * (b + i)) * kItemRows + r0 + r; };
+    float m[4], l[4], acc[4][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.f;
-        if (any)
-#pragma unroll 4
-            for (int i = 0; i < d.parts; ++i) {
-                const float2 v = wk.ml[slot(i)];
-                const float f = v.y != 0.f ? ex2(v.x - m) : 0.f;
-                const float* p = wk.acc + slot(i) * D + lane * E;
-                l += v.y * f;
+    for (int r = 0; r < 4; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] += f == 0.f ? 0.f : p[e] * f;
+        for (int e = 0; e < E; ++e) acc[r][e] = 0.f;
+        if (r0 + r < d.rows)
+            for (int i = lane; i < d.parts; i += 32) {
+                const float2 v = wk.ml[slot(i, r)];
+                if (v.y != 0.f) m[r] = fmaxf(m[r], v.x);  // a part in which the row sees a key
             }
-        const int row = d.row0 + r;
-        uint16_t* dst = a.out + (static_cast<int64_t>(d.first + row / a.G) * a.nq + d.head * a.G + row % a.G) * D + lane * E;
-        const float inv = any ? 1.f / l : 0.f;
-        if (E == 4)
-            *reinterpret_cast<uint2*>(dst) = make_uint2(bf16x2_hw(acc[0] * inv, acc[1] * inv), bf16x2_hw(acc[E - 2] * inv, acc[E - 1] * inv));
-        else
-            *reinterpret_cast<uint32_t*>(dst) = bf16x2_hw(acc[0] * inv, acc[1] * inv);
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], o));
+#pragma unroll 1
+    for (int i0 = 0; i0 < d.parts; i0 += 4) {
+        float2 v[4][4];
+        float p[4][4][E];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool in = i0 + i < d.parts && r0 + r < d.rows;
+                v[i][r] = in ? wk.ml[slot(i0 + i, r)] : make_float2(0.f, 0.f);
+                const float* src = wk.acc + slot(i0 + i, r) * D + lane * E;
+                if (E == 4) {
+                    const float4 x = in ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    p[i][r][0] = x.x;
+                    p[i][r][1] = x.y;
+                    p[i][r][E - 2] = x.z;
+                    p[i][r][E - 1] = x.w;
+                } else {
+                    const float2 x = in ? *reinterpret_cast<const float2*>(src) : make_float2(0.f, 0.f);
+                    p[i][r][0] = x.x;
+                    p[i][r][1] = x.y;
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float f = v[i][r].y != 0.f ? ex2(v[i][r].x - m[r]) : 0.f;
+                l[r] += v[i][r].y * f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[r][e] += f == 0.f ? 0.f : p[i][r][e] * f;
+            }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (r0 + r >= d.rows) continue;
+        const int row = d.row0 + r0 + r, node = row / a.G;
+        uint16_t* dst = a.out + (static_cast<int64_t>(d.first + node) * a.nq + d.head * a.G + (row - node * a.G)) * D + lane * E;
+        const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+        if (E == 4)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(bf16x2_hw(acc[r][0] * inv, acc[r][1] * inv),
+                                                        bf16x2_hw(acc[r][E - 2] * inv, acc[r][E - 1] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(dst) = bf16x2_hw(acc[r][0] * inv, acc[r][1] * inv);
+    }
+}
+
+// The same for items of few rows, a warp a row, in little code: such a call's
+// time is its latency, and much of that the first run through each instruction.
+template <int D>
+__global__ void __launch_bounds__(256) tree_join_few_kernel(const __grid_constant__ TreeArgs a) {
+    pdl_wait();
+    const Work wk = work_at(a.work);
+    const int b = blockIdx.x;
+    const JoinDesc d = wk.join[b];
+    const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (d.parts == 0 || r >= d.rows) return;
+    constexpr int E = D / 32;
+    float m = -INFINITY, l = 0.f, acc[E] = {};
+#pragma unroll 4
+    for (int i = 0; i < d.parts; ++i) {
+        const int64_t at = static_cast<int64_t>(i == 0 ? 2 * b + 1 : 2 * (b + i)) * kItemRows + r;
+        const float2 v = wk.ml[at];
+        float x[E];
+        if (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(wk.acc + at * D + lane * E);
+        else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(wk.acc + at * D + lane * E);
+        if (v.y == 0.f) continue;  // the row sees no key of this part
+        const float mn = fmaxf(m, v.x), f0 = ex2(m - mn), f1 = ex2(v.x - mn);
+        m = mn;
+        l = l * f0 + v.y * f1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + x[e] * f1;
+    }
+    const int row = d.row0 + r, node = row / a.G;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(
+        a.out + (static_cast<int64_t>(d.first + node) * a.nq + d.head * a.G + (row - node * a.G)) * D + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) dst[e / 2] = bf16x2_hw(acc[e] * inv, acc[e + 1] * inv);
 }
 
 template <int D, bool FP8>
@@ -885,8 +1019,9 @@ cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int r
                     : fp8 ? (wide ? launch_many<128, true>(c, a, grid, st) : launch_many<64, true>(c, a, grid, st))
                           : (wide ? launch_many<128, false>(c, a, grid, st) : launch_many<64, false>(c, a, grid, st));
     if (e == cudaSuccess)
-        e = wide ? launch_dependent(tree_join_kernel<128>, dim3(grid, 4), dim3(256), 0, st, a)
-                 : launch_dependent(tree_join_kernel<64>, dim3(grid, 4), dim3(256), 0, st, a);
+        e = nt ? launch_dependent(wide ? tree_join_few_kernel<128> : tree_join_few_kernel<64>, dim3(grid, nt), dim3(256), 0, st, a)
+               : launch_dependent(wide ? tree_join_kernel<128> : tree_join_kernel<64>, dim3(grid, kItemRows / kJoinRows),
+                                  dim3(256), 0, st, a);
     return e;
 }
 

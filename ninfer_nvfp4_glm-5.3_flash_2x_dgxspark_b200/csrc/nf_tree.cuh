@@ -26,7 +26,8 @@ constexpr int kMaxCtas = 148;    // CTAs (one per SM) the workspace has parts fo
 constexpr int kParts = 8;        // part descriptors in flight
 constexpr uint64_t kWaitNs = 10000000000ull;  // some waits last as long as a whole part
 
-// What joins an item's parts: written by the CTA of its first part.
+// What the join's kernel needs of an item in several parts: written by the CTA
+// of its first part.
 struct JoinDesc {
     int32_t parts;   // 0: nothing to join
     int32_t rows;    // rows of the item
@@ -127,7 +128,7 @@ struct Share {
 struct ShareScratch {
     int64_t base, head;  // weight before the share's first sequence, and of one of that one's heads
     int64_t warp[32];
-    int32_t seq, pairs;
+    int32_t seq;
 };
 
 // ---------------------------------------------------------------------------
@@ -179,8 +180,6 @@ struct Walk {
         }
         return w;
     }
-    // whether some item of the sequence weighs 2 a tile
-    __device__ __forceinline__ bool two(int G) const { return ROWS > kTileRows && n * G > kTileRows; }
     // the share's first part
     __device__ __forceinline__ void start(const TreeArgs& a, const Share& s, const ShareScratch& sh) {
         valid = true;
@@ -193,7 +192,7 @@ struct Walk {
         pt = 0;
         seek(a, true);
     }
-    // the part's descriptor, and, for an item that other CTAs go on with, how many parts there are to join
+    // the part's descriptor, and, for an item that other CTAs go on with, what its join needs
     __device__ __forceinline__ Part describe(const TreeArgs& a, const Share& s) const {
         Part p{};
         if (!valid) return p;
@@ -249,17 +248,16 @@ struct Walk {
     }
 };
 
-// Finds the CTA's share (every thread sums the weights of a run of sequences;
-// sh.pairs is 0 before) and fills the rows of bad sequences with NaN.  Ends
-// with a __syncthreads.
-template <int D, int THREADS, typename W>
+// Finds the CTA's share (every thread sums the weights of a run of sequences) and fills the rows of bad sequences with NaN.  A share
+// is not smaller than LEAST, the weight that a CTA takes at a time: smaller
+// ones would only make more parts to join.  Ends with a __syncthreads.
+template <int D, int THREADS, int LEAST, typename W>
 __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     W w;
     const int run = (a.batch + THREADS - 1) / THREADS;
     const int i0 = min(a.batch, static_cast<int>(threadIdx.x) * run), i1 = min(a.batch, i0 + run);
     int64_t mine = 0;
-    bool pairs = false;
 #pragma unroll 1
     for (w.i = i0; w.i < i1; ++w.i) {
         w.load(a);
@@ -273,9 +271,7 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
             continue;
         }
         mine += w.head_weight(a) * a.nkv;
-        pairs |= w.two(a.G);
     }
-    if (pairs) sh.pairs = 1;
     int64_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -291,7 +287,7 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
         total += sh.warp[k];
     }
     Share s;
-    s.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(sh.pairs ? 2 : 1));
+    s.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(LEAST));
     s.lo = s.per * blockIdx.x;
     s.hi = min(total, s.lo + s.per);
     if (mine > 0 && s.lo >= base && s.lo < base + mine) {

@@ -103,7 +103,6 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
         }
         *s_abort = 0;
         for (int s = 0; s < 4; ++s) s_bad[s] = 0;
-        s_share.pairs = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
@@ -112,7 +111,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
     __syncthreads();
     pdl_trigger();  // the join's blocks may wait for this grid beside it
     using ItemWalk = Walk<kRows, kKeys>;
-    const Share share = find_share<D, G_::kThreads, ItemWalk>(a, s_share);
+    const Share share = find_share<D, G_::kThreads, G_::kGroups, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;
     volatile int* abort_flag = s_abort;
     // A bounded wait.  After a time-out no role waits or loads any more, and
