@@ -24,6 +24,9 @@ cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int r
                                   const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* cache_seq,
                                   const uint64_t* mask, int mask_words, float scale, uint16_t* out, void* work,
                                   int32_t* status, cudaStream_t st);
+cudaError_t launch_token_logprobs(const void* logits, int type, int64_t stride, int rows, int64_t vocab,
+                                  const int32_t* target, int top, float* logprob, float* entropy, int32_t* top_idx,
+                                  float* top_lp, cudaStream_t st);
 cudaError_t launch_kv_accept(const nf_kv_cache* caches, int layers, const int32_t* prefix, const int32_t* path,
                              int max_path, const int32_t* path_len, const int32_t* cache_seq, int batch,
                              int32_t* status, cudaStream_t st);
