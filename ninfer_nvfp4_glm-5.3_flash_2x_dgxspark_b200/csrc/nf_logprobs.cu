@@ -3,6 +3,7 @@
 #include "nf_kv.h"
 
 #include "nf_common.cuh"
+#include "nf_gemm_shared.cuh"
 #include "nf_internal.h"
 
 #include <cmath>
@@ -98,6 +99,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {  // value_key's inverse; 0 is a NaN
+    return k == 0 ? NAN : __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+}
+
 // Sums of a set of logits: m the greatest, s = sum e^(x - m), t = sum e^(x - m) (x - m).
 struct Sums {
     float m, s, t;
@@ -148,7 +163,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __
     __shared__ uint16_t s_hot[kThreads];
     __shared__ uint64_t s_cand[kCandidates];
     __shared__ uint64_t s_red[kThreads / 32];
-    __shared__ Sums s_sums[kThreads / 32];
+    __shared__ float2 s_sums[kThreads / 32];
+    __shared__ uint32_t s_wmax[kThreads / 32];
     __shared__ uint32_t s_bound;
     __shared__ int s_hots, s_count;
     uint32_t ranks;
@@ -173,6 +189,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __
         u.s *= f;
         u.m = m;
     };
+    // two logits at a time: the loop is bound by the instructions issued
+    uint64_t s2 = 0, t2 = 0;
+    const uint64_t l2 = f32x2_pack(kLog2e, kLog2e);
 #pragma unroll 1
     for (int64_t g = mine; g < part.groups; g += 4 * part.step) {
         uint4 w[4][BF16 ? 1 : 2];
@@ -184,37 +203,70 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __
             if (g + k * part.step >= part.groups) break;
             float f[8];
             unpack<BF16>(w[k], f);
-            grow(max3(max3(max3(u.m, f[0], f[1]), f[2], f[3]), max3(f[4], f[5], f[6]), f[7]));
-            const float mu = u.m == -INFINITY ? 0.f : u.m;
+            const float m = max3(max3(max3(u.m, f[0], f[1]), f[2], f[3]), max3(f[4], f[5], f[6]), f[7]);
+            const float d = fmaxf(u.m - m, kFar), c = ex2(d * kLog2e);  // m = -infinity: d NaN becomes kFar, c 0
+            const uint64_t c2 = f32x2_pack(c, c);
+            t2 = mul_f32x2(fma_f32x2(s2, f32x2_pack(d, d), t2), c2);
+            s2 = mul_f32x2(s2, c2);
+            u.m = m;
+            const float mu = m == -INFINITY ? 0.f : m;
+            const uint64_t nm = f32x2_pack(-mu, -mu);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) add(f[e], mu);
+            for (int e = 0; e < 8; e += 2) {
+                const uint64_t x2 = add_f32x2(f32x2_pack(f[e], f[e + 1]), nm), y2 = mul_f32x2(x2, l2);
+                const uint64_t e2 = f32x2_pack(ex2(f32x2_lo(y2)), ex2(f32x2_hi(y2)));
+                s2 = add_f32x2(s2, e2);
+                t2 = fma_f32x2(e2, f32x2_pack(fmaxf(f32x2_lo(x2), kFar), fmaxf(f32x2_hi(x2), kFar)), t2);
+            }
         }
     }
+    u.s = f32x2_lo(s2) + f32x2_hi(s2);
+    u.t = f32x2_lo(t2) + f32x2_hi(t2);
     if (single >= 0) {
         const float f = load_logit<BF16>(x, single);
         grow(fmaxf(u.m, f));
         add(f, u.m == -INFINITY ? 0.f : u.m);
     }
 
+    // ---- the CTA's sums
+    const bool any = mine < part.groups || single >= 0;
+    // 0: no logit; a NaN or -infinity alone is 1 at least
+    const uint32_t best = any ? max(1u, value_key(u.m)) : 0u;
+    const uint32_t warp_best = __reduce_max_sync(0xffffffffu, best);
+    s_max[threadIdx.x] = best;
+    if ((threadIdx.x & 31) == 0) s_wmax[threadIdx.x >> 5] = warp_best;
+    if (threadIdx.x == 0) s_hots = s_count = 0;
+    __syncthreads();
+    uint32_t top_key = s_wmax[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) top_key = max(top_key, s_wmax[w]);
+    grow(fmaxf(u.m, key_value(top_key)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        u.s += __shfl_xor_sync(0xffffffffu, u.s, o);
+        u.t += __shfl_xor_sync(0xffffffffu, u.t, o);
+    }
+    if ((threadIdx.x & 31) == 0) s_sums[threadIdx.x >> 5] = make_float2(u.s, u.t);
+
     // ---- the CTA's top tokens
     if (top > 0) {
-        // 0: no logit; a NaN or -infinity alone is 1 at least
-        const bool any = mine < part.groups || single >= 0;
-        const uint32_t best = any ? max(1u, value_key(u.m)) : 0u;
-        s_max[threadIdx.x] = best;
-        if (threadIdx.x == 0) {
-            s_bound = 0xffffffffu;
-            s_hots = s_count = 0;
+        // the top-th greatest of the threads' maxima (0 if fewer have a logit), bit by bit, by the first warp
+        if (threadIdx.x < 32) {
+            uint32_t b = top_key;
+            if (top > 1) {
+                const uint4 k0 = *reinterpret_cast<const uint4*>(s_max + 8 * threadIdx.x);
+                const uint4 k1 = *reinterpret_cast<const uint4*>(s_max + 8 * threadIdx.x + 4);
+                b = 0;
+#pragma unroll 1
+                for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+                    const uint32_t c = b | bit;
+                    const uint32_t n = (k0.x >= c) + (k0.y >= c) + (k0.z >= c) + (k0.w >= c) + (k1.x >= c) + (k1.y >= c) +
+                                       (k1.z >= c) + (k1.w >= c);
+                    if (__reduce_add_sync(0xffffffffu, n) >= static_cast<uint32_t>(top)) b = c;
+                }
+            }
+            if (threadIdx.x == 0) s_bound = b;
         }
-        __syncthreads();
-        int above = 0;  // threads with a greater maximum
-#pragma unroll 4
-        for (int i = 0; i < kThreads; i += 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(s_max + i);
-            above += (v.x > best) + (v.y > best) + (v.z > best) + (v.w > best);
-        }
-        // the least of the top maxima, or of all if fewer than `top` threads have a logit
-        if (above < top) atomicMin(&s_bound, best);
         __syncthreads();
         uint32_t bound = s_bound;
         if (bound <= value_key(-INFINITY)) bound = 0;  // -infinities and NaNs among the top: look at all
@@ -283,15 +335,12 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __
             if (threadIdx.x == 0) s_told.count = top;
         }
     }
-    // ---- the CTA's sums
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        u = join(u, Sums{__shfl_xor_sync(0xffffffffu, u.m, o), __shfl_xor_sync(0xffffffffu, u.s, o),
-                         __shfl_xor_sync(0xffffffffu, u.t, o)});
-    if ((threadIdx.x & 31) == 0) s_sums[threadIdx.x >> 5] = u;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 32; ++w) u = join(u, s_sums[w]);
+        for (int w = 1; w < kThreads / 32; ++w) {
+            u.s += s_sums[w].x;
+            u.t += s_sums[w].y;
+        }
         s_told.sums = u;
     }
     // ---- the row's, in the first CTA
