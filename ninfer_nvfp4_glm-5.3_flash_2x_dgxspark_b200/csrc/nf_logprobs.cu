@@ -401,9 +401,10 @@ cudaError_t launch_token_logprobs(const void* logits, int type, int64_t stride, 
                                   const int32_t* target, int top, float* logprob, float* entropy, int32_t* top_idx,
                                   float* top_lp, cudaStream_t st) {
     if (rows <= 0) return cudaSuccess;
-    // enough CTAs for eight on every SM, as long as each has 4,096 logits
+    // clusters give a few rows every SM: two CTAs on each, as long as each has 4,096 logits (256 rows of 151,552 logits:
+    // 36.3 us with one CTA a row, 34.9 with two, 43.0 with four, 65.8 with eight)
     unsigned ranks = 1;
-    while (ranks < 8 && static_cast<int64_t>(rows) * ranks < 8 * 148 && vocab / (2 * ranks) >= 4096) ranks *= 2;
+    while (ranks < 8 && static_cast<int64_t>(rows) * ranks < 2 * 148 && vocab / (2 * ranks) >= 4096) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows) * ranks);
     cfg.blockDim = dim3(kThreads);

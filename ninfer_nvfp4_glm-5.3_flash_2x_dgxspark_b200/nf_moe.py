@@ -885,9 +885,38 @@ DTYPE_F32, DTYPE_BF16 = 0, 1
 ROPE_LAYOUT = dict(half=0, interleaved=1)
 ROPE_SCALING = dict(none=0, linear=1, yarn=2)
 MAX_TOP = 32  # top tokens of one token_logprobs call
-_BF16 = ("torch.bfloat16", "torch.int16", "torch.uint16")
-_CODES = ("torch.float8_e4m3fn", "torch.uint8")
-_I32, _U64 = ("torch.int32",), ("torch.int64", "torch.uint64")
+
+
+class _Kinds:
+    """The dtypes the calls below take, as sets of torch dtypes (torch is imported when the first call needs it)."""
+
+    def __getattr__(self, name):
+        import torch
+
+        self.bf16 = frozenset((torch.bfloat16, torch.int16, torch.uint16))
+        self.codes = frozenset((torch.float8_e4m3fn, torch.uint8))
+        self.f32 = frozenset((torch.float32,))
+        self.i32 = frozenset((torch.int32,))
+        self.u8 = frozenset((torch.uint8,))
+        self.u64 = frozenset((torch.int64, torch.uint64))
+        self.number = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+        self.current = torch.cuda.current_device
+        return self.__dict__[name]
+
+
+_K = _Kinds()
+
+
+def _buf(a, need: int, kinds, name: str, device: int) -> int | None:
+    """_dev for the calls whose time is their launch: the same checks, in the order of a good buffer."""
+    if a is None:
+        return None
+    try:
+        if a.dtype in kinds and a.get_device() == device and a.is_contiguous() and a.numel() >= need:
+            return a.data_ptr()
+    except AttributeError:
+        pass
+    return _dev(a, need, tuple(str(k) for k in kinds), name, device)
 
 
 def _kv_check(st: int) -> None:
@@ -909,19 +938,19 @@ class KvCache:
     context].  Keeps the tensors alive."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        if isinstance(k, (int, np.ndarray)) or not getattr(k, "is_cuda", False):
+        if not getattr(k, "is_cuda", False):
             raise NfError(1, "k is not a CUDA tensor")
         self.device = dv = k.device.index
         seqs, heads, context, dim = (_dim(k, i, "k", 4) for i in range(4))
-        kind = KV_BF16 if str(k.dtype) in _BF16 else KV_E4M3
-        types = _BF16 if kind == KV_BF16 else _CODES
+        kind = KV_BF16 if k.dtype in _K.bf16 else KV_E4M3
+        types = _K.bf16 if kind == KV_BF16 else _K.codes
         n = seqs * heads * context
         if (k_scale is None) != (kind == KV_BF16) or (v_scale is None) != (kind == KV_BF16):
             raise NfError(1, "an E4M3 cache has scales, a BF16 cache has none")
         if tuple(v.shape) != tuple(k.shape):
             raise NfError(2, "k and v differ in shape")
-        self.desc = KvDesc(_dev(k, n * dim, types, "k", dv), _dev(v, n * dim, types, "v", dv),
-                           _dev(k_scale, n, _F32, "k_scale", dv), _dev(v_scale, n, _F32, "v_scale", dv), kind, seqs,
+        self.desc = KvDesc(_buf(k, n * dim, types, "k", dv), _buf(v, n * dim, types, "v", dv),
+                           _buf(k_scale, n, _K.f32, "k_scale", dv), _buf(v_scale, n, _K.f32, "v_scale", dv), kind, seqs,
                            heads, context, dim)
         self.ref = ctypes.byref(self.desc)
         self.tensors = (k, v, k_scale, v_scale)
@@ -957,7 +986,7 @@ class Rope:
 
 
 def _on_current(device: int, what: str) -> None:
-    if device != _current_device():
+    if device != _K.current():
         raise NfError(1, f"{what} is on cuda:{device}, which is not the current device")
 
 
@@ -975,17 +1004,17 @@ def kv_write(cache: KvCache, rope: Rope, qkv, q_heads: int, positions, q, *, seq
     stride = qkv.stride(0) if tokens > 1 else width
     if not getattr(qkv, "is_cuda", False) or qkv.device.index != dv or (tokens and qkv.stride(1) != 1):
         raise NfError(1, f"qkv is not on cuda:{dv} with contiguous rows")
-    kind = str(qkv.dtype)
-    if kind not in ("torch.float32", "torch.bfloat16"):
+    kind = _K.number.get(qkv.dtype)
+    if kind is None:
         raise NfError(1, f"qkv has dtype {qkv.dtype}; expected float32 or bfloat16")
     if seqs is None and tokens > d.seqs:
         raise NfError(2, f"{tokens} tokens for a cache of {d.seqs} sequences: pass seqs")
     _kv_check(load().nf_kv_write(
-        cache.ref, rope.ref, qkv.data_ptr(), DTYPE_F32 if kind == "torch.float32" else DTYPE_BF16, stride, tokens,
-        q_heads, _dev(q_norm, d.head_dim, _F32, "q_norm", dv), _dev(k_norm, d.head_dim, _F32, "k_norm", dv), eps,
-        _dev(positions, tokens, _I32, "positions", dv), _dev(seqs, tokens, _I32, "seqs", dv),
-        _dev(slots, tokens, _I32, "slots", dv), _dev(q, tokens * q_heads * d.head_dim, _BF16, "q", dv),
-        _dev(status, 1, _I32, "status", dv), stream or None))
+        cache.ref, rope.ref, qkv.data_ptr(), kind, stride, tokens,
+        q_heads, _buf(q_norm, d.head_dim, _K.f32, "q_norm", dv), _buf(k_norm, d.head_dim, _K.f32, "k_norm", dv), eps,
+        _buf(positions, tokens, _K.i32, "positions", dv), _buf(seqs, tokens, _K.i32, "seqs", dv),
+        _buf(slots, tokens, _K.i32, "slots", dv), _buf(q, tokens * q_heads * d.head_dim, _K.bf16, "q", dv),
+        _buf(status, 1, _K.i32, "status", dv), stream or None))
 
 
 def tree_attention_workspace(head_dim: int) -> int:
@@ -1010,11 +1039,11 @@ def tree_attention(cache: KvCache, q, row_start, prefix, out, workspace, *, cach
         raise NfError(2, "row_start holds no sequence")
     words = 0 if mask is None else _dim(mask, 1, "mask", 2)
     _kv_check(load().nf_tree_attention(
-        cache.ref, _dev(q, rows * heads * dim, _BF16, "q", dv), rows, heads,
-        _dev(row_start, batch + 1, _I32, "row_start", dv), batch, _dev(prefix, batch, _I32, "prefix", dv),
-        _dev(cache_seq, batch, _I32, "cache_seq", dv), _dev(mask, rows * words, _U64, "mask", dv), words,
-        dim ** -0.5 if scale is None else scale, _dev(out, rows * heads * dim, _BF16, "out", dv),
-        _dev(workspace, 0, _U8, "workspace", dv), workspace.numel(), _dev(status, 1, _I32, "status", dv),
+        cache.ref, _buf(q, rows * heads * dim, _K.bf16, "q", dv), rows, heads,
+        _buf(row_start, batch + 1, _K.i32, "row_start", dv), batch, _buf(prefix, batch, _K.i32, "prefix", dv),
+        _buf(cache_seq, batch, _K.i32, "cache_seq", dv), _buf(mask, rows * words, _K.u64, "mask", dv), words,
+        dim ** -0.5 if scale is None else scale, _buf(out, rows * heads * dim, _K.bf16, "out", dv),
+        _buf(workspace, 0, _K.u8, "workspace", dv), workspace.numel(), _buf(status, 1, _K.i32, "status", dv),
         stream or None))
 
 
@@ -1034,18 +1063,18 @@ def token_logprobs(logits, targets, logprob, entropy, top_idx, top_logprob, work
         raise NfError(1, "logits is not a CUDA tensor with contiguous rows")
     dv = logits.device.index
     _on_current(dv, "logits")
-    kind = str(logits.dtype)
-    if kind not in ("torch.float32", "torch.bfloat16"):
+    kind = _K.number.get(logits.dtype)
+    if kind is None:
         raise NfError(1, f"logits has dtype {logits.dtype}; expected float32 or bfloat16")
     if (top_idx is None) != (top_logprob is None):
         raise NfError(1, "top_idx and top_logprob go together")
     top = 0 if top_idx is None else _dim(top_idx, 1, "top_idx", 2)
     _kv_check(load().nf_token_logprobs(
-        logits.data_ptr(), DTYPE_F32 if kind == "torch.float32" else DTYPE_BF16,
-        logits.stride(0) if rows > 1 else max(1, vocab), rows, vocab, _dev(targets, rows, _I32, "targets", dv), top,
-        _dev(logprob, rows, _F32, "logprob", dv), _dev(entropy, rows, _F32, "entropy", dv),
-        _dev(top_idx, rows * top, _I32, "top_idx", dv), _dev(top_logprob, rows * top, _F32, "top_logprob", dv),
-        _dev(workspace, 0, _U8, "workspace", dv), workspace.numel(), stream or None))
+        logits.data_ptr(), kind,
+        logits.stride(0) if rows > 1 else max(1, vocab), rows, vocab, _buf(targets, rows, _K.i32, "targets", dv), top,
+        _buf(logprob, rows, _K.f32, "logprob", dv), _buf(entropy, rows, _K.f32, "entropy", dv),
+        _buf(top_idx, rows * top, _K.i32, "top_idx", dv), _buf(top_logprob, rows * top, _K.f32, "top_logprob", dv),
+        _buf(workspace, 0, _K.u8, "workspace", dv), workspace.numel(), stream or None))
 
 
 def kv_accept(caches: KvCaches, prefix, path, path_len, *, cache_seq=None, status=None, stream=0) -> None:
@@ -1058,6 +1087,6 @@ def kv_accept(caches: KvCaches, prefix, path, path_len, *, cache_seq=None, statu
     if cache_seq is None and batch > caches.caches[0].desc.seqs:
         raise NfError(2, f"{batch} paths for a cache of {caches.caches[0].desc.seqs} sequences: pass cache_seq")
     _kv_check(load().nf_kv_accept(
-        caches.descs, len(caches.caches), _dev(prefix, batch, _I32, "prefix", dv),
-        _dev(path, batch * longest, _I32, "path", dv), longest, _dev(path_len, batch, _I32, "path_len", dv),
-        _dev(cache_seq, batch, _I32, "cache_seq", dv), batch, _dev(status, 1, _I32, "status", dv), stream or None))
+        caches.descs, len(caches.caches), _buf(prefix, batch, _K.i32, "prefix", dv),
+        _buf(path, batch * longest, _K.i32, "path", dv), longest, _buf(path_len, batch, _K.i32, "path_len", dv),
+        _buf(cache_seq, batch, _K.i32, "cache_seq", dv), batch, _buf(status, 1, _K.i32, "status", dv), stream or None))
