@@ -621,6 +621,42 @@ NF_API int nf_kv_accept(const nf_kv_cache* caches, int layers, const int32_t* pr
                         int max_path, const int32_t* path_len_dev, const int32_t* cache_seq_dev, int batch,
                         int32_t* status_dev, void* stream);
 
+/* The log-probabilities of the last nf_tp_linear_bf16's output on every rank
+ * (rows = the vocabulary), as nf_token_logprobs gives them. */
+NF_API int nf_tp_logprobs(nf_tp* handle, int tokens, int64_t rows, const int32_t* target_dev, int top,
+                          float* logprob_dev, float* entropy_dev, int32_t* top_idx_dev, float* top_logprob_dev,
+                          void* stream);
+
+/* ---- the decoder stack over several rows of a sequence ---------------------
+ * nf_stack_create with the caches' kind (nf_stack_create: NF_KV_BF16).  With
+ * NF_KV_E4M3 the caches take half the bytes; nf_stack_decode, _load_kv and
+ * _fill_kv work the same (the latter two quantise their BF16 rows), and
+ * nf_stack_kv_cache returns NF_ERR_UNSUPPORTED. */
+NF_API int nf_stack_create_kv(const nf_stack_desc* desc, int kv_kind, int device, nf_stack** out);
+/* A layer's caches as the calls above take them (device pointers). */
+NF_API int nf_stack_kv(nf_stack* stack, int layer, nf_kv_cache* out);
+/* One step over `rows` (at most max_batch) new tokens of `batch` sequences: a
+ * chain or a tree of drafted tokens of each, or a chunk of a prompt.  Sequence
+ * i is cache sequence i, holds prefix_dev[i] positions, and its rows are
+ * row_start_dev[i] .. row_start_dev[i + 1] - 1 (see nf_tree_attention for
+ * row_start, the mask and what a bad sequence gives).  Row j of a sequence is
+ * written to cache position prefix + j and turned to position prefix +
+ * depth_dev[row] (INT32 [rows]; NULL: prefix + j).  next_dev (INT32 [rows],
+ * optional) receives every row's greedy token, final_dev (F32 [rows, H],
+ * optional) the final norm's output; nf_stack_logprobs reads the step's
+ * logits.  Rows behind row_start_dev[batch] write nothing to the caches; their
+ * outputs mean nothing.  The caches' positions from prefix on hold the rows of
+ * the step until the next one writes there: nf_stack_accept keeps a path. */
+NF_API int nf_stack_verify(nf_stack* stack, const int32_t* tokens_dev, const int32_t* depth_dev,
+                           const int32_t* row_start_dev, const int32_t* prefix_dev, const uint64_t* mask_dev,
+                           int mask_words, int rows, int batch, int32_t* next_dev, float* final_dev, void* stream);
+/* nf_token_logprobs of the last step's logits (a step of at least `rows` rows). */
+NF_API int nf_stack_logprobs(nf_stack* stack, int rows, const int32_t* target_dev, int top, float* logprob_dev,
+                             float* entropy_dev, int32_t* top_idx_dev, float* top_logprob_dev, void* stream);
+/* nf_kv_accept over every layer's caches (sequence i is cache sequence i). */
+NF_API int nf_stack_accept(nf_stack* stack, const int32_t* prefix_dev, const int32_t* path_dev, int max_path,
+                           const int32_t* path_len_dev, int batch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

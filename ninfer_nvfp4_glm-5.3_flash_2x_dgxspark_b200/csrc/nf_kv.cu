@@ -106,12 +106,44 @@ __device__ __forceinline__ void store_bf16(uint16_t* dst, const float* x) {
     else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
+// A lane's dims of a row whose greatest magnitude is `peak` as E4M3 codes;
+// returns the row's scale.
+template <int E>
+__device__ __forceinline__ float quantize_row(float (&y)[E], float peak, uint32_t (&code)[E / 4]) {
+    const float scale = peak * (1.f / 448.f);
+    if (peak >= 1e-30f && peak <= 1e30f) {
+        const float inv = __fdividef(448.f, peak);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] *= inv;
+    } else {  // zeros, where the quotient might overflow, and NaN
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = scale > 0.f || isnan(scale) ? __fdiv_rn(y[e], scale) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[e + 1]), "f"(y[e]));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[e + 3]), "f"(y[e + 2]));
+        code[e / 4] = lo | static_cast<uint32_t>(hi) << 16;
+    }
+    return scale;
+}
+template <int E>
+__device__ __forceinline__ float half_warp_peak(const float (&y)[E]) {
+    float peak = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) peak = max_nan(peak, fabsf(y[e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+    return peak;
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
     const __grid_constant__ nf_kv_cache c, const __grid_constant__ nf_rope rope, const void* __restrict__ qkv,
-    int64_t row_stride, int nq, const float* __restrict__ q_norm, const float* __restrict__ k_norm, float eps,
-    const int32_t* __restrict__ pos, const int32_t* __restrict__ seq, const int32_t* __restrict__ slot,
-    uint16_t* __restrict__ q_out, int32_t* __restrict__ status) {
+    int slices, int64_t slice_stride, int64_t row_stride, int nq, const float* __restrict__ q_norm,
+    const float* __restrict__ k_norm, float eps, const int32_t* __restrict__ pos, const int32_t* __restrict__ seq,
+    const int32_t* __restrict__ slot, uint16_t* __restrict__ q_out, int32_t* __restrict__ status) {
     constexpr int E = D / 16, W = BF16 ? E / 2 : E;
     const int step = blockDim.x >> 4;  // heads at a time
     __shared__ float2 s_turn[D / 2];  // (cos, sin) of every pair's angle, times the magnitude
@@ -167,6 +199,14 @@ __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
             const uint32_t w = next[BF16 ? e / 2 : e];
             y[e] = !in ? 0.f : __uint_as_float(!BF16 ? w : (e & 1) ? w & 0xffff0000u : w << 16);
         }
+        if (!BF16 && in)
+#pragma unroll 1
+            for (int k = 1; k < slices; ++k) {
+                uint32_t w[W];
+                load_words<W>(row + (k * slice_stride + static_cast<int64_t>(h) * D) * 4, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] = __fadd_rn(y[e], __uint_as_float(w[BF16 ? 0 : e]));
+            }
         load(h + step);
         if (__any_sync(0xffffffffu, is_q || is_k)) {
             if (q_norm || k_norm) {
@@ -205,12 +245,7 @@ __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
             }
         }
         float peak = 0.f;
-        if (c.kind == NF_KV_E4M3 && __any_sync(0xffffffffu, in && !is_q)) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) peak = max_nan(peak, fabsf(y[e]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-        }
+        if (c.kind == NF_KV_E4M3 && __any_sync(0xffffffffu, in && !is_q)) peak = half_warp_peak<E>(y);
         if (!in) continue;
         if (is_q) {
             if (!ok)
@@ -225,28 +260,52 @@ __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
             store_bf16<E>(static_cast<uint16_t*>(is_k ? c.k : c.v) + r * D + lane * E, y);
             continue;
         }
-        const float scale = peak * (1.f / 448.f);
-        if (peak >= 1e-30f && peak <= 1e30f) {
-            const float inv = __fdividef(448.f, peak);
-#pragma unroll
-            for (int e = 0; e < E; ++e) y[e] *= inv;
-        } else {  // zeros, where the quotient might overflow, and NaN
-#pragma unroll
-            for (int e = 0; e < E; ++e) y[e] = scale > 0.f || isnan(scale) ? __fdiv_rn(y[e], scale) : 0.f;
-        }
         uint32_t code[E / 4];
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            uint16_t lo, hi;
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[e + 1]), "f"(y[e]));
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[e + 3]), "f"(y[e + 2]));
-            code[e / 4] = lo | static_cast<uint32_t>(hi) << 16;
-        }
+        const float scale = quantize_row<E>(y, peak, code);
         uint8_t* dst = static_cast<uint8_t*>(is_k ? c.k : c.v) + r * D + lane * E;
         if (E == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[E / 4 - 1]);
         else *reinterpret_cast<uint32_t*>(dst) = code[0];
         if (lane == 0) (is_k ? c.k_scale : c.v_scale)[r] = scale;
     }
+}
+
+// A loaded history's rows, half a warp each.
+template <int D>
+__global__ void __launch_bounds__(256) kv_quantize_kernel(const uint16_t* __restrict__ x, int64_t n,
+                                                          uint8_t* __restrict__ codes, float* __restrict__ scale) {
+    constexpr int E = D / 16;
+    const int lane = threadIdx.x & 15;
+    const int64_t r = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = r < n ? bf16_bits_to_f32(x[r * D + lane * E + e]) : 0.f;
+    uint32_t code[E / 4];
+    const float s = quantize_row<E>(y, half_warp_peak<E>(y), code);
+    if (r >= n) return;
+#pragma unroll
+    for (int e = 0; e < E / 4; ++e) *reinterpret_cast<uint32_t*>(codes + r * D + lane * E + 4 * e) = code[e];
+    if (lane == 0) scale[r] = s;
+}
+
+__global__ void __launch_bounds__(128) kv_places_kernel(int rows, const int32_t* __restrict__ row_start, int batch,
+                                                        const int32_t* __restrict__ prefix,
+                                                        const int32_t* __restrict__ depth, int32_t* __restrict__ seq,
+                                                        int32_t* __restrict__ slot, int32_t* __restrict__ pos) {
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r >= rows) return;
+    int lo = 0, hi = batch;  // the last sequence that starts at or before r
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (row_start[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    const int j = r - row_start[lo];
+    const bool in = j >= 0 && r < row_start[lo + 1];
+    // a place outside the cache is left to the write to refuse
+    const int64_t at = static_cast<int64_t>(prefix[lo]) + j, p = static_cast<int64_t>(prefix[lo]) + (depth ? depth[r] : j);
+    seq[r] = lo;
+    slot[r] = !in ? -1 : at < 0 || at > 0x7fffffff ? 0x7fffffff : static_cast<int32_t>(at);
+    pos[r] = !in ? 0 : p < 0 || p > 0x7fffffff ? -1 : static_cast<int32_t>(p);
 }
 
 // ---------------------------------------------------------------------------
@@ -326,7 +385,7 @@ __global__ void __launch_bounds__(128) kv_accept_kernel(const __grid_constant__ 
 cudaError_t launch_kv_write(const nf_kv_cache& c, const nf_rope& rope, const void* qkv, int qkv_type,
                             int64_t row_stride, int tokens, int q_heads, const float* q_norm, const float* k_norm,
                             float eps, const int32_t* pos, const int32_t* seq, const int32_t* slot, uint16_t* q,
-                            int32_t* status, cudaStream_t st) {
+                            int32_t* status, cudaStream_t st, int slices, int64_t slice_stride) {
     if (tokens <= 0) return cudaSuccess;
     const bool bf16 = qkv_type == NF_DTYPE_BF16;
     auto kernel = c.head_dim == 128 ? (bf16 ? kv_write_kernel<128, true> : kv_write_kernel<128, false>)
@@ -335,8 +394,23 @@ cudaError_t launch_kv_write(const nf_kv_cache& c, const nf_rope& rope, const voi
     // 9.2 and 6.9); many: fewer, so that less of the time goes to what is done once per token (8,192 tokens: 57.8 us with
     // 4, 51.0 with 2).
     const int warps = tokens <= 2 * 148 ? kWriteWarps : tokens <= 1000 ? 4 : 2;
-    kernel<<<static_cast<unsigned>(tokens), 32 * warps, 0, st>>>(c, rope, qkv, row_stride, q_heads, q_norm, k_norm,
-                                                                       eps, pos, seq, slot, q, status);
+    kernel<<<static_cast<unsigned>(tokens), 32 * warps, 0, st>>>(c, rope, qkv, slices, slice_stride, row_stride, q_heads,
+                                                                 q_norm, k_norm, eps, pos, seq, slot, q, status);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_kv_quantize(const uint16_t* x, int64_t n, int head_dim, uint8_t* codes, float* scale, cudaStream_t st) {
+    if (n <= 0) return cudaSuccess;
+    const unsigned grid = static_cast<unsigned>((n + 15) / 16);
+    if (head_dim == 128) kv_quantize_kernel<128><<<grid, 256, 0, st>>>(x, n, codes, scale);
+    else kv_quantize_kernel<64><<<grid, 256, 0, st>>>(x, n, codes, scale);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_kv_places(int rows, const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* depth,
+                             int32_t* seq, int32_t* slot, int32_t* pos, cudaStream_t st) {
+    if (rows <= 0) return cudaSuccess;
+    kv_places_kernel<<<(rows + 127) / 128, 128, 0, st>>>(rows, row_start, batch, prefix, depth, seq, slot, pos);
     return cudaGetLastError();
 }
 

@@ -152,7 +152,9 @@ __device__ __forceinline__ int rank_of(uint64_t v, const uint64_t* s, int n) {
 // whose maximum reaches it (`top` of 256, but for equals) can be among them;
 // the CTA looks at these once more.
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __restrict__ logits, int64_t stride,
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __restrict__ logits,
+                                                                  const uint32_t* __restrict__ epoch,
+                                                                  int64_t epoch_bytes, int64_t stride,
                                                                   int64_t vocab, const int32_t* __restrict__ target,
                                                                   int top, float* __restrict__ logprob,
                                                                   float* __restrict__ entropy,
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
     const int rank = static_cast<int>(cluster_ctarank());
     const int64_t row = blockIdx.x / ranks;
-    const void* x = static_cast<const uint8_t*>(logits) + row * stride * (BF16 ? 2 : 4);
+    const void* x = static_cast<const uint8_t*>(logits) + (epoch ? (*epoch & 1u) * epoch_bytes : 0) + row * stride * (BF16 ? 2 : 4);
     const Slice<BF16> part(x, vocab, ranks);
     const int64_t g0 = static_cast<int64_t>(rank) * kThreads;  // the CTA's first thread in the cluster
     const int64_t mine = g0 + threadIdx.x, single = part.single(mine);
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const void* __
 
 cudaError_t launch_token_logprobs(const void* logits, int type, int64_t stride, int rows, int64_t vocab,
                                   const int32_t* target, int top, float* logprob, float* entropy, int32_t* top_idx,
-                                  float* top_lp, cudaStream_t st) {
+                                  float* top_lp, cudaStream_t st, const uint32_t* epoch, int64_t epoch_bytes) {
     if (rows <= 0) return cudaSuccess;
     // clusters give a few rows every SM: two CTAs on each, as long as each has 4,096 logits (256 rows of 151,552 logits:
     // 36.3 us with one CTA a row, 34.9 with two, 43.0 with four, 65.8 with eight)
@@ -416,7 +418,7 @@ cudaError_t launch_token_logprobs(const void* logits, int type, int64_t stride, 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, type == NF_DTYPE_BF16 ? token_logprobs_kernel<true> : token_logprobs_kernel<false>,
-                              logits, stride, vocab, target, top, logprob, entropy, top_idx, top_lp);
+                              logits, epoch, epoch_bytes, stride, vocab, target, top, logprob, entropy, top_idx, top_lp);
 }
 
 }  // namespace nf

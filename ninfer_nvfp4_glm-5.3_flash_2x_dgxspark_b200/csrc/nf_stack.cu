@@ -26,8 +26,10 @@
 
 #include "nf_common.cuh"
 #include "nf_internal.h"
+#include "nf_kv.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -49,8 +51,10 @@ struct StackLayer {
     float* ffn_norm = nullptr;
     float* q_norm = nullptr;
     float* k_norm = nullptr;
-    uint16_t* kc = nullptr;    // [B][nkv][L][D]
+    uint16_t* kc = nullptr;    // [B][nkv][L][D] (NF_KV_E4M3: the same as codes)
     uint16_t* vc = nullptr;
+    float* ks = nullptr;       // NF_KV_E4M3: [B][nkv][L] scales
+    float* vs = nullptr;
     CUtensorMap tm_qkv{}, tm_o{};
     CUtensorMap tm_kc{}, tm_vc{};  // the caches as [B nkv L, 128] tensors for the attention's TMA tiles
     uint16_t bound = 0;        // bit per NF_STACK_* tensor
@@ -89,6 +93,19 @@ struct nf_stack {
     int* counters = nullptr;       // GEMM tile counters [2 * layers]
     int* err = nullptr;
     CUtensorMap tm_a{}, tm_a_s{}, tm_att{}, tm_att_s{};
+    // several rows of a sequence at a time, and E4M3 caches
+    int kv_kind = NF_KV_BF16;
+    nf_rope rope{};
+    bool rope_ok = false;
+    int32_t *row_seq = nullptr, *row_slot = nullptr, *row_pos = nullptr;  // [B] places of a step's rows
+    int32_t* iota = nullptr;       // [B + 1] 0, 1, 2, ...
+    void* tree_work = nullptr;
+    int last_rows = 0;             // rows of the last step enqueued
+
+    nf_kv_cache cache(int layer) const {
+        const StackLayer& l = layers[static_cast<size_t>(layer)];
+        return nf_kv_cache{l.kc, l.vc, l.ks, l.vs, kv_kind, d.max_batch, d.kv_heads, d.max_context, d.head_dim};
+    }
 
     int fail(int status, const char* fmt, ...) {
         char buf[512];
@@ -173,6 +190,10 @@ cudaError_t launch_projection(nf_stack* s, const CUtensorMap& tma, const CUtenso
 extern "C" {
 
 int nf_stack_create(const nf_stack_desc* desc, int device, nf_stack** out) {
+    return nf_stack_create_kv(desc, NF_KV_BF16, device, out);
+}
+
+int nf_stack_create_kv(const nf_stack_desc* desc, int kv_kind, int device, nf_stack** out) {
     std::string& err = g_stack_create_error;
     err.clear();
     if (!desc || !out) {
@@ -195,6 +216,10 @@ int nf_stack_create(const nf_stack_desc* desc, int device, nf_stack** out) {
         err = "max_batch in [1, 4096] and max_context in [1, 2^20]";
         return NF_ERR_INVALID;
     }
+    if (kv_kind != NF_KV_BF16 && kv_kind != NF_KV_E4M3) {
+        err = "unknown cache kind";
+        return NF_ERR_INVALID;
+    }
     if (d.dense_layers > 0 && (d.dense_inter < 128 || d.dense_inter % 128 != 0)) {
         err = "dense_inter must be a positive multiple of 128";
         return NF_ERR_SHAPE;
@@ -210,11 +235,17 @@ int nf_stack_create(const nf_stack_desc* desc, int device, nf_stack** out) {
     s->d = d;
     s->device = device;
     s->sms = gemm_grid_size(device);
+    s->kv_kind = kv_kind;
+    s->rope_ok = nf_rope_init(&s->rope, kHeadDim, kHeadDim, NF_ROPE_HALF, d.rope_theta, NF_ROPE_PLAIN, 1.0, 0.0, 0.0, 0.0) == NF_OK;
     s->layers.resize(static_cast<size_t>(d.layers));
     s->qkv_host.resize(static_cast<size_t>(d.layers));
     const int64_t B = d.max_batch, H = d.hidden, L = d.max_context, nkv = d.kv_heads;
     const int64_t NQKV = qkv_rows(d), NQ = static_cast<int64_t>(d.q_heads) * kHeadDim;
     int st = NF_OK;
+    if (kv_kind == NF_KV_E4M3 && !s->rope_ok) {
+        st = NF_ERR_INVALID;
+        err = nf_kv_last_error();
+    }
     // the FFN of every layer: dense NVFP4 MLP, NVFP4 MoE, or BF16-expert MoE
     for (int l = 0; l < d.layers && st == NF_OK; ++l) {
         nf_moe* f = nullptr;
@@ -231,15 +262,18 @@ int nf_stack_create(const nf_stack_desc* desc, int device, nf_stack** out) {
         s->layers[static_cast<size_t>(l)].ffn = f;
     }
     bool ok = st == NF_OK;
+    const size_t cache_bytes = static_cast<size_t>(B * nkv * L * kHeadDim) * (kv_kind == NF_KV_E4M3 ? 1 : 2);
     for (auto& Ly : s->layers) {
         if (!ok) break;
         ok = s->alloc(&Ly.w_qkv, static_cast<size_t>(box_order_bytes(NQKV, 2 * H))) &&
              s->alloc(&Ly.w_o, static_cast<size_t>(box_order_bytes(H, 2 * NQ))) && s->alloc(&Ly.attn_norm, H) &&
              s->alloc(&Ly.ffn_norm, H) && s->alloc(&Ly.q_norm, kHeadDim) && s->alloc(&Ly.k_norm, kHeadDim) &&
-             s->alloc(&Ly.kc, static_cast<size_t>(B * nkv * L * kHeadDim)) &&
-             s->alloc(&Ly.vc, static_cast<size_t>(B * nkv * L * kHeadDim));
-        if (ok) ok = cudaMemset(Ly.kc, 0, static_cast<size_t>(B * nkv * L * kHeadDim) * 2) == cudaSuccess &&
-                     cudaMemset(Ly.vc, 0, static_cast<size_t>(B * nkv * L * kHeadDim) * 2) == cudaSuccess;
+             s->alloc(&Ly.kc, cache_bytes / 2) && s->alloc(&Ly.vc, cache_bytes / 2);
+        if (ok) ok = cudaMemset(Ly.kc, 0, cache_bytes) == cudaSuccess && cudaMemset(Ly.vc, 0, cache_bytes) == cudaSuccess;
+        if (ok && kv_kind == NF_KV_E4M3)
+            ok = s->alloc(&Ly.ks, static_cast<size_t>(B * nkv * L)) && s->alloc(&Ly.vs, static_cast<size_t>(B * nkv * L)) &&
+                 cudaMemset(Ly.ks, 0, static_cast<size_t>(B * nkv * L) * 4) == cudaSuccess &&
+                 cudaMemset(Ly.vs, 0, static_cast<size_t>(B * nkv * L) * 4) == cudaSuccess;
     }
     const int64_t max_splits = kAttnMaxSplitsHost;
     ok = ok && s->alloc(&s->embed, static_cast<size_t>(d.vocab) * H) &&
@@ -251,6 +285,16 @@ int nf_stack_create(const nf_stack_desc* desc, int device, nf_stack** out) {
          s->alloc(&s->part_acc, B * d.q_heads * max_splits * kHeadDim) &&
          s->alloc(&s->counters, 2 * static_cast<size_t>(d.layers)) && s->alloc(&s->err, 1) &&
          cudaMemset(s->err, 0, 4) == cudaSuccess;
+    uint8_t* work = nullptr;
+    ok = ok && s->alloc(&s->row_seq, B) && s->alloc(&s->row_slot, B) && s->alloc(&s->row_pos, B) && s->alloc(&s->iota, B + 1) &&
+         s->alloc(&work, static_cast<size_t>(nf_tree_attention_workspace(kHeadDim))) &&
+         cudaMemset(s->att16, 0, static_cast<size_t>(B * NQ) * 2) == cudaSuccess;
+    s->tree_work = work;
+    if (ok) {
+        std::vector<int32_t> n(static_cast<size_t>(B) + 1);
+        for (size_t i = 0; i < n.size(); ++i) n[i] = static_cast<int32_t>(i);
+        ok = cudaMemcpy(s->iota, n.data(), n.size() * 4, cudaMemcpyHostToDevice) == cudaSuccess;
+    }
     if (ok)
         ok = make_tmap_2d(&s->tm_a, s->a16, true, H, B, 64, 128) && make_tmap_2d(&s->tm_a_s, s->a16, true, H, B, 64, 32) &&
              make_tmap_2d(&s->tm_att, s->att16, true, NQ, B, 64, 128) &&
@@ -384,8 +428,8 @@ int nf_stack_finalize(nf_stack* s) {
         const uint64_t cache_rows = static_cast<uint64_t>(d.max_batch) * d.kv_heads * d.max_context;
         if (!make_tmap_blocked(&Ly.tm_qkv, Ly.w_qkv, static_cast<uint64_t>(box_order_bytes(qkv_rows(d), 2 * H))) ||
             !make_tmap_blocked(&Ly.tm_o, Ly.w_o, static_cast<uint64_t>(box_order_bytes(H, 2 * NQ))) ||
-            !make_tmap_2d(&Ly.tm_kc, Ly.kc, true, kHeadDim, cache_rows, 64, 32) ||
-            !make_tmap_2d(&Ly.tm_vc, Ly.vc, true, kHeadDim, cache_rows, 64, 32))
+            (s->kv_kind == NF_KV_BF16 && (!make_tmap_2d(&Ly.tm_kc, Ly.kc, true, kHeadDim, cache_rows, 64, 32) ||
+                                          !make_tmap_2d(&Ly.tm_vc, Ly.vc, true, kHeadDim, cache_rows, 64, 32))))
             return s->fail(NF_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     }
     s->qkv_host.clear();
@@ -396,8 +440,15 @@ int nf_stack_finalize(nf_stack* s) {
 
 int nf_stack_kv_cache(nf_stack* s, int layer, uint16_t** k_dev, uint16_t** v_dev) {
     if (!s || !k_dev || !v_dev || layer < 0 || layer >= s->d.layers) return NF_ERR_INVALID;
+    if (s->kv_kind != NF_KV_BF16) return s->fail(NF_ERR_UNSUPPORTED, "the caches are not BF16: see nf_stack_kv");
     *k_dev = s->layers[static_cast<size_t>(layer)].kc;
     *v_dev = s->layers[static_cast<size_t>(layer)].vc;
+    return NF_OK;
+}
+
+int nf_stack_kv(nf_stack* s, int layer, nf_kv_cache* out) {
+    if (!s || !out || layer < 0 || layer >= s->d.layers) return NF_ERR_INVALID;
+    *out = s->cache(layer);
     return NF_OK;
 }
 
@@ -408,8 +459,22 @@ int nf_stack_load_kv(nf_stack* s, int layer, const uint16_t* k_host, const uint1
     cudaGetDevice(&prev);
     cudaSetDevice(s->device);
     const StackLayer& Ly = s->layers[static_cast<size_t>(layer)];
-    cudaError_t e = cudaMemcpy(Ly.kc, k_host, n * 2, cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaMemcpy(Ly.vc, v_host, n * 2, cudaMemcpyHostToDevice);
+    cudaError_t e = cudaSuccess;
+    if (s->kv_kind == NF_KV_BF16) {
+        e = cudaMemcpy(Ly.kc, k_host, n * 2, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaMemcpy(Ly.vc, v_host, n * 2, cudaMemcpyHostToDevice);
+    } else {
+        uint16_t* wide = nullptr;
+        e = cudaMalloc(&wide, n * 2);
+        for (int kv = 0; kv < 2 && e == cudaSuccess; ++kv) {
+            e = cudaMemcpy(wide, kv ? v_host : k_host, n * 2, cudaMemcpyHostToDevice);
+            if (e == cudaSuccess)
+                e = launch_kv_quantize(wide, static_cast<int64_t>(n / kHeadDim), kHeadDim,
+                                       reinterpret_cast<uint8_t*>(kv ? Ly.vc : Ly.kc), kv ? Ly.vs : Ly.ks, nullptr);
+            if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        }
+        cudaFree(wide);
+    }
     cudaSetDevice(prev);
     if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "cache upload: %s", cudaGetErrorString(e));
     return NF_OK;
@@ -422,32 +487,43 @@ int nf_stack_fill_kv(nf_stack* s, uint64_t seed) {
     cudaGetDevice(&prev);
     cudaSetDevice(s->device);
     cudaError_t e = cudaSuccess;
+    uint16_t* wide = nullptr;
+    const bool e4m3 = s->kv_kind == NF_KV_E4M3;
+    if (e4m3) e = cudaMalloc(&wide, static_cast<size_t>(n) * 2);
     for (int l = 0; l < s->d.layers && e == cudaSuccess; ++l) {
         const StackLayer& Ly = s->layers[static_cast<size_t>(l)];
-        e = launch_fill_bf16_hash(Ly.kc, n, seed * 1000003ull + 2ull * l, nullptr);
-        if (e == cudaSuccess) e = launch_fill_bf16_hash(Ly.vc, n, seed * 1000003ull + 2ull * l + 1ull, nullptr);
+        for (int kv = 0; kv < 2 && e == cudaSuccess; ++kv) {
+            uint16_t* cache = kv ? Ly.vc : Ly.kc;
+            e = launch_fill_bf16_hash(e4m3 ? wide : cache, n, seed * 1000003ull + 2ull * l + kv, nullptr);
+            if (e == cudaSuccess && e4m3)
+                e = launch_kv_quantize(wide, n / kHeadDim, kHeadDim, reinterpret_cast<uint8_t*>(cache), kv ? Ly.vs : Ly.ks, nullptr);
+        }
     }
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    cudaFree(wide);
     cudaSetDevice(prev);
     if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "cache fill: %s", cudaGetErrorString(e));
     return NF_OK;
 }
 
-int nf_stack_decode(nf_stack* s, const int32_t* tokens, const int32_t* positions, int batch, int32_t* next,
-                    float* final_dev, void* stream) {
-    if (!s) return NF_ERR_INVALID;
-    s->msg.clear();
-    if (!s->finalized) return s->fail(NF_ERR_STATE, "nf_stack_finalize has not run");
-    if (!tokens || !positions || !next) return s->fail(NF_ERR_INVALID, "null token, position or output pointer");
-    if (batch < 0 || batch > s->d.max_batch) return s->fail(NF_ERR_CAPACITY, "batch must be in [0, max_batch]");
-    if (batch == 0) return NF_OK;
+// The layers, the final norm and the lm_head of T rows.  tree: the rows'
+// sequences, places and masks (else row t is sequence t's next token at
+// positions[t], over BF16 caches).
+struct TreeRows {
+    const int32_t *row_start, *prefix, *seq, *slot, *pos;
+    int batch;
+    const uint64_t* mask;
+    int mask_words;
+};
+static int stack_step(nf_stack* s, const int32_t* tokens, const int32_t* positions, int T, const TreeRows* tree,
+                      float* final_dev, int32_t* next, void* stream) {
     const nf_stack_desc& d = s->d;
-    const int T = batch, H = d.hidden, nq = d.q_heads, nkv = d.kv_heads, L = d.max_context;
+    const int H = d.hidden, nq = d.q_heads, nkv = d.kv_heads, L = d.max_context;
     const int NQKV = qkv_rows(d), NQ = nq * kHeadDim;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     int prev = 0;
     cudaGetDevice(&prev);
     cudaSetDevice(s->device);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = launch_embed(s->embed, d.vocab, H, tokens, T, s->x, s->err, st);
     int status = NF_OK;
     const float eps = d.norm_eps;
@@ -459,12 +535,24 @@ int nf_stack_decode(nf_stack* s, const int32_t* tokens, const int32_t* positions
         if (e == cudaSuccess)
             e = launch_projection(s, s->tm_a, s->tm_a_s, Ly.tm_qkv, Ly.w_qkv, T, NQKV, H, s->qkv_part,
                                   s->counters + 2 * l, &S1, st);
-        if (e == cudaSuccess)
-            e = launch_qk_norm_rope(s->qkv_part, S1, static_cast<int64_t>(T) * NQKV, T, nq, nkv, Ly.q_norm, Ly.k_norm,
-                                    1e-5f, d.rope_theta, positions, L, s->q, Ly.kc, Ly.vc, s->err, st);
-        if (e == cudaSuccess)
-            e = launch_gqa_decode(Ly.tm_kc, Ly.tm_vc, s->q, positions, T, nq, nkv, L, splits, s->part_ml,
-                                  s->part_acc, s->att16, s->err, st);
+        if (tree) {
+            const nf_kv_cache cache = s->cache(l);
+            uint16_t* q16 = reinterpret_cast<uint16_t*>(s->q);
+            if (e == cudaSuccess)
+                e = launch_kv_write(cache, s->rope, s->qkv_part, NF_DTYPE_F32, NQKV, T, nq, Ly.q_norm, Ly.k_norm, 1e-5f, tree->pos,
+                                    tree->seq, tree->slot, q16, s->err, st, S1, static_cast<int64_t>(T) * NQKV);
+            if (e == cudaSuccess)
+                e = launch_tree_attention(cache, q16, T, nq, tree->row_start, tree->batch, tree->prefix, nullptr, tree->mask,
+                                          tree->mask_words, 1.f / sqrtf(static_cast<float>(kHeadDim)), s->att16, s->tree_work,
+                                          s->err, st);
+        } else {
+            if (e == cudaSuccess)
+                e = launch_qk_norm_rope(s->qkv_part, S1, static_cast<int64_t>(T) * NQKV, T, nq, nkv, Ly.q_norm, Ly.k_norm,
+                                        1e-5f, d.rope_theta, positions, L, s->q, Ly.kc, Ly.vc, s->err, st);
+            if (e == cudaSuccess)
+                e = launch_gqa_decode(Ly.tm_kc, Ly.tm_vc, s->q, positions, T, nq, nkv, L, splits, s->part_ml,
+                                      s->part_acc, s->att16, s->err, st);
+        }
         if (e == cudaSuccess)
             e = launch_projection(s, s->tm_att, s->tm_att_s, Ly.tm_o, Ly.w_o, T, H, NQ, s->o_part,
                                   s->counters + 2 * l + 1, &S2, st);
@@ -484,8 +572,76 @@ int nf_stack_decode(nf_stack* s, const int32_t* tokens, const int32_t* positions
     if (status != NF_OK) return status;
     if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "decode launch: %s", cudaGetErrorString(e));
     int tst = nf_tp_linear_bf16(s->head, s->lm_head, d.vocab, H, final_dev ? final_dev : s->fin, T, nullptr, stream);
-    if (tst == NF_OK) tst = nf_tp_argmax(s->head, T, d.vocab, next, stream);
+    if (tst == NF_OK && next) tst = nf_tp_argmax(s->head, T, d.vocab, next, stream);
     if (tst != NF_OK) return s->fail(tst, "lm_head: %s", nf_tp_last_error(s->head));
+    s->last_rows = T;
+    return NF_OK;
+}
+
+int nf_stack_decode(nf_stack* s, const int32_t* tokens, const int32_t* positions, int batch, int32_t* next,
+                    float* final_dev, void* stream) {
+    if (!s) return NF_ERR_INVALID;
+    s->msg.clear();
+    if (!s->finalized) return s->fail(NF_ERR_STATE, "nf_stack_finalize has not run");
+    if (!tokens || !positions || !next) return s->fail(NF_ERR_INVALID, "null token, position or output pointer");
+    if (batch < 0 || batch > s->d.max_batch) return s->fail(NF_ERR_CAPACITY, "batch must be in [0, max_batch]");
+    if (batch == 0) return NF_OK;
+    if (s->kv_kind == NF_KV_BF16) return stack_step(s, tokens, positions, batch, nullptr, final_dev, next, stream);
+    const TreeRows rows{s->iota, positions, nullptr, nullptr, positions, batch, nullptr, 0};
+    return stack_step(s, tokens, positions, batch, &rows, final_dev, next, stream);
+}
+
+int nf_stack_verify(nf_stack* s, const int32_t* tokens, const int32_t* depth, const int32_t* row_start,
+                    const int32_t* prefix, const uint64_t* mask, int mask_words, int rows, int batch, int32_t* next,
+                    float* final_dev, void* stream) {
+    if (!s) return NF_ERR_INVALID;
+    s->msg.clear();
+    if (!s->finalized) return s->fail(NF_ERR_STATE, "nf_stack_finalize has not run");
+    if (rows < 0 || rows > s->d.max_batch || batch < 0 || batch > s->d.max_batch)
+        return s->fail(NF_ERR_CAPACITY, "rows and batch must be in [0, max_batch]");
+    if (mask && (mask_words < 1 || mask_words > 64)) return s->fail(NF_ERR_SHAPE, "mask_words must be in [1, 64]");
+    if (reinterpret_cast<uintptr_t>(mask) % 8 != 0) return s->fail(NF_ERR_LAYOUT, "the mask must be 8-byte aligned");
+    if (!s->rope_ok) return s->fail(NF_ERR_INVALID, "rope_theta must be finite and > 0");
+    if (rows == 0 || batch == 0) return NF_OK;
+    if (!tokens || !row_start || !prefix) return s->fail(NF_ERR_INVALID, "null token, row_start or prefix pointer");
+    int prev = 0;
+    cudaGetDevice(&prev);
+    cudaSetDevice(s->device);
+    const cudaError_t e = launch_kv_places(rows, row_start, batch, prefix, depth, s->row_seq, s->row_slot, s->row_pos,
+                                           static_cast<cudaStream_t>(stream));
+    cudaSetDevice(prev);
+    if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "verify launch: %s", cudaGetErrorString(e));
+    const TreeRows tree{row_start, prefix, s->row_seq, s->row_slot, s->row_pos, batch, mask, mask_words};
+    return stack_step(s, tokens, nullptr, rows, &tree, final_dev, next, stream);
+}
+
+int nf_stack_logprobs(nf_stack* s, int rows, const int32_t* target, int top, float* logprob, float* entropy,
+                      int32_t* top_idx, float* top_lp, void* stream) {
+    if (!s) return NF_ERR_INVALID;
+    s->msg.clear();
+    if (rows > s->last_rows) return s->fail(NF_ERR_STATE, "the last step had %d rows", s->last_rows);
+    const int st = nf_tp_logprobs(s->head, rows, s->d.vocab, target, top, logprob, entropy, top_idx, top_lp, stream);
+    if (st != NF_OK) return s->fail(st, "lm_head: %s", nf_tp_last_error(s->head));
+    return NF_OK;
+}
+
+int nf_stack_accept(nf_stack* s, const int32_t* prefix, const int32_t* path, int max_path, const int32_t* path_len,
+                    int batch, void* stream) {
+    if (!s) return NF_ERR_INVALID;
+    s->msg.clear();
+    if (batch < 0 || batch > s->d.max_batch) return s->fail(NF_ERR_CAPACITY, "batch must be in [0, max_batch]");
+    if (max_path < 0) return s->fail(NF_ERR_INVALID, "max_path must be >= 0");
+    if (batch == 0 || max_path == 0) return NF_OK;
+    if (!prefix || !path || !path_len) return s->fail(NF_ERR_INVALID, "null prefix, path or length pointer");
+    std::vector<nf_kv_cache> caches;
+    for (int l = 0; l < s->d.layers; ++l) caches.push_back(s->cache(l));
+    int prev = 0;
+    cudaGetDevice(&prev);
+    cudaSetDevice(s->device);
+    const cudaError_t e = launch_kv_accept(caches.data(), s->d.layers, prefix, path, max_path, path_len, nullptr, batch, s->err,
+                                           static_cast<cudaStream_t>(stream));
+    cudaSetDevice(prev);
+    if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "accept launch: %s", cudaGetErrorString(e));
     return NF_OK;
 }
 

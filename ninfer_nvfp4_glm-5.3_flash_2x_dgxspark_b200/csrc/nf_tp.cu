@@ -27,6 +27,7 @@
 
 #include "nf_common.cuh"
 #include "nf_internal.h"
+#include "nf_kv.h"
 #include "nf_nccl.h"
 
 #include <algorithm>
@@ -633,6 +634,26 @@ int nf_tp_argmax(nf_tp* h, int tokens, int64_t rows, int32_t* idx, void* stream)
     const cudaError_t e = cudaGetLastError();
     cudaSetDevice(prev);
     if (e != cudaSuccess) return h->fail(NF_ERR_CUDA, "argmax launch: %s", cudaGetErrorString(e));
+    return NF_OK;
+}
+
+int nf_tp_logprobs(nf_tp* h, int tokens, int64_t rows, const int32_t* target, int top, float* logprob, float* entropy,
+                   int32_t* top_idx, float* top_lp, void* stream) {
+    if (!h) return NF_ERR_INVALID;
+    h->msg.clear();
+    if (tokens < 0 || tokens > h->max_tokens || rows < 1 || rows > h->max_rows || rows > 0x7fffffffll)
+        return h->fail(NF_ERR_CAPACITY, "tokens or rows beyond the handle's capacity");
+    if (top < 0 || top > 32 || top > rows) return h->fail(NF_ERR_UNSUPPORTED, "top must be in [0, 32] and at most rows");
+    if (!target != !logprob) return h->fail(NF_ERR_INVALID, "targets and log-probabilities go together");
+    if (tokens == 0) return NF_OK;
+    if (top > 0 && (!top_idx || !top_lp)) return h->fail(NF_ERR_INVALID, "null top pointer");
+    int prev = 0;
+    cudaGetDevice(&prev);
+    cudaSetDevice(h->device);
+    const cudaError_t e = launch_token_logprobs(h->mbox + kFlagsBytes, NF_DTYPE_F32, rows, tokens, rows, target, top, logprob,
+                                                entropy, top_idx, top_lp, static_cast<cudaStream_t>(stream), h->epoch, h->cap);
+    cudaSetDevice(prev);
+    if (e != cudaSuccess) return h->fail(NF_ERR_CUDA, "log-probability launch: %s", cudaGetErrorString(e));
     return NF_OK;
 }
 

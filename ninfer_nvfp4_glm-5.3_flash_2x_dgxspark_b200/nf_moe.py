@@ -48,7 +48,8 @@ EXPORTED = [
     "nf_stack_last_error", "nf_stack_layer_ffn", "nf_stack_bind_bf16", "nf_stack_bind_f32", "nf_stack_finalize",
     "nf_stack_kv_cache", "nf_stack_decode", "nf_stack_sync", "nf_stack_load_kv", "nf_stack_fill_kv",
     "nf_kv_last_error", "nf_rope_init", "nf_kv_write", "nf_tree_attention_workspace", "nf_tree_attention",
-    "nf_token_logprobs_workspace", "nf_token_logprobs", "nf_kv_accept",
+    "nf_token_logprobs_workspace", "nf_token_logprobs", "nf_kv_accept", "nf_tp_logprobs", "nf_stack_create_kv",
+    "nf_stack_kv", "nf_stack_verify", "nf_stack_logprobs", "nf_stack_accept",
 ]
 STAGES = ["router", "permute", "gate_up", "down", "shared", "combine"]
 
@@ -161,6 +162,12 @@ def load() -> ctypes.CDLL:
         "nf_token_logprobs_workspace": ([I32, I64, I32], I64),
         "nf_token_logprobs": ([P, I32, I64, I32, I64, P, I32, P, P, P, P, P, I64, P], I32),
         "nf_kv_accept": ([P, I32, P, P, I32, P, P, I32, P, P], I32),
+        "nf_tp_logprobs": ([P, I32, I64, P, I32, P, P, P, P, P], I32),
+        "nf_stack_create_kv": ([ctypes.POINTER(StackDesc), I32, I32, ctypes.POINTER(P)], I32),
+        "nf_stack_kv": ([P, I32, P], I32),
+        "nf_stack_verify": ([P, P, P, P, P, P, I32, I32, I32, P, P, P], I32),
+        "nf_stack_logprobs": ([P, I32, P, I32, P, P, P, P, P], I32),
+        "nf_stack_accept": ([P, P, P, I32, P, I32, P], I32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -721,6 +728,17 @@ class TpGroup:
         self._check(self.lib.nf_tp_argmax(self.h, tokens, rows, _dev(idx, n, ("torch.int32",), "idx", self.device),
                                           stream or None))
 
+    def logprobs(self, tokens: int, rows: int, targets, logprob, entropy=None, top_idx=None, top_logprob=None,
+                 stream=0) -> None:
+        """Log-probabilities of the last linear's output (nf_tp_logprobs; the
+        buffers of token_logprobs)."""
+        dv, top = self.device, _top(top_idx, top_logprob)
+        n = tokens if 0 <= tokens <= self.max_tokens else 0
+        self._check(self.lib.nf_tp_logprobs(
+            self.h, tokens, rows, _buf(targets, n, _K.i32, "targets", dv), top, _buf(logprob, n, _K.f32, "logprob", dv),
+            _buf(entropy, n, _K.f32, "entropy", dv), _buf(top_idx, n * top, _K.i32, "top_idx", dv),
+            _buf(top_logprob, n * top, _K.f32, "top_logprob", dv), stream or None))
+
     def sync(self, stream=0) -> None:
         self._check(self.lib.nf_tp_sync(self.h, stream or None))
 
@@ -773,17 +791,20 @@ class DecoderStack:
                  dense_inter: int, experts: int, top_k: int, inter: int, shared_inter: int, routed_scaling: float,
                  swiglu_limit: float = 10.0, q_heads: int, kv_heads: int, head_dim: int = 128,
                  rope_theta: float = 10000.0, norm_eps: float = 1e-5, max_batch: int = 1, max_context: int = 2048,
-                 device: int = 0):
+                 device: int = 0, kv: str = "bf16"):
+        """kv: the caches' kind, "bf16" or "e4m3"."""
         self.lib = load()
+        if kv not in KV_KIND:
+            raise NfError(1, f"unknown cache kind {kv!r}")
         moe = Desc(hidden, experts, top_k, inter, shared_inter, 1, 1, 1, routed_scaling, swiglu_limit, EXPERTS_NVFP4,
                    max_batch)
         self.desc = StackDesc(vocab, hidden, layers, dense_layers, bf16_expert_layers, dense_inter, moe, q_heads,
                               kv_heads, head_dim, rope_theta, norm_eps, max_batch, max_context)
         h = ctypes.c_void_p()
-        st = self.lib.nf_stack_create(ctypes.byref(self.desc), device, ctypes.byref(h))
+        st = self.lib.nf_stack_create_kv(ctypes.byref(self.desc), KV_KIND[kv], device, ctypes.byref(h))
         if st != NF_OK:
             raise NfError(st, self.lib.nf_stack_last_error(None).decode())
-        self.h, self.device = h, device
+        self.h, self.device, self.kv = h, device, kv
 
     def close(self) -> None:
         if getattr(self, "h", None):
@@ -875,12 +896,59 @@ class DecoderStack:
                                              _dev(final_dev, n * d.hidden, ("torch.float32",), "final", dv),
                                              stream or None))
 
+    def kv_desc(self, layer: int) -> "KvDesc":
+        """The layer's caches (device pointers; valid as long as the stack)."""
+        d = KvDesc()
+        st = self.lib.nf_stack_kv(self.h, layer, ctypes.byref(d))
+        if st != NF_OK:
+            raise NfError(st, f"layer {layer} out of range")
+        return d
+
+    def verify(self, tokens_dev, row_start, prefix, rows: int, next_dev=None, final_dev=None, *, depth=None, mask=None,
+               stream=0) -> None:
+        """One step over several new tokens of every sequence (nf_stack_verify):
+        int32 tokens, depth and next [rows], row_start [batch + 1], prefix
+        [batch]; mask 64-bit words [rows, words] or None (chains); final fp32
+        [rows, H].  Asynchronous on `stream`."""
+        d, dv = self.desc, self.device
+        batch = _dim(row_start, 0, "row_start", 1) - 1
+        if batch < 0:
+            raise NfError(2, "row_start holds no sequence")
+        n, b = (v if 0 <= v <= d.max_batch else 0 for v in (rows, batch))
+        words = 0 if mask is None else _dim(mask, 1, "mask", 2)
+        self._check(self.lib.nf_stack_verify(
+            self.h, _buf(tokens_dev, n, _K.i32, "tokens", dv), _buf(depth, n, _K.i32, "depth", dv),
+            _buf(row_start, b + 1, _K.i32, "row_start", dv), _buf(prefix, b, _K.i32, "prefix", dv),
+            _buf(mask, n * words, _K.u64, "mask", dv), words, rows, batch, _buf(next_dev, n, _K.i32, "next", dv),
+            _buf(final_dev, n * d.hidden, _K.f32, "final", dv), stream or None))
+
+    def logprobs(self, rows: int, targets, logprob, entropy=None, top_idx=None, top_logprob=None, stream=0) -> None:
+        """Log-probabilities of the last step's rows (nf_stack_logprobs; the
+        buffers of token_logprobs)."""
+        dv, top = self.device, _top(top_idx, top_logprob)
+        n = rows if 0 <= rows <= self.desc.max_batch else 0
+        self._check(self.lib.nf_stack_logprobs(
+            self.h, rows, _buf(targets, n, _K.i32, "targets", dv), top, _buf(logprob, n, _K.f32, "logprob", dv),
+            _buf(entropy, n, _K.f32, "entropy", dv), _buf(top_idx, n * top, _K.i32, "top_idx", dv),
+            _buf(top_logprob, n * top, _K.f32, "top_logprob", dv), stream or None))
+
+    def accept(self, prefix, path, path_len, stream=0) -> None:
+        """Keeps the accepted path of every sequence's last verify in all
+        layers' caches (nf_stack_accept): int32 prefix and path_len [batch],
+        path [batch, max_path]."""
+        batch, longest = _dim(path, 0, "path", 2), path.shape[1]
+        dv, b = self.device, batch if batch <= self.desc.max_batch else 0
+        self._check(self.lib.nf_stack_accept(self.h, _buf(prefix, b, _K.i32, "prefix", dv),
+                                             _buf(path, b * longest, _K.i32, "path", dv), longest,
+                                             _buf(path_len, b, _K.i32, "path_len", dv), batch, stream or None))
+
     def sync(self, stream=0) -> None:
         self._check(self.lib.nf_stack_sync(self.h, stream or None))
 
 
 # ---- verifying drafted tokens: cache, tree attention, log-probabilities --------
 KV_BF16, KV_E4M3 = 0, 1
+KV_KIND = dict(bf16=KV_BF16, e4m3=KV_E4M3)
 DTYPE_F32, DTYPE_BF16 = 0, 1
 ROPE_LAYOUT = dict(half=0, interleaved=1)
 ROPE_SCALING = dict(none=0, linear=1, yarn=2)
@@ -929,6 +997,13 @@ def _dim(a, axis: int, name: str, rank: int) -> int:
     if len(a.shape) != rank:
         raise NfError(2, f"{name} has {len(a.shape)} axes; expected {rank}")
     return a.shape[axis]
+
+
+def _top(top_idx, top_logprob) -> int:
+    """How many top tokens the buffers ask for."""
+    if (top_idx is None) != (top_logprob is None):
+        raise NfError(1, "top_idx and top_logprob go together")
+    return 0 if top_idx is None else _dim(top_idx, 1, "top_idx", 2)
 
 
 class KvCache:
@@ -1066,9 +1141,7 @@ def token_logprobs(logits, targets, logprob, entropy, top_idx, top_logprob, work
     kind = _K.number.get(logits.dtype)
     if kind is None:
         raise NfError(1, f"logits has dtype {logits.dtype}; expected float32 or bfloat16")
-    if (top_idx is None) != (top_logprob is None):
-        raise NfError(1, "top_idx and top_logprob go together")
-    top = 0 if top_idx is None else _dim(top_idx, 1, "top_idx", 2)
+    top = _top(top_idx, top_logprob)
     _kv_check(load().nf_token_logprobs(
         logits.data_ptr(), kind,
         logits.stride(0) if rows > 1 else max(1, vocab), rows, vocab, _buf(targets, rows, _K.i32, "targets", dv), top,

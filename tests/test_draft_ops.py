@@ -196,3 +196,16 @@ def test_python_calls_refuse_host_tensors():
         m.token_logprobs(torch.zeros(2, 8), None, None, None, None, None, None)
     with pytest.raises(m.NfError, match="no caches"):
         m.KvCaches([])
+
+
+def test_handle_calls_refuse_without_gpu():
+    lib = m.load()
+    assert lib.nf_stack_verify(None, None, None, None, None, None, 0, 1, 1, None, None, None) == 1
+    assert lib.nf_stack_logprobs(None, 1, None, 0, None, None, None, None, None) == 1
+    assert lib.nf_stack_accept(None, None, None, 1, None, 1, None) == 1
+    assert lib.nf_stack_kv(None, 0, None) == 1
+    assert lib.nf_tp_logprobs(None, 1, 10, None, 0, None, None, None, None, None) == 1
+    h = ctypes.c_void_p()
+    d = m.StackDesc(100, 256, 1, 0, 0, 0, m.Desc(256, 8, 2, 128, 128, 1, 1, 1, 1.0, 10.0, 0, 4), 8, 1, 128, 10000.0, 1e-5, 4, 64)
+    assert lib.nf_stack_create_kv(ctypes.byref(d), 7, 0, ctypes.byref(h)) == 1 and not h.value
+    assert b"cache kind" in lib.nf_stack_last_error(None)
