@@ -776,9 +776,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             float other_m = -INFINITY, other_l = 0.f;
             if (!pair) {
                 // both streams hold parts of the same rows: exchange (m, l), then each finishes half of the columns
+                tc_fence_before();
+                __syncwarp();
                 if (lane == 0) mbar_arrive(ml_in);
                 wait(ml_in, ml_n & 1u);
                 __syncwarp();
+                tc_fence_after();
                 const float2 o = s_ml[(s ^ 1) * kTileRows + r];
                 other_m = o.x;
                 other_l = o.y;
@@ -819,8 +822,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                 *reinterpret_cast<uint4*>(dst + 32 * c + 2 * j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4)
-                                *reinterpret_cast<float4*>(part_o + 32 * c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                            for (int j = 0; j < 32; j += 8)
+                                st_global_v8(part_o + 32 * c + j, __float_as_uint(o[j]), __float_as_uint(o[j + 1]),
+                                             __float_as_uint(o[j + 2]), __float_as_uint(o[j + 3]), __float_as_uint(o[j + 4]),
+                                             __float_as_uint(o[j + 5]), __float_as_uint(o[j + 6]), __float_as_uint(o[j + 7]));
                         }
                     }
                 }
