@@ -240,8 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
     TileInfo* s_info = reinterpret_cast<TileInfo*>(sm + G_::kInfoAt);
-    using ItemWalk = Walk<kItemRows, kKeys>;
-    const Share share = find_share<D, kThreads, 2, ItemWalk>(a, s_share);
+    using ItemWalk = Walk<kItemRows, kKeys, 8, 2, 3>;
+    const Share share = find_share<D, kThreads, 1, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;
     const uint32_t tmem = *s_tmem;
     volatile int* abort_flag = s_abort;

@@ -133,16 +133,18 @@ struct ShareScratch {
 
 // ---------------------------------------------------------------------------
 // The work: every (sequence, KV head, up to ROWS rows) is an item of ceil(keys
-// / KEYS) tiles.  A tile weighs 1, or 2 when the item's rows fill two tcgen05
-// tiles.  The items in order (sequence, head, rows) form one line of weight,
-// which the CTAs cut into equal shares; a tile belongs to the share in which
-// it starts.  So the SMs get the same work whatever the lengths, and a long
+// / KEYS) tiles.  An item weighs ITEM, for its start and end, and a tile ONE, or
+// TWO when the item's rows fill two tcgen05 tiles.  The items in order
+// (sequence, head, rows) form one line of weight, each item's ITEM before its
+// tiles, which the CTAs cut into equal shares; a tile belongs to the share in
+// which it starts.  So the SMs get the same work whatever the lengths, and a long
 // sequence is cut into as many parts as it has shares.  One warp walks through
 // the parts of the CTA's share and publishes them to the others in a ring of
 // descriptors.
 // ---------------------------------------------------------------------------
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int ITEM, int ONE, int TWO>
 struct Walk {
+    static constexpr int kTile = ONE > TWO ? ONE : TWO;  // the most that a tile weighs
     // the sequence
     int i, first, n, p0, sq, npt;
     // the part: rows [row0, row0 + rows) of KV head g, tiles [t0, t1) of kt
@@ -169,7 +171,13 @@ struct Walk {
         keys = p0 + (a.mask ? n : min(n, (row0 + rows - 1) / a.G + 1));
         kt = (keys + KEYS - 1) / KEYS;
     }
-    __device__ __forceinline__ int weight() const { return pair() ? 2 * kt : kt; }
+    // where the item's tile t starts, from the item's start, and the first tile that starts at `w` or behind it
+    __device__ __forceinline__ int64_t tile_at(int t) const { return ITEM + static_cast<int64_t>(t) * (pair() ? TWO : ONE); }
+    __device__ __forceinline__ int tile_from(int64_t w) const {
+        const int64_t x = max(w - ITEM, static_cast<int64_t>(0));
+        return static_cast<int>(min(static_cast<int64_t>(kt), pair() ? (x + TWO - 1) / TWO : (x + ONE - 1) / ONE));
+    }
+    __device__ __forceinline__ int64_t weight() const { return tile_at(kt); }
     // weight of the sequence's items of one head
     __device__ __forceinline__ int64_t head_weight(const TreeArgs& a) {
         int64_t w = 0;
@@ -208,7 +216,7 @@ struct Walk {
         p.kind = (t0 == 0) | (t1 == kt) << 1;
         if (p.kind == 1) {
             JoinDesc d{};
-            d.parts = static_cast<int>((at + (static_cast<int64_t>(kt - 1) << (pair() ? 1 : 0))) / s.per) - static_cast<int>(blockIdx.x) + 1;
+            d.parts = static_cast<int>((at + tile_at(kt - 1)) / s.per) - static_cast<int>(blockIdx.x) + 1;
             d.rows = rows;
             d.row0 = row0;
             d.first = first;
@@ -240,17 +248,17 @@ struct Walk {
                 }
             }
             item(a);
-            const int two = pair() ? 1 : 0;  // tile t starts at weight at + (t << two)
-            t0 = lo > at ? static_cast<int>(min(static_cast<int64_t>(kt), (lo - at + two) >> two)) : 0;
-            t1 = static_cast<int>(min(static_cast<int64_t>(kt), (hi - at + two) >> two));
+            t0 = tile_from(lo - at);
+            t1 = tile_from(hi - at);
             if (t0 < t1) return;
         }
     }
 };
 
 // Finds the CTA's share (every thread sums the weights of a run of sequences) and fills the rows of bad sequences with NaN.  A share
-// is not smaller than LEAST, the weight that a CTA takes at a time: smaller
-// ones would only make more parts to join.  Ends with a __syncthreads.
+// is not smaller than LEAST tiles, those that a CTA takes at a time: smaller
+// ones would only make more parts to join, and no share inside an item may be
+// without a tile.  Ends with a __syncthreads.
 template <int D, int THREADS, int LEAST, typename W>
 __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -287,7 +295,7 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
         total += sh.warp[k];
     }
     Share s;
-    s.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(LEAST));
+    s.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(LEAST * W::kTile));
     s.lo = s.per * blockIdx.x;
     s.hi = min(total, s.lo + s.per);
     if (mine > 0 && s.lo >= base && s.lo < base + mine) {
