@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
     TileInfo* s_info = reinterpret_cast<TileInfo*>(sm + G_::kInfoAt);
-    using ItemWalk = Walk<kItemRows, kKeys, 8, 2, 3>;
+    using ItemWalk = Walk<kItemRows, kKeys, 10, 2, 3>;
     const Share share = find_share<D, kThreads, 1, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;
     const uint32_t tmem = *s_tmem;
@@ -412,8 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // ----------------------- the walk, and q's rows into swizzled tiles
         ItemWalk w;
         w.start(a, share, s_share);
-        int at = 0;
-        for (int idx = 0;; ++idx) {
+        auto publish = [&](int idx) {
             const int r = idx % kParts;
             if (idx >= kParts) wait(&pt_empty[r], ((idx / kParts) & 1u) ^ 1u);
             if (lane == 0) {
@@ -421,26 +420,39 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 mbar_arrive(&pt_full[r]);
             }
             __syncwarp();
-            if (!w.valid || *abort_flag) break;
-            for (int sub = 0; sub < (w.pair() ? 2 : 1); ++sub, ++at) {
+        };
+        publish(0);
+        int at = 0;
+        for (int idx = 1; w.valid && !*abort_flag; ++idx) {
+            // the next part is published first: its keys are on their way while these rows are fetched
+            const int row0 = w.row0, all = w.rows;
+            const uint16_t* q = a.q + (static_cast<int64_t>(w.first) * a.nq + w.g * a.G) * D;
+            w.seek(a, false);
+            publish(idx);
+            constexpr int C = D / 8, S = 32 / C;  // 16-byte chunks of a row; rows at a time
+            const int ch = lane % C;
+            for (int r0 = 0; r0 < all; r0 += kTileRows, ++at) {
                 const int slot = at & 1;
                 if (at >= 2) wait(&q_empty[slot], ((at >> 1) & 1u) ^ 1u);
-                const uint32_t dst = smem_u32(sm + G_::kQ + slot * G_::kTileBytes);
-                const int rows = min(kTileRows, w.rows - sub * kTileRows);
-                constexpr int C = D / 8;  // 16-byte chunks of a row
-                for (int e = lane; e < rows * C; e += 32) {
-                    const int r = e / C, ch = e % C, row = w.row0 + sub * kTileRows + r;
-                    const uint16_t* src =
-                        a.q + (static_cast<int64_t>(w.first + row / a.G) * a.nq + w.g * a.G + row % a.G) * D + ch * 8;
-                    const uint32_t to = dst + (ch >> 3) * G_::kHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                const uint32_t dst = smem_u32(sm + G_::kQ + slot * G_::kTileBytes) + (ch >> 3) * G_::kHalf;
+                int node = (row0 + r0 + lane / C) / a.G, h = row0 + r0 + lane / C - node * a.G;
+                const int rows = min(kTileRows, all - r0);
+#pragma unroll 4
+                for (int r = lane / C; r < rows; r += S) {
+                    const uint16_t* src = q + (static_cast<int64_t>(node) * a.nq + h) * D + ch * 8;
+                    const uint32_t to = dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+                    h += S;
+                    while (h >= a.G) {
+                        h -= a.G;
+                        ++node;
+                    }
                 }
                 asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[slot]);
             }
-            w.seek(a, false);
         }
     } else if (warp == kScaleWarp) {
         // ------------------- E4M3: a task's 128 key scales (times c) and value scales

@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
     }
     __syncthreads();
     pdl_trigger();  // the join's blocks may wait for this grid beside it
-    using ItemWalk = Walk<kRows, kKeys, 0, 1, 1>;
+    using ItemWalk = Walk<kRows, kKeys, 8, 1, 1>;
     const Share share = find_share<D, G_::kThreads, G_::kGroups, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;
     volatile int* abort_flag = s_abort;
