@@ -10,6 +10,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 namespace nf {
 
@@ -82,7 +83,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // E neighbouring dims as loaded: 4-byte words, of one F32 or two BF16 dims.
 template <int W>
 __device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
-    if (W == 2) {
+    if (W == 1) {
+        w[0] = __ldg(static_cast<const uint32_t*>(p));
+    } else if (W == 2) {
         const uint2 v = __ldg(static_cast<const uint2*>(p));
         w[0] = v.x;
         w[W - 1] = v.y;
@@ -103,7 +106,8 @@ __device__ __forceinline__ void store_bf16(uint16_t* dst, const float* x) {
 #pragma unroll
     for (int e = 0; e < E; e += 2) w[e / 2] = bf16x2_hw(x[e], x[e + 1]);
     if (E == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[E / 2 - 2], w[E / 2 - 1]);
-    else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else if (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[E / 2 - 1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
 }
 
 // A lane's dims of a row whose greatest magnitude is `peak` as E4M3 codes;
@@ -138,24 +142,35 @@ __device__ __forceinline__ float half_warp_peak(const float (&y)[E]) {
     return peak;
 }
 
-template <int D, bool BF16>
+// FULL: the two halves of all dims rotate with one another.  Then a lane holds
+// E / 2 dims of either half, so that its pairs need no exchange.
+template <int D, bool BF16, bool FULL>
 __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
     const __grid_constant__ nf_kv_cache c, const __grid_constant__ nf_rope rope, const void* __restrict__ qkv,
     int slices, int64_t slice_stride, int64_t row_stride, int nq, const float* __restrict__ q_norm,
     const float* __restrict__ k_norm, float eps, const int32_t* __restrict__ pos, const int32_t* __restrict__ seq,
     const int32_t* __restrict__ slot, uint16_t* __restrict__ q_out, int32_t* __restrict__ status) {
-    constexpr int E = D / 16, W = BF16 ? E / 2 : E;
+    constexpr int E = D / 16, W = BF16 ? E / 2 : E, H = FULL ? E / 2 : E, kSize = BF16 ? 2 : 4;
     const int step = blockDim.x >> 4;  // heads at a time
     __shared__ float2 s_turn[D / 2];  // (cos, sin) of every pair's angle, times the magnitude
-    __shared__ float s_row[2 * kWriteWarps][D];
+    __shared__ float s_row[FULL ? 1 : 2 * kWriteWarps][FULL ? 1 : D];
     const int sub = threadIdx.x >> 4, lane = threadIdx.x & 15;  // which half warp, and the lane in it
     const int nkv = c.kv_heads, heads = nq + 2 * nkv, t = blockIdx.x;
-    const uint8_t* row = static_cast<const uint8_t*>(qkv) + (static_cast<int64_t>(t) * row_stride + lane * E) * (BF16 ? 2 : 4);
+    auto dim = [&](int e) { return (e < H ? 0 : D / 2 - H) + lane * H + e; };  // the lane's e-th
+    const uint8_t* row = static_cast<const uint8_t*>(qkv) + (static_cast<int64_t>(t) * row_stride + lane * H) * kSize;
+    auto fetch = [&](int64_t at, uint32_t* w) {
+        if constexpr (FULL) {
+            load_words<W / 2>(row + at * kSize, w);
+            load_words<W / 2>(row + (at + D / 2) * kSize, w + W / 2);
+        } else {
+            load_words<W>(row + at * kSize, w);
+        }
+    };
     uint32_t next[W];
     auto load = [&](int h) {
-        if (h < heads) load_words<W>(row + static_cast<int64_t>(h) * D * (BF16 ? 2 : 4), next);
+        if (h < heads) fetch(static_cast<int64_t>(h) * D, next);
     };
-    load(sub);
+    load(sub < nq ? sub : nq + sub);
 
     const int p = pos[t], sq = seq ? seq[t] : t, sl = slot ? slot[t] : p;
     const bool ok = p >= 0 && (sl == -1 || (sq >= 0 && sq < c.seqs && sl >= 0 && sl < c.max_context));
@@ -173,15 +188,15 @@ __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
     float wq[E], wk[E];  // the norms' weights of the lane's dims
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        wq[e] = q_norm ? __ldg(q_norm + lane * E + e) : 1.f;
-        wk[e] = k_norm ? __ldg(k_norm + lane * E + e) : 1.f;
+        wq[e] = q_norm ? __ldg(q_norm + dim(e)) : 1.f;
+        wk[e] = k_norm ? __ldg(k_norm + dim(e)) : 1.f;
     }
     __syncthreads();
     // the lane's dims' angles, the same in every head; dims behind rd do not turn
     float co[E], si[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int i = lane * E + e;
+        const int i = dim(e);
         const float2 f = i >= rd ? make_float2(1.f, 0.f) : s_turn[inter ? i >> 1 : i < half ? i : i - half];
         co[e] = f.x;
         si[e] = (inter ? (i & 1) == 0 : i < half) ? -f.y : f.y;  // first a cos - b sin, second b cos + a sin
@@ -190,10 +205,7 @@ __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
     const int other = (threadIdx.x & 16) + ((lane * E < half ? lane + half / E : lane - half / E) & 15);
     const int64_t base = sl < 0 ? 0 : static_cast<int64_t>(sq) * nkv * c.max_context + sl;
 
-#pragma unroll 1
-    for (int h = sub; h - sub < heads; h += step) {  // both halves of a warp take the same steps
-        const bool is_q = h < nq, is_k = !is_q && h < nq + nkv, in = h < heads;
-        float y[E];
+    auto take = [&](int h, bool in, int following, float (&y)[E]) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const uint32_t w = next[BF16 ? e / 2 : e];
@@ -203,68 +215,104 @@ __global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
 #pragma unroll 1
             for (int k = 1; k < slices; ++k) {
                 uint32_t w[W];
-                load_words<W>(row + (k * slice_stride + static_cast<int64_t>(h) * D) * 4, w);
+                fetch(k * slice_stride + static_cast<int64_t>(h) * D, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) y[e] = __fadd_rn(y[e], __uint_as_float(w[BF16 ? 0 : e]));
             }
-        load(h + step);
-        if (__any_sync(0xffffffffu, is_q || is_k)) {
-            if (q_norm || k_norm) {
-                float ss = 0.f;
+        load(following);
+    };
+    auto normalise = [&](float (&y)[E], const float (&w)[E], bool on) {
+        float ss = 0.f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) ss = __fmaf_rn(y[e], y[e], ss);
-                ss = half_warp_sum(ss);
-                const float inv = rsqrtf(__fmaf_rn(ss, 1.f / D, eps));
-                if (is_q ? q_norm != nullptr : is_k && k_norm)
+        for (int e = 0; e < E; ++e) ss = __fmaf_rn(y[e], y[e], ss);
+        ss = half_warp_sum(ss);
+        const float inv = rsqrtf(__fmaf_rn(ss, 1.f / D, eps));
+        if (on)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) y[e] = __fmul_rn(__fmul_rn(y[e], inv), is_q ? wq[e] : wk[e]);
+            for (int e = 0; e < E; ++e) y[e] = __fmul_rn(__fmul_rn(y[e], inv), w[e]);
+    };
+    auto rotate = [&](float (&y)[E], bool on) {
+        if (rd == 0) return;
+        float z[E];
+        if (FULL) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) z[e] = y[e < H ? e + H : e - H];
+        } else if (inter) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) z[e] = y[e ^ 1];
+        } else if (near) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) z[e] = __shfl_sync(0xffffffffu, y[e], other);
+        } else {
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < E; ++e) s_row[FULL ? 0 : sub][FULL ? 0 : lane * E + e] = y[e];
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = lane * E + e;
+                z[e] = i >= rd ? 0.f : s_row[FULL ? 0 : sub][FULL ? 0 : i < half ? i + half : i - half];
             }
-            if (rd > 0) {
-                float z[E];
-                if (inter) {
+        }
+        if (on)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) z[e] = y[e ^ 1];
-                } else if (near) {
+            for (int e = 0; e < E; ++e)
+                if (FULL || lane * E + e < rd) y[e] = fmaf(z[e], si[e], y[e] * co[e]);
+    };
+    auto store = [&](uint16_t* dst, const float (&y)[E]) {
+        if constexpr (FULL) {
+            store_bf16<H>(dst + lane * H, y);
+            store_bf16<H>(dst + D / 2 + lane * H, y + H);
+        } else {
+            store_bf16<E>(dst + lane * E, y);
+        }
+    };
+
+    // q's heads, then K's and V's; both halves of a warp take the same steps
+#pragma unroll 1
+    for (int h = sub; h - sub < nq; h += step) {
+        const bool in = h < nq;
+        float y[E];
+        take(h, in, h + step < nq ? h + step : nq + sub, y);
+        if (q_norm) normalise(y, wq, true);
+        rotate(y, true);
+        if (!in) continue;
+        if (!ok)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) z[e] = __shfl_sync(0xffffffffu, y[e], other);
-                } else {
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < E; ++e) s_row[sub][lane * E + e] = y[e];
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const int i = lane * E + e;
-                        z[e] = i >= rd ? 0.f : s_row[sub][i < half ? i + half : i - half];
-                    }
-                }
-                if (is_q || is_k)
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (lane * E + e < rd) y[e] = fmaf(z[e], si[e], y[e] * co[e]);
-            }
+            for (int e = 0; e < E; ++e) y[e] = NAN;
+        store(q_out + (static_cast<int64_t>(t) * nq + h) * D, y);
+    }
+#pragma unroll 1
+    for (int h = nq + sub; h - sub < heads; h += step) {
+        const bool in = h < heads, is_k = h < nq + nkv;
+        float y[E];
+        take(h, in, h + step, y);
+        if (__any_sync(0xffffffffu, is_k)) {
+            if (k_norm) normalise(y, wk, is_k);
+            rotate(y, is_k);
         }
         float peak = 0.f;
-        if (c.kind == NF_KV_E4M3 && __any_sync(0xffffffffu, in && !is_q)) peak = half_warp_peak<E>(y);
-        if (!in) continue;
-        if (is_q) {
-            if (!ok)
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[e] = NAN;
-            store_bf16<E>(q_out + (static_cast<int64_t>(t) * nq + h) * D + lane * E, y);
-            continue;
-        }
-        if (!ok || sl < 0) continue;
+        if (c.kind == NF_KV_E4M3) peak = half_warp_peak<E>(y);
+        if (!in || !ok || sl < 0) continue;
         const int64_t r = base + static_cast<int64_t>(is_k ? h - nq : h - nq - nkv) * c.max_context;
         if (c.kind == NF_KV_BF16) {
-            store_bf16<E>(static_cast<uint16_t*>(is_k ? c.k : c.v) + r * D + lane * E, y);
+            store(static_cast<uint16_t*>(is_k ? c.k : c.v) + r * D, y);
             continue;
         }
         uint32_t code[E / 4];
         const float scale = quantize_row<E>(y, peak, code);
-        uint8_t* dst = static_cast<uint8_t*>(is_k ? c.k : c.v) + r * D + lane * E;
-        if (E == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[E / 4 - 1]);
-        else *reinterpret_cast<uint32_t*>(dst) = code[0];
+        uint8_t* dst = static_cast<uint8_t*>(is_k ? c.k : c.v) + r * D + lane * H;
+        if constexpr (FULL && E == 8) {
+            *reinterpret_cast<uint32_t*>(dst) = code[0];
+            *reinterpret_cast<uint32_t*>(dst + D / 2) = code[E / 4 - 1];
+        } else if constexpr (FULL) {
+            *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(code[0]);
+            *reinterpret_cast<uint16_t*>(dst + D / 2) = static_cast<uint16_t>(code[0] >> 16);
+        } else if constexpr (E == 8) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[E / 4 - 1]);
+        } else {
+            *reinterpret_cast<uint32_t*>(dst) = code[0];
+        }
         if (lane == 0) (is_k ? c.k_scale : c.v_scale)[r] = scale;
     }
 }
@@ -388,8 +436,15 @@ cudaError_t launch_kv_write(const nf_kv_cache& c, const nf_rope& rope, const voi
                             int32_t* status, cudaStream_t st, int slices, int64_t slice_stride) {
     if (tokens <= 0) return cudaSuccess;
     const bool bf16 = qkv_type == NF_DTYPE_BF16;
-    auto kernel = c.head_dim == 128 ? (bf16 ? kv_write_kernel<128, true> : kv_write_kernel<128, false>)
-                                    : (bf16 ? kv_write_kernel<64, true> : kv_write_kernel<64, false>);
+    const bool full = rope.rotary_dim == c.head_dim && rope.layout == NF_ROPE_HALF;
+    auto pick = [&](auto d, auto f) {
+        return bf16 ? kv_write_kernel<decltype(d)::value, true, decltype(f)::value>
+                    : kv_write_kernel<decltype(d)::value, false, decltype(f)::value>;
+    };
+    using Wide = std::integral_constant<int, 128>;
+    using Narrow = std::integral_constant<int, 64>;
+    auto kernel = c.head_dim == 128 ? (full ? pick(Wide(), std::true_type()) : pick(Wide(), std::false_type()))
+                                    : (full ? pick(Narrow(), std::true_type()) : pick(Narrow(), std::false_type()));
     // Few tokens: more warps share a token's heads (1 token, 40 heads of 128: 4.0 us with 8 warps, 4.8 with 4; 600 tokens:
     // 9.2 and 6.9); many: fewer, so that less of the time goes to what is done once per token (8,192 tokens: 57.8 us with
     // 4, 51.0 with 2).
