@@ -145,7 +145,7 @@ __device__ __forceinline__ float half_warp_peak(const float (&y)[E]) {
 // FULL: the two halves of all dims rotate with one another.  Then a lane holds
 // E / 2 dims of either half, so that its pairs need no exchange.
 template <int D, bool BF16, bool FULL>
-__global__ void __launch_bounds__(32 * kWriteWarps, 3) kv_write_kernel(
+__global__ void __launch_bounds__(32 * kWriteWarps, 4) kv_write_kernel(
     const __grid_constant__ nf_kv_cache c, const __grid_constant__ nf_rope rope, const void* __restrict__ qkv,
     int slices, int64_t slice_stride, int64_t row_stride, int nq, const float* __restrict__ q_norm,
     const float* __restrict__ k_norm, float eps, const int32_t* __restrict__ pos, const int32_t* __restrict__ seq,
