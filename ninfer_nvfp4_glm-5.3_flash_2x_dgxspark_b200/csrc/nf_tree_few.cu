@@ -33,7 +33,10 @@ struct Geo {
     static constexpr int kRows = 8 * NT;
     static constexpr int kPitch = D + 8;        // floats of an output row in shared memory
     static constexpr int kTileBytes = kKeys * D * (FP8 ? 1 : 2);  // K or V
-    static constexpr int kStages = (FP8 ? 10 : 5) - (NT - 1) * (FP8 ? 2 : 1);
+    // A multiple of kGroups: then a stage is always the same group's, which has waited for its load before when it waits
+    // for the next.  Loads may land out of order, and another group's wait could take the phase before for its own.
+    static constexpr int kStages = FP8 ? 8 : 4;
+    static_assert(kStages % kGroups == 0);
     static constexpr int kOutAt = kStages * 2 * kTileBytes;             // [warp][row][D] floats
     static constexpr int kMlAt = kOutAt + kWarps * kRows * kPitch * 4;  // [warp][row] (m, l)
     static constexpr int kQPitch = 2 * D + 16;  // bytes of a row of q

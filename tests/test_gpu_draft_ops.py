@@ -427,6 +427,42 @@ def test_attention_repeats_bit_for_bit():
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("batch, nodes", [(32, 1), (24, 2), (12, 16)])
+def test_attention_from_cold_memory(kind, batch, nodes):
+    """Long caches that the L2 does not hold, whose loads land in any order."""
+    nq, nkv, dim, context = 32, 4, 128, 4000
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    x = [torch.randn(batch, nkv, context, dim, device="cuda", generator=g) for _ in range(2)]
+    if kind == "bf16":
+        c = m.KvCache(*(t.bfloat16() for t in x))
+        k, v = (t.double() for t in c.tensors[:2])
+    else:
+        s = [0.01 * torch.rand(batch, nkv, context, device="cuda", generator=g) for _ in x]
+        c = m.KvCache(*((60 * t).clamp(-448, 448).to(torch.float8_e4m3fn) for t in x), *s)
+        k, v = (t.float().double() * f.double()[..., None] for t, f in zip(c.tensors[:2], s))
+    q = torch.randn(batch * nodes, nq, dim, device="cuda", generator=g).bfloat16()
+    lengths = [context - nodes - 37 * i for i in range(batch)]
+    start, prefix = ints(range(0, batch * nodes + 1, nodes)), ints(lengths)
+    work = torch.empty(m.tree_attention_workspace(dim), dtype=torch.uint8, device="cuda")
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    outs = []
+    for _ in range(10):
+        flush.zero_()
+        outs.append(torch.empty_like(q))
+        m.tree_attention(c, q, start, prefix, outs[-1], work)
+    torch.cuda.synchronize()
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+    for i in (0, batch // 2, batch - 1):
+        for r in {0, nodes - 1}:
+            for h in (0, nkv - 1):
+                heads = slice(h * nq // nkv, (h + 1) * nq // nkv)
+                want, tol = exact_attention(q[i * nodes + r, heads].double().cpu().numpy(), k[i, h].cpu().numpy(),
+                                            v[i, h].cpu().numpy(), np.arange(context) <= lengths[i] + r, dim ** -0.5)
+                err = np.abs(outs[0][i * nodes + r, heads].double().cpu().numpy() - want)
+                assert np.all(err <= tol), (i, r, h, float(err.max()))
+
+
 def test_attention_refuses_tensors():
     rng = np.random.default_rng(1)
     c, _, _ = make_cache(rng, "bf16", 2, 2, 8, 64)
