@@ -59,11 +59,14 @@ namespace {
 // kv_write: a CTA per token, half a warp per head in turn; lane l of 16 holds
 // the head's dims l D / 16 .. (l + 1) D / 16 - 1.  The bytes of q, k and v are
 // the floor; what bounds it is the instructions issued, of which half are per
-// head and not per dim, so a warp takes two heads at a time.  The rows of
-// kAhead heads are on their way at a time, and the angles' sines are taken
-// once per token, while these come in.  A rotated pair lies in a lane
-// (interleaved), or in two lanes whose distance is the pairs' (halves, when
-// that is a whole number of lanes), else it goes through shared memory.
+// head and not per dim, so a warp takes two heads at a time.  The next heads'
+// rows are on their way meanwhile, and the angles' sines are taken once per
+// token, while the first come in.  A rotated pair lies in a lane (interleaved;
+// FULL below), or in two lanes whose distance is the pairs' (halves, when that
+// is a whole number of lanes), else it goes through shared memory.
+// 8,192 tokens, 32 + 2 x 4 heads of 128, BF16 to E4M3: 43 us, 3.7 TB/s of the
+// bytes; exchanging the pairs' dims between lanes it was 51.  Two or three
+// heads ahead instead of one: 50.
 // ---------------------------------------------------------------------------
 constexpr int kWriteWarps = 8;  // at most
 
@@ -445,9 +448,9 @@ cudaError_t launch_kv_write(const nf_kv_cache& c, const nf_rope& rope, const voi
     using Narrow = std::integral_constant<int, 64>;
     auto kernel = c.head_dim == 128 ? (full ? pick(Wide(), std::true_type()) : pick(Wide(), std::false_type()))
                                     : (full ? pick(Narrow(), std::true_type()) : pick(Narrow(), std::false_type()));
-    // Few tokens: more warps share a token's heads (1 token, 40 heads of 128: 4.0 us with 8 warps, 4.8 with 4; 600 tokens:
-    // 9.2 and 6.9); many: fewer, so that less of the time goes to what is done once per token (8,192 tokens: 57.8 us with
-    // 4, 51.0 with 2).
+    // Few tokens: more warps share a token's heads; many: fewer, so that less of the time goes to what is done once per
+    // token.  Measured with 8, 4, 2 warps (us between events, 40 heads of 128, BF16 rows): 64 tokens 9.2 10.2 13.2;
+    // 600: 13.3 12.3 14.4; 1,000: 15.3 13.3 15.4; 2,000: 22.5 19.4 17.5; 8,192: 64.5 50.2 48.0 (one warp: 48.2).
     const int warps = tokens <= 2 * 148 ? kWriteWarps : tokens <= 1000 ? 4 : 2;
     kernel<<<static_cast<unsigned>(tokens), 32 * warps, 0, st>>>(c, rope, qkv, slices, slice_stride, row_stride, q_heads,
                                                                  q_norm, k_norm, eps, pos, seq, slot, q, status);

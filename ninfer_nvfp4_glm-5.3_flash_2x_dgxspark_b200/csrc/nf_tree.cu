@@ -1029,9 +1029,15 @@ cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int r
     if (!sms[dev]) sms[dev] = std::min(kMaxCtas, gemm_grid_size(dev));
     const int grid = sms[dev];
     const bool fp8 = c.kind == NF_KV_E4M3, wide = c.head_dim == 128;
-    // by the rows of an average item; either kernel is right for every item
+    // By the rows that a sequence has per KV head, on average; any choice is right for any rows.  Measured (us, 32
+    // sequences on 4,000 keys, D 128, 4 KV heads, keys from DRAM) with items of 8 rows, 16 rows, and the kernel for many:
+    //   rows      8             16            24            32            64
+    //   E4M3  37.9 52.2 66.6  48.1 56.3 66.6  54.3 62.5 72.7  72.7 74.8 72.7  130 114 72.7
+    //   BF16  50.2 52.2 60.4  58.4 54.3 62.4  74.8 62.5 62.5  97.3 72.7 62.5  175 114 64.5
+    // and one sequence on 65,000 keys: E4M3, 32 rows: 62.5 64.5 72.7; BF16, 24 rows: 80.9 68.6 70.7.  E4M3's keys take
+    // longer to convert than a second look at them in the L2.
     const int64_t all = static_cast<int64_t>(rows) * a.G;
-    const int nt = all <= 8ll * batch ? 1 : all <= static_cast<int64_t>(kFewRows) * batch ? 2 : 0;
+    const int nt = all <= (fp8 ? 32ll : 8ll) * batch ? 1 : !fp8 && all <= 24ll * batch ? 2 : 0;
     cudaError_t e = nt    ? launch_tree_few(c, a, nt, grid, st)
                     : fp8 ? (wide ? launch_many<128, true>(c, a, grid, st) : launch_many<64, true>(c, a, grid, st))
                           : (wide ? launch_many<128, false>(c, a, grid, st) : launch_many<64, false>(c, a, grid, st));

@@ -21,7 +21,6 @@ namespace nf {
 constexpr int kStatusBad = NF_DEVERR_BAD_TOKEN;
 constexpr int kTileRows = 128;   // rows per tcgen05 tile
 constexpr int kItemRows = 256;   // most rows of a work item
-constexpr int kFewRows = 16;     // most rows of a work item of the kernel for few rows
 constexpr int kMaxCtas = 148;    // CTAs (one per SM) the workspace has parts for
 constexpr int kParts = 8;        // part descriptors in flight
 constexpr uint64_t kWaitNs = 10000000000ull;  // some waits last as long as a whole part
@@ -315,7 +314,7 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
     return s;
 }
 
-// The kernel for few rows (nf_tree_few.cu), with items of up to 8 nt rows.
+// The kernel for few rows (nf_tree_few.cu), with items of up to 8 nt rows; E4M3: nt 1.
 cudaError_t launch_tree_few(const nf_kv_cache& c, const TreeArgs& a, int nt, int grid, cudaStream_t st);
 
 }  // namespace nf

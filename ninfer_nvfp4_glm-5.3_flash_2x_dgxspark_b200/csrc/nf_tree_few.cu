@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kKeys = 64;     // keys per tile
 
-// NT: column tiles of 8 rows (1 or 2).
+// NT: column tiles of 8 rows (1, or with BF16 2).
 template <int D, bool FP8, int NT>
 struct Geo {
     static constexpr int kWarps = 8;            // consuming warps
@@ -329,7 +329,8 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
             // E4M3: the weights p * (value's scale) enter the product as F16 times inv, a power of two that keeps the
-            // row's largest weight so far, ref (as the running max has it), within [2^-4, 2^15]
+            // row's largest weight so far, ref (as the running max has it), within [2^8, 2^15]: F16's last place is then
+            // below 2^-32 of it, where a weight is rounded otherwise by 2^-11 of itself
             float m[NT][2], l[NT][2], ref[NT][2], inv[NT][2];
 #pragma unroll
             for (int c = 0; c < NT; ++c)
@@ -462,8 +463,8 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                                 wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 16));
                                 ref[c][e] = fmaxf(ref[c][e] * f[c][e], wm);
                                 const float top = ref[c][e] * inv[c][e];
-                                if (__builtin_expect(ref[c][e] > 0.f && !(top >= 0.0625f && top <= 32768.f), 0)) {
-                                    const int ex = min(max(258 - static_cast<int>(__float_as_uint(ref[c][e]) >> 23), 7), 247);
+                                if (__builtin_expect(ref[c][e] > 0.f && !(top >= 256.f && top <= 32768.f), 0)) {
+                                    const int ex = min(max(266 - static_cast<int>(__float_as_uint(ref[c][e]) >> 23), 7), 247);
                                     const float to = __uint_as_float(static_cast<uint32_t>(ex) << 23);
                                     f[c][e] *= fminf(to / inv[c][e], 1.7e38f);
                                     inv[c][e] = to;
@@ -583,17 +584,17 @@ cudaError_t launch(const nf_kv_cache& c, const TreeArgs& a, int grid, cudaStream
     tree_few_kernel<D, FP8, NT><<<grid, G_::kThreads, G_::kSmem, st>>>(tmk, tmv, a);
     return cudaGetLastError();
 }
-template <int D, bool FP8>
-cudaError_t launch_nt(const nf_kv_cache& c, const TreeArgs& a, int nt, int grid, cudaStream_t st) {
-    return nt == 1 ? launch<D, FP8, 1>(c, a, grid, st) : launch<D, FP8, 2>(c, a, grid, st);
+template <int D>
+cudaError_t launch_dim(const nf_kv_cache& c, const TreeArgs& a, int nt, int grid, cudaStream_t st) {
+    return c.kind == NF_KV_E4M3 ? launch<D, true, 1>(c, a, grid, st)
+           : nt == 1            ? launch<D, false, 1>(c, a, grid, st)
+                                : launch<D, false, 2>(c, a, grid, st);
 }
 
 }  // namespace
 
 cudaError_t launch_tree_few(const nf_kv_cache& c, const TreeArgs& a, int nt, int grid, cudaStream_t st) {
-    if (c.head_dim == 128)
-        return c.kind == NF_KV_E4M3 ? launch_nt<128, true>(c, a, nt, grid, st) : launch_nt<128, false>(c, a, nt, grid, st);
-    return c.kind == NF_KV_E4M3 ? launch_nt<64, true>(c, a, nt, grid, st) : launch_nt<64, false>(c, a, nt, grid, st);
+    return c.head_dim == 128 ? launch_dim<128>(c, a, nt, grid, st) : launch_dim<64>(c, a, nt, grid, st);
 }
 
 }  // namespace nf
