@@ -372,6 +372,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 #pragma unroll
                     for (int j = 0; j < kKeys / 16; ++j)
                         mma_bf16_ts(tmem + 256 + s * D, tmem + s * kKeys + j * 8, vd + j * (2048 >> 4), id_o, !(start && j == 0));
+                    if (FP8 && v.tail())
+#pragma unroll
+                        for (int j = 0; j < kKeys / 16; ++j)
+                            mma_bf16_ts(tmem + 256 + s * D, tmem + s * kKeys + kKeys / 2 + j * 8, vd + j * (2048 >> 4), id_o, 1);
                     if (v.done()) tc_commit(&kv_empty[v_stage]);
                     if (last) tc_commit(&o_full[s]);
                 }
@@ -738,6 +742,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             }
                         }
                         tmem_st_pairs(t_s + lane0, pk);
+                        if (FP8 && __builtin_expect(tail, 0)) {
+                            // What the rounding to BF16 leaves, for a second product: rows that see a few drafted keys
+                            // would else carry the rounding of one key's scale in all their dims.
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const uint64_t g = *reinterpret_cast<const uint64_t*>(sc + kKeys + 8 * i);
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint64_t y = add_f32x2(
+                                        f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), nm[h]);
+                                    const uint64_t pr = mul_f32x2(f32x2_pack(ex2(f32x2_lo(y)), ex2(f32x2_hi(y))), g);
+                                    const uint32_t hi = pk[2 * i + h];
+                                    const float a0 = __uint_as_float(hi << 16), a1 = __uint_as_float(hi & 0xffff0000u);
+                                    pk[2 * i + h] = bf16x2_hw(isinf(a0) ? 0.f : f32x2_lo(pr) - a0, isinf(a1) ? 0.f : f32x2_hi(pr) - a1);
+                                }
+                            }
+                            tmem_st_pairs(t_s + lane0 + kKeys / 2, pk);
+                        }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) l[h] += f32x2_lo(sum[h]) + f32x2_hi(sum[h]);  // of the thread's columns
                     }
