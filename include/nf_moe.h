@@ -575,8 +575,11 @@ NF_API int nf_kv_write(const nf_kv_cache* cache, const nf_rope* rope, const void
  *   workspace_dev   nf_tree_attention_workspace(head_dim) bytes, 256-byte
  *                   aligned: calls in flight at the same time need one each
  * q_heads a multiple of kv_heads, at most 128 per KV head; mask_words 1 to 64.
- * Scores, softmax statistics and sums are F32; the probabilities are rounded
- * to BF16 for the product with the values.  What the cache holds outside the
+ * Scores, softmax statistics and sums are F32.  For the product with the
+ * values the probabilities (E4M3: times the value's scale) are rounded to
+ * BF16, with the rest as a second BF16 term in E4M3 tiles that hold new rows,
+ * or, with an E4M3 cache and few rows, to F16 (one below 2^-22 of the row's
+ * largest by up to 2^-32 of that one).  What the cache holds outside the
  * positions a row sees never reaches the row's result.  Rows behind
  * row_start_dev[batch] stay as they were; the rows of a sequence whose
  * prefix, rows or cache sequence lie outside the buffers become NaN, and
@@ -602,7 +605,9 @@ NF_API int nf_tree_attention(const nf_kv_cache* cache, const uint16_t* q_dev, in
  * has no distribution: its log-probabilities and entropy are NaN, its top
  * indices still those of the order above.
  * workspace_dev: nf_token_logprobs_workspace(rows, vocab, top) bytes, 16-byte
- * aligned; calls in flight at the same time need one each. */
+ * aligned; calls in flight at the same time need one each (what the CTAs of a
+ * row exchange travels through their cluster's shared memory, so it is small
+ * and its contents do not matter). */
 NF_API int64_t nf_token_logprobs_workspace(int rows, int64_t vocab, int top);
 NF_API int nf_token_logprobs(const void* logits_dev, int logits_type, int64_t row_stride, int rows, int64_t vocab,
                              const int32_t* target_dev, int top, float* logprob_dev, float* entropy_dev,

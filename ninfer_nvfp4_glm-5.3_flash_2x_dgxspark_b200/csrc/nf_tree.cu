@@ -7,6 +7,18 @@
 // that take turns: while one stream's scores go through the softmax, the other
 // stream's products run.  An item of more than 128 rows gives each stream its
 // own 128 rows over the same tiles; a smaller one gives them every other tile.
+//
+// Per tile of 128 keys and 256 rows (D 128) the tensor cores need 2,048 cycles
+// and the exponentials 2,048; it takes 6,200.  What bounds it is the chain of a
+// stream: scores (512 cycles), softmax (2,000 alone, 3,000 to 4,000 beside the
+// other stream's and the E4M3 widening on the same schedulers), product with V
+// (512), and the barriers between them; a stream's scores and probabilities
+// share their 128 TMEM columns, as two streams with outputs of 128 columns
+// leave no room for a second set.  More and smaller tasks (64 keys, scores a
+// task ahead) took 20% longer, twice the softmax warps 8%.
+// 4 sequences of 64 nodes, 8 rows a node, on up to 65,000 E4M3 keys: 231 us,
+// 570 TFLOP/s; 24 of 16 nodes on 8,191 BF16 keys, where a tile of 128 rows
+// waits for its 64 KB more than for the products: 77 us, 4.0 TB/s.
 #include "nf_tree.cuh"
 
 #include <algorithm>
@@ -241,6 +253,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     Part* s_part = reinterpret_cast<Part*>(sm + G_::kPartAt);
     TileInfo* s_info = reinterpret_cast<TileInfo*>(sm + G_::kInfoAt);
     using ItemWalk = Walk<kItemRows, kKeys, 10, 2, 3>;
+    // Weights in units of about 2,070 cycles, from the CTAs' times: a tile with two row tiles 6,200, with one 4,200, an
+    // item's start and end 17,000 to 24,000.  With tiles alone a few CTAs took 1.5 times the others' (287 us above).
     const Share share = find_share<D, kThreads, 1, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;
     const uint32_t tmem = *s_tmem;
