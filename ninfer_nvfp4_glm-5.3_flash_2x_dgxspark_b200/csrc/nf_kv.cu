@@ -393,14 +393,14 @@ __device__ __forceinline__ void move_rows(uint8_t* base, int64_t pitch, const in
 }
 
 __global__ void __launch_bounds__(128) kv_accept_kernel(const __grid_constant__ AcceptCaches a, int e4m3, int seqs,
-                                                        int nkv, int L, int row_bytes,
+                                                        int nkv, int L, int row_bytes, int first,
                                                         const int32_t* __restrict__ prefix,
                                                         const int32_t* __restrict__ path, int max_path,
                                                         const int32_t* __restrict__ path_len,
                                                         const int32_t* __restrict__ cache_seq,
                                                         int32_t* __restrict__ status) {
     const int i = blockIdx.y, layer = blockIdx.z;
-    const int n = path_len[i], p0 = prefix[i], sq = cache_seq ? cache_seq[i] : i;
+    const int n = path_len[i], p0 = prefix[i], sq = cache_seq ? cache_seq[i] : first + i;
     const int32_t* pa = path + static_cast<int64_t>(i) * max_path;
     bool ok = n >= 0 && n <= max_path && p0 >= 0 && p0 <= L && sq >= 0 && sq < seqs;
     if (ok) {
@@ -492,7 +492,7 @@ cudaError_t launch_kv_accept(const nf_kv_cache* caches, int layers, const int32_
         for (int i0 = 0; i0 < batch; i0 += 65535) {
             const int nb = std::min(65535, batch - i0);
             kv_accept_kernel<<<dim3(gx, nb, n), 128, 0, st>>>(a, c.kind == NF_KV_E4M3, c.seqs, c.kv_heads,
-                                                              c.max_context, row_bytes, prefix + i0,
+                                                              c.max_context, row_bytes, i0, prefix + i0,
                                                               path + static_cast<int64_t>(i0) * max_path, max_path,
                                                               path_len + i0, cache_seq ? cache_seq + i0 : nullptr, status);
             const cudaError_t e = cudaGetLastError();

@@ -641,7 +641,100 @@ def test_accept_bad_paths():
             assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
 
 
+def test_accept_more_sequences_than_a_grid_has_rows():
+    n = 70000
+    k = torch.arange(n, device="cuda").remainder(251).to(torch.int16)[:, None, None, None].repeat(1, 1, 2, 64)
+    k[:, :, 1] += 1000
+    c = m.KvCache(k, k.clone())
+    m.kv_accept(m.KvCaches([c]), ints(np.zeros(n)), ints(np.ones((n, 1))), ints(np.ones(n)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t[:, :, 0], t[:, :, 1]) and torch.equal(t[:, 0, 1, 5], k[:, 0, 1, 5]) for t in c.tensors[:2])
+    assert k[66000, 0, 0, 0].item() == 66000 % 251 + 1000
+
+
 # ------------------------------------------------------------------------------------------------------------- together
+def test_offsets_beyond_32_bits():
+    """The last sequence of a cache of more than 2^32 codes: written, read by both attention kernels, and moved."""
+    seqs, nkv, context, dim, nq = 33, 4, 1 << 18, 128, 32
+    assert seqs * nkv * context * dim > 1 << 32
+    code = [torch.zeros(seqs, nkv, context, dim, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scale = [torch.zeros(seqs, nkv, context, device="cuda") for _ in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for t, f in zip(code, scale):
+        t[-1] = (60 * torch.randn(nkv, context, dim, device="cuda", generator=g)).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+        f[-1] = 0.01 * torch.rand(nkv, context, device="cuda", generator=g)
+    c = m.KvCache(code[0], code[1], scale[0], scale[1])
+    host = lambda t, f, h, n: t[-1, h, :n].view(torch.float8_e4m3fn).double().cpu().numpy() * f[-1, h, :n].double().cpu().numpy()[:, None]  # noqa: E731
+    work = torch.empty(m.tree_attention_workspace(dim), dtype=torch.uint8, device="cuda")
+    for rows in (3, 40):
+        prefix = context - rows
+        slots = ints(range(prefix, context))
+        qkv = torch.randn(rows, (nq + 2 * nkv) * dim, device="cuda", generator=g)
+        q = torch.empty(rows, nq, dim, dtype=torch.bfloat16, device="cuda")
+        out, status = torch.empty_like(q), ints([0])
+        m.kv_write(c, m.Rope(dim, rotary_dim=0), qkv, nq, slots, q, seqs=ints([seqs - 1] * rows), slots=slots, status=status)
+        m.tree_attention(c, q, ints([0, rows]), ints([prefix]), out, work, cache_seq=ints([seqs - 1]), status=status)
+        torch.cuda.synchronize()
+        assert status.item() == 0
+        wrote = qkv.view(rows, -1, dim)[:, nq + nkv - 1].double().cpu().numpy()
+        got = host(code[0], scale[0], nkv - 1, context)[prefix:]
+        assert np.all(np.abs(got - wrote) <= H_E4M3 * np.abs(wrote) + 2.0 ** -10 * np.abs(wrote).max(1, keepdims=True) / 448 * 1.001)
+        heads = slice(nq - nq // nkv, nq)
+        for r in (0, rows - 1):
+            want, tol = exact_attention(q[r, heads].double().cpu().numpy(), host(code[0], scale[0], nkv - 1, context),
+                                        host(code[1], scale[1], nkv - 1, context), np.arange(context) <= prefix + r, dim ** -0.5)
+            err = np.abs(out[r, heads].double().cpu().numpy() - want)
+            assert np.all(err <= tol), (rows, r, float(err.max()))
+    last = code[0][-1, :, context - 1].clone()
+    m.kv_accept(m.KvCaches([c]), ints([context - 40]), ints([[39]]), ints([1]), cache_seq=ints([seqs - 1]))
+    torch.cuda.synchronize()
+    assert torch.equal(code[0][-1, :, context - 40], last) and not code[0][:-1].any()
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured: nothing is set up that a capture forbids."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    script = """
+import sys; sys.path.insert(0, %r)
+import torch
+from helpers import nfm
+m = nfm()
+g = torch.Generator(device="cuda").manual_seed(1)
+k, v = (torch.randn(2, 2, 64, 128, device="cuda", generator=g).bfloat16() for _ in range(2))
+qkv = torch.randn(40, 20 * 128, device="cuda", generator=g)
+i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+slots, seqs, start, prefix = i(list(range(20)) * 2), i([0] * 20 + [1] * 20), i([0, 20, 40]), i([0, 0])
+path, length, target = i([[1], [2]]), i([1, 1]), i([3] * 40)
+q = torch.empty(40, 16, 128, dtype=torch.bfloat16, device="cuda")
+out, lp = torch.zeros_like(q), torch.zeros(40, device="cuda")
+work = torch.empty(m.tree_attention_workspace(128), dtype=torch.uint8, device="cuda")
+c, rope = m.KvCache(k, v), m.Rope(128)
+cs = m.KvCaches([c])
+def step(s):
+    m.kv_write(c, rope, qkv, 16, slots, q, seqs=seqs, slots=slots, stream=s)
+    m.tree_attention(c, q, start, prefix, out, work, stream=s)                       # many rows
+    m.tree_attention(c, q[:2], i2, prefix, out[:2], work, stream=s)                  # few
+    m.token_logprobs(out.view(40, -1), target, lp, None, None, None, work, stream=s)
+    m.kv_accept(cs, prefix, path, length, stream=s)
+i2 = i([0, 1, 2])
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step(torch.cuda.current_stream().cuda_stream)
+k0, v0 = k.clone(), v.clone()
+graph.replay(); torch.cuda.synchronize()
+first = [t.clone() for t in (out, lp, k, v)]
+k.copy_(k0); v.copy_(v0); step(0); torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(first, (out, lp, k, v)))
+print("same")
+""" % here
+    r = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("kind", ["e4m3", "bf16"])
 def test_operators_in_a_graph_on_a_side_stream(kind):
     """Write, attend, log-probabilities and accept captured on another stream and replayed give what the eager calls give;
