@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace nf {
 
@@ -667,9 +668,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 if (FP8) wait(&sc_full[2 * s + b], (mine_n >> 1) & 1u);
                 __syncwarp();
                 tc_fence_after();
-                const bool tail = (t + 1) * kKeys > p0;
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
+                // a tile with drafted keys has code of its own, so that the other's stays short
+                auto half_rows = [&](int half, auto tail) {
+                    constexpr bool kTail = decltype(tail)::value;
                     if (mine_rows > 16 * half) {
                         const uint32_t lane0 = static_cast<uint32_t>(half) << 20;
                         uint32_t v[64];
@@ -687,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                 v[4 * i + 2 * h + 1] = __float_as_uint(f32x2_hi(y));
                             }
                         }
-                        if (__builtin_expect(tail, 0)) {
+                        if constexpr (kTail) {
                             const int ra = (warp & 3) * 32 + 16 * half + (lane >> 2);  // the thread's first row
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
@@ -756,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             }
                         }
                         tmem_st_pairs(t_s + lane0, pk);
-                        if (FP8 && __builtin_expect(tail, 0)) {
+                        if constexpr (FP8 && kTail) {
                             // What the rounding to BF16 leaves, for a second product: rows that see a few drafted keys
                             // would else carry the rounding of one key's scale in all their dims.
 #pragma unroll
@@ -785,6 +786,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         mo[h] = tm;
                         lo[h] = tl;
                     }
+                };
+                if ((t + 1) * kKeys > p0) {
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) half_rows(half, std::true_type());
+                } else {
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) half_rows(half, std::false_type());
                 }
                 tmem_wait_st();
                 tc_fence_before();
