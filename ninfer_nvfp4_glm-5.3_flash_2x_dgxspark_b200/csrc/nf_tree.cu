@@ -9,15 +9,17 @@
 // own 128 rows over the same tiles; a smaller one gives them every other tile.
 //
 // Per tile of 128 keys and 256 rows (D 128) the tensor cores need 2,048 cycles
-// and the exponentials 2,048; it takes 6,200.  What bounds it is the chain of a
-// stream: scores (512 cycles), softmax (2,000 alone, 3,000 to 4,000 beside the
-// other stream's and the E4M3 widening on the same schedulers), product with V
-// (512), and the barriers between them; a stream's scores and probabilities
+// and the exponentials 2,048; it takes 6,000.  What bounds it is the chain of a
+// stream: scores (512 cycles), softmax (about 3,000 beside the other stream's
+// and the E4M3 widening on the same schedulers), product with V (512), and the
+// barriers between them; a stream's scores and probabilities
 // share their 128 TMEM columns, as two streams with outputs of 128 columns
 // leave no room for a second set.  More and smaller tasks (64 keys, scores a
 // task ahead) took 20% longer, twice the softmax warps 8%.
-// 4 sequences of 64 nodes, 8 rows a node, on up to 65,000 E4M3 keys: 231 us,
-// 570 TFLOP/s; 24 of 16 nodes on 8,191 BF16 keys, where a tile of 128 rows
+// The softmax subtracts the maxima that the tiles before had: no weight gets
+// beyond 2^8 with them, or they rise (227 to 223 us).
+// 4 sequences of 64 nodes, 8 rows a node, on up to 65,000 E4M3 keys: 223 us,
+// 590 TFLOP/s; 24 of 16 nodes on 8,191 BF16 keys, where a tile of 128 rows
 // waits for its 64 KB more than for the products: 77 us, 4.0 TB/s.
 #include "nf_tree.cuh"
 
@@ -38,6 +40,11 @@ constexpr float kRescale = 8.f;  // the running max may lag the true one by 2^8
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -674,73 +681,110 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     if (mine_rows > 16 * half) {
                         const uint32_t lane0 = static_cast<uint32_t>(half) << 20;
                         uint32_t v[64];
-                        tmem_ld_frag(t_s + lane0, v);
-                        tmem_wait_ld();
-                        // x = S * factor
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint64_t f = FP8 ? *reinterpret_cast<const uint64_t*>(sc + 8 * i) : f32x2_pack(a.c, a.c);
+                        uint64_t nm[2];
+                        auto pick = [&](int i, int h) {
+                            return f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1]));
+                        };
+                        auto put = [&](int i, int h, uint64_t y) {
+                            v[4 * i + 2 * h] = __float_as_uint(f32x2_lo(y));
+                            v[4 * i + 2 * h + 1] = __float_as_uint(f32x2_hi(y));
+                        };
+                        auto factor = [&](int i) { return FP8 ? *reinterpret_cast<const uint64_t*>(sc + 8 * i) : f32x2_pack(a.c, a.c); };
+                        auto negate = [&]() {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint64_t y = mul_f32x2(
-                                    f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), f);
-                                v[4 * i + 2 * h] = __float_as_uint(f32x2_lo(y));
-                                v[4 * i + 2 * h + 1] = __float_as_uint(f32x2_hi(y));
+                                const float mu = m[h] == -INFINITY ? 0.f : m[h];
+                                nm[h] = f32x2_pack(-mu, -mu);
                             }
-                        }
-                        if constexpr (kTail) {
-                            const int ra = (warp & 3) * 32 + 16 * half + (lane >> 2);  // the thread's first row
+                        };
+                        // v = x - m with the maxima brought up to date, and the sums and outputs with them
+                        auto rise = [&]() {
+                            tmem_ld_frag(t_s + lane0, v);
+                            tmem_wait_ld();
+                            // x = S * factor
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const int nd = (w.row0 + row0 + ra + 8 * h) / a.G;
+                            for (int i = 0; i < 16; ++i) {
+                                const uint64_t f = factor(i);
 #pragma unroll
-                                for (int c = 0; c < 4; ++c) {
-                                    const uint32_t vis = visible(a, w.first + nd, nd, n, t * kKeys + 32 * c - p0, ra + 8 * h < rows) >>
-                                                         (2 * (lane & 3));
+                                for (int h = 0; h < 2; ++h) put(i, h, mul_f32x2(pick(i, h), f));
+                            }
+                            if constexpr (kTail) {
+                                const int ra = (warp & 3) * 32 + 16 * half + (lane >> 2);  // the thread's first row
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i)
+                                for (int h = 0; h < 2; ++h) {
+                                    const int nd = (w.row0 + row0 + ra + 8 * h) / a.G;
 #pragma unroll
-                                        for (int e = 0; e < 2; ++e)
-                                            if (!((vis >> (8 * i + e)) & 1u)) v[16 * c + 4 * i + 2 * h + e] = 0xff800000u;
+                                    for (int c = 0; c < 4; ++c) {
+                                        const uint32_t vis = visible(a, w.first + nd, nd, n, t * kKeys + 32 * c - p0, ra + 8 * h < rows) >>
+                                                             (2 * (lane & 3));
+#pragma unroll
+                                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                            for (int e = 0; e < 2; ++e)
+                                                if (!((vis >> (8 * i + e)) & 1u)) v[16 * c + 4 * i + 2 * h + e] = 0xff800000u;
+                                    }
                                 }
                             }
-                        }
-                        float mn[2], f[2];
-                        bool grow = done == 0;
+                            float mn[2], f[2];
+                            bool grow = done == 0;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float mx[2] = {__uint_as_float(v[2 * h]), __uint_as_float(v[4 + 2 * h])};
+                            for (int h = 0; h < 2; ++h) {
+                                float mx[2] = {__uint_as_float(v[2 * h]), __uint_as_float(v[4 + 2 * h])};
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                    mx[i & 1] = max3(mx[i & 1], __uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1]));
+                                float x = fmaxf(mx[0], mx[1]);
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                                mn[h] = fmaxf(m[h], x);
+                                grow |= x > m[h] + kRescale;
+                            }
+                            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    f[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn[h]);
+                                    m[h] = mn[h];
+                                    l[h] *= f[h];
+                                }
+                                // the products up to the previous task are complete: the scores' commit covers them
+                                if (done > 0)
+#pragma unroll 1
+                                    for (int c = 0; c < D; c += 16) {
+                                        uint32_t o[8];
+                                        tmem_ld_frag16(t_o + lane0 + c, o);
+                                        tmem_wait_ld();
+#pragma unroll
+                                        for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f[(k >> 1) & 1]);
+                                        tmem_st_frag16(t_o + lane0 + c, o);
+                                    }
+                            }
+                            negate();
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
-                                mx[i & 1] = max3(mx[i & 1], __uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1]));
-                            float x = fmaxf(mx[0], mx[1]);
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                            mn[h] = fmaxf(m[h], x);
-                            grow |= x > m[h] + kRescale;
-                        }
-                        if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                f[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn[h]);
-                                m[h] = mn[h];
-                                l[h] *= f[h];
-                            }
-                            // the products up to the previous task are complete: the scores' commit covers them
-                            if (done > 0)
-#pragma unroll 1
-                                for (int c = 0; c < D; c += 16) {
-                                    uint32_t o[8];
-                                    tmem_ld_frag16(t_o + lane0 + c, o);
-                                    tmem_wait_ld();
+                                for (int h = 0; h < 2; ++h) put(i, h, add_f32x2(pick(i, h), nm[h]));
+                        };
+                        if constexpr (kTail) {
+                            rise();
+                        } else {
+                            // the maxima of the tiles before, as long as no weight gets beyond 2^kRescale with them
+                            negate();
+                            tmem_ld_frag(t_s + lane0, v);
+                            tmem_wait_ld();
+                            float top[2] = {m[0] == -INFINITY || m[1] == -INFINITY ? INFINITY : -INFINITY, -INFINITY};
 #pragma unroll
-                                    for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f[(k >> 1) & 1]);
-                                    tmem_st_frag16(t_o + lane0 + c, o);
+                            for (int i = 0; i < 16; ++i) {
+                                const uint64_t f = factor(i);
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint64_t y = fma_f32x2(pick(i, h), f, nm[h]);
+                                    put(i, h, y);
+                                    top[h] = max3(top[h], f32x2_lo(y), f32x2_hi(y));
                                 }
+                            }
+                            if (__builtin_expect(__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > kRescale), 0)) rise();
                         }
                         uint32_t pk[32];
-                        const float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
-                        const uint64_t nm[2] = {f32x2_pack(-mu0, -mu0), f32x2_pack(-mu1, -mu1)};
                         uint64_t sum[2] = {0, 0};
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
@@ -748,8 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             if (FP8) g = *reinterpret_cast<const uint64_t*>(sc + kKeys + 8 * i);
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint64_t y = add_f32x2(
-                                    f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), nm[h]);
+                                const uint64_t y = pick(i, h);
                                 uint64_t pr = f32x2_pack(ex2(f32x2_lo(y)), ex2(f32x2_hi(y)));
                                 sum[h] = add_f32x2(sum[h], pr);
                                 if (FP8) pr = mul_f32x2(pr, g);
@@ -765,8 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                 const uint64_t g = *reinterpret_cast<const uint64_t*>(sc + kKeys + 8 * i);
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) {
-                                    const uint64_t y = add_f32x2(
-                                        f32x2_pack(__uint_as_float(v[4 * i + 2 * h]), __uint_as_float(v[4 * i + 2 * h + 1])), nm[h]);
+                                    const uint64_t y = pick(i, h);
                                     const uint64_t pr = mul_f32x2(f32x2_pack(ex2(f32x2_lo(y)), ex2(f32x2_hi(y))), g);
                                     const uint32_t hi = pk[2 * i + h];
                                     const float a0 = __uint_as_float(hi << 16), a1 = __uint_as_float(hi & 0xffff0000u);

@@ -428,6 +428,36 @@ def test_attention_repeats_bit_for_bit():
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 20, 48])
+@pytest.mark.parametrize("course", ["rising", "falling", "late", "flat"])
+def test_attention_courses_of_the_maximum(kind, rows, course):
+    """Scores that rise or fall along the keys by hundreds, so that the running maximum moves in every tile or never."""
+    nq, nkv, dim, prefix = 8, 1, 128, 1000
+    rng = np.random.default_rng(rows)
+    c, k, v = make_cache(rng, kind, 1, nkv, prefix + rows, dim)
+    at = np.arange(prefix + rows) / (prefix + rows)
+    gain = {"rising": at, "falling": 1 - at, "late": (at > 0.9) * 1.0, "flat": 0 * at}[course]
+    u = np.sign(rng.standard_normal(dim))
+    # every key: a multiple of u (exact in both types) instead of its random row
+    want = np.round(gain * 16) / 16
+    if kind == "bf16":
+        c.tensors[0][0, 0] = torch.from_numpy(want[:, None] * u).bfloat16().cuda()
+    else:
+        c.tensors[0][0, 0] = torch.from_numpy(want[:, None] * u).float().cuda().to(torch.float8_e4m3fn)
+        c.tensors[2].fill_(1.0)
+    k = c.tensors[0][0, 0].float().double().cpu().numpy()
+    q = torch.from_numpy(np.tile(2.5 * u, (rows, nq, 1)) + 0.1 * rng.standard_normal((rows, nq, dim))).bfloat16()
+    out = torch.empty(rows, nq, dim, dtype=torch.bfloat16, device="cuda")
+    work = torch.empty(m.tree_attention_workspace(dim), dtype=torch.uint8, device="cuda")
+    m.tree_attention(c, q.cuda(), ints([0, rows]), ints([prefix]), out, work, scale=1.0)
+    got = out.double().cpu().numpy()
+    for r in (0, rows // 2, rows - 1):
+        w, tol = exact_attention(q[r].double().numpy(), k, v[0, 0], np.arange(prefix + rows) <= prefix + r, 1.0)
+        err = np.abs(got[r] - w)
+        assert np.all(err <= tol), (r, float(err.max()), float(tol.flat[err.argmax()]))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("batch, nodes", [(32, 1), (24, 2), (12, 16)])
 def test_attention_from_cold_memory(kind, batch, nodes):
     """Long caches that the L2 does not hold, whose loads land in any order."""
