@@ -151,8 +151,10 @@ __device__ __forceinline__ int rank_of(uint64_t v, const uint64_t* s, int n) {
 // threads' maxima bounds them from below, and only the logits of the threads
 // whose maximum reaches it (`top` of 256, but for equals) can be among them;
 // the CTA looks at these once more.
-// The floor is one read of the logits; what bounds a call of many rows is the
-// instructions issued (nine for two logits), one of a few rows its latency.
+// The floor is one read of the logits; what bounds it is the loads' latency and
+// the top tokens behind them where all rows' CTAs run at the same time, the
+// instructions issued (nine for two logits) with more rows, and a row's own
+// latency with few.
 // 256 rows of 151,552 F32 logits, top 5: 34.9 us, 4.45 TB/s; 4,001 rows of
 // 32,003 BF16 logits: 63.5 us, 4.0 TB/s.  The CTAs an SM holds matter: F32 with
 // 76 registers, so three, 48.2 us; BF16 with four 71.6, with five 66.4.
