@@ -493,6 +493,38 @@ def test_attention_from_cold_memory(kind, batch, nodes):
                 assert np.all(err <= tol), (i, r, h, float(err.max()))
 
 
+@pytest.mark.parametrize("nodes", [1, 24])
+def test_attention_from_two_threads_on_two_streams(nodes):
+    """Calls in flight at the same time, with a workspace each."""
+    import threading
+    rng = np.random.default_rng(nodes)
+    c, _, _ = make_cache(rng, "e4m3", 6, 2, 900, 128)
+    q = [torch.from_numpy(rng.standard_normal((6 * nodes, 16, 128)).astype(np.float32)).bfloat16().cuda() for _ in range(2)]
+    start, prefix = ints(range(0, 6 * nodes + 1, nodes)), ints([876, 3, 500, 0, 129, 800])
+    want = [torch.empty_like(x) for x in q]
+    for x, o in zip(q, want):
+        m.tree_attention(c, x, start, prefix, o, torch.empty(m.tree_attention_workspace(128), dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        w = torch.empty(m.tree_attention_workspace(128), dtype=torch.uint8, device="cuda")
+        o = [torch.empty_like(q[i]) for _ in range(20)]
+        torch.cuda.synchronize()
+        for x in o:
+            m.tree_attention(c, q[i], start, prefix, x, w, stream=s.cuda_stream)
+        s.synchronize()
+        bad.extend(1 for x in o if not torch.equal(x, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_attention_refuses_tensors():
     rng = np.random.default_rng(1)
     c, _, _ = make_cache(rng, "bf16", 2, 2, 8, 64)
