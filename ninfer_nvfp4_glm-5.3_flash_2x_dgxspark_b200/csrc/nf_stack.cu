@@ -91,7 +91,8 @@ struct nf_stack {
     AttnPart* part_ml = nullptr;   // attention split partials
     float* part_acc = nullptr;
     int* counters = nullptr;       // GEMM tile counters [2 * layers]
-    int* err = nullptr;
+    int* err = nullptr;            // [2]; the projections give up once the first is set
+    int* bad = nullptr;            // err + 1: an index outside, of a row that the step leaves out by itself
     CUtensorMap tm_a{}, tm_a_s{}, tm_att{}, tm_att_s{};
     // several rows of a sequence at a time, and E4M3 caches
     int kv_kind = NF_KV_BF16;
@@ -283,8 +284,9 @@ int nf_stack_create_kv(const nf_stack_desc* desc, int kv_kind, int device, nf_st
          s->alloc(&s->att16, B * NQ) && s->alloc(&s->o_part, kMaxSlices * B * H) &&
          s->alloc(&s->part_ml, B * d.q_heads * max_splits) &&
          s->alloc(&s->part_acc, B * d.q_heads * max_splits * kHeadDim) &&
-         s->alloc(&s->counters, 2 * static_cast<size_t>(d.layers)) && s->alloc(&s->err, 1) &&
-         cudaMemset(s->err, 0, 4) == cudaSuccess;
+         s->alloc(&s->counters, 2 * static_cast<size_t>(d.layers)) && s->alloc(&s->err, 2) &&
+         cudaMemset(s->err, 0, 8) == cudaSuccess;
+    s->bad = s->err + 1;
     uint8_t* work = nullptr;
     ok = ok && s->alloc(&s->row_seq, B) && s->alloc(&s->row_slot, B) && s->alloc(&s->row_pos, B) && s->alloc(&s->iota, B + 1) &&
          s->alloc(&work, static_cast<size_t>(nf_tree_attention_workspace(kHeadDim))) &&
@@ -524,7 +526,9 @@ static int stack_step(nf_stack* s, const int32_t* tokens, const int32_t* positio
     int prev = 0;
     cudaGetDevice(&prev);
     cudaSetDevice(s->device);
-    cudaError_t e = launch_embed(s->embed, d.vocab, H, tokens, T, s->x, s->err, st);
+    // A row or sequence of a tree step that is refused becomes NaN, and the others go on: its indices must not stop the
+    // projections.
+    cudaError_t e = launch_embed(s->embed, d.vocab, H, tokens, T, s->x, tree ? s->bad : s->err, st);
     int status = NF_OK;
     const float eps = d.norm_eps;
     const int splits = attn_splits(T, nkv, L, s->sms);
@@ -540,11 +544,11 @@ static int stack_step(nf_stack* s, const int32_t* tokens, const int32_t* positio
             uint16_t* q16 = reinterpret_cast<uint16_t*>(s->q);
             if (e == cudaSuccess)
                 e = launch_kv_write(cache, s->rope, s->qkv_part, NF_DTYPE_F32, NQKV, T, nq, Ly.q_norm, Ly.k_norm, 1e-5f, tree->pos,
-                                    tree->seq, tree->slot, q16, s->err, st, S1, static_cast<int64_t>(T) * NQKV);
+                                    tree->seq, tree->slot, q16, s->bad, st, S1, static_cast<int64_t>(T) * NQKV);
             if (e == cudaSuccess)
                 e = launch_tree_attention(cache, q16, T, nq, tree->row_start, tree->batch, tree->prefix, nullptr, tree->mask,
                                           tree->mask_words, 1.f / sqrtf(static_cast<float>(kHeadDim)), s->att16, s->tree_work,
-                                          s->err, st);
+                                          s->bad, st);
         } else {
             if (e == cudaSuccess)
                 e = launch_qk_norm_rope(s->qkv_part, S1, static_cast<int64_t>(T) * NQKV, T, nq, nkv, Ly.q_norm, Ly.k_norm,
@@ -638,7 +642,7 @@ int nf_stack_accept(nf_stack* s, const int32_t* prefix, const int32_t* path, int
     int prev = 0;
     cudaGetDevice(&prev);
     cudaSetDevice(s->device);
-    const cudaError_t e = launch_kv_accept(caches.data(), s->d.layers, prefix, path, max_path, path_len, nullptr, batch, s->err,
+    const cudaError_t e = launch_kv_accept(caches.data(), s->d.layers, prefix, path, max_path, path_len, nullptr, batch, s->bad,
                                            static_cast<cudaStream_t>(stream));
     cudaSetDevice(prev);
     if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "accept launch: %s", cudaGetErrorString(e));
@@ -651,9 +655,10 @@ int nf_stack_sync(nf_stack* s, void* stream) {
     cudaGetDevice(&prev);
     cudaSetDevice(s->device);
     cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
-    int derr = 0;
-    if (e == cudaSuccess) e = cudaMemcpy(&derr, s->err, 4, cudaMemcpyDeviceToHost);
-    if (e == cudaSuccess && derr != 0) cudaMemset(s->err, 0, 4);
+    int both[2] = {0, 0};
+    if (e == cudaSuccess) e = cudaMemcpy(both, s->err, 8, cudaMemcpyDeviceToHost);
+    const int derr = both[0] != 0 ? both[0] : both[1];
+    if (e == cudaSuccess && derr != 0) cudaMemset(s->err, 0, 8);
     cudaSetDevice(prev);
     if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "synchronise: %s", cudaGetErrorString(e));
     if (derr == NF_DEVERR_BAD_TOKEN)
