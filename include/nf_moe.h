@@ -652,9 +652,11 @@ NF_API int nf_stack_kv(nf_stack* stack, int layer, nf_kv_cache* out);
  * logits.  Rows behind row_start_dev[batch] write nothing to the caches; their
  * outputs mean nothing.  The caches' positions from prefix on hold the rows of
  * the step until the next one writes there: nf_stack_accept keeps a path.
- * A row whose token lies outside the vocabulary becomes NaN, a sequence that
- * nf_tree_attention refuses likewise; nf_stack_sync reports them, and the other
- * sequences' results stand (so too in nf_stack_decode over E4M3 caches). */
+ * A row whose token lies outside the vocabulary becomes NaN; a sequence that
+ * nf_tree_attention refuses, or with a position below 0 or from 2^31 on,
+ * becomes NaN as a whole and writes nothing.  nf_stack_sync reports both, and
+ * the other sequences' results stand (so too in nf_stack_decode over E4M3
+ * caches). */
 NF_API int nf_stack_verify(nf_stack* stack, const int32_t* tokens_dev, const int32_t* depth_dev,
                            const int32_t* row_start_dev, const int32_t* prefix_dev, const uint64_t* mask_dev,
                            int mask_words, int rows, int batch, int32_t* next_dev, float* final_dev, void* stream);

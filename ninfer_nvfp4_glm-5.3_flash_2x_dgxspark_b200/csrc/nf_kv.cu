@@ -338,25 +338,35 @@ __global__ void __launch_bounds__(256) kv_quantize_kernel(const uint16_t* __rest
     if (lane == 0) scale[r] = s;
 }
 
-__global__ void __launch_bounds__(128) kv_places_kernel(int rows, const int32_t* __restrict__ row_start, int batch,
+// The same view of a batch as the attention's: row_start is clamped to
+// [0, rows], and a sequence is refused as a whole, so that none of its rows is
+// written when one of them, or its position, lies outside.
+__global__ void __launch_bounds__(128) kv_places_kernel(int rows, int L, const int32_t* __restrict__ row_start, int batch,
                                                         const int32_t* __restrict__ prefix,
                                                         const int32_t* __restrict__ depth, int32_t* __restrict__ seq,
                                                         int32_t* __restrict__ slot, int32_t* __restrict__ pos) {
     const int r = blockIdx.x * blockDim.x + threadIdx.x;
     if (r >= rows) return;
+    auto start = [&](int i) { return min(max(row_start[i], 0), rows); };
     int lo = 0, hi = batch;  // the last sequence that starts at or before r
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (row_start[mid] <= r) lo = mid;
+        if (start(mid) <= r) lo = mid;
         else hi = mid;
     }
-    const int j = r - row_start[lo];
-    const bool in = j >= 0 && r < row_start[lo + 1];
-    // a place outside the cache is left to the write to refuse
-    const int64_t at = static_cast<int64_t>(prefix[lo]) + j, p = static_cast<int64_t>(prefix[lo]) + (depth ? depth[r] : j);
+    const int first = start(lo), n = start(lo + 1) - first, j = r - first, p0 = prefix[lo];
+    const bool in = j >= 0 && j < n;
+    bool bad = p0 < 0 || p0 > L - n;
+    if (in && depth)
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const int64_t p = static_cast<int64_t>(p0) + depth[first + k];
+            bad |= p < 0 || p > 0x7fffffff;
+        }
+    // the write refuses these places
     seq[r] = lo;
-    slot[r] = !in ? -1 : at < 0 || at > 0x7fffffff ? 0x7fffffff : static_cast<int32_t>(at);
-    pos[r] = !in ? 0 : p < 0 || p > 0x7fffffff ? -1 : static_cast<int32_t>(p);
+    slot[r] = !in ? -1 : bad ? 0x7fffffff : p0 + j;
+    pos[r] = !in ? 0 : bad ? -1 : p0 + (depth ? depth[r] : j);
 }
 
 // ---------------------------------------------------------------------------
@@ -467,10 +477,10 @@ cudaError_t launch_kv_quantize(const uint16_t* x, int64_t n, int head_dim, uint8
     return cudaGetLastError();
 }
 
-cudaError_t launch_kv_places(int rows, const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* depth,
+cudaError_t launch_kv_places(int rows, int max_context, const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* depth,
                              int32_t* seq, int32_t* slot, int32_t* pos, cudaStream_t st) {
     if (rows <= 0) return cudaSuccess;
-    kv_places_kernel<<<(rows + 127) / 128, 128, 0, st>>>(rows, row_start, batch, prefix, depth, seq, slot, pos);
+    kv_places_kernel<<<(rows + 127) / 128, 128, 0, st>>>(rows, max_context, row_start, batch, prefix, depth, seq, slot, pos);
     return cudaGetLastError();
 }
 

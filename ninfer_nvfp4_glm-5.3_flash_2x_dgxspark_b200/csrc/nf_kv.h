@@ -26,8 +26,9 @@ cudaError_t launch_kv_write(const nf_kv_cache& c, const nf_rope& rope, const voi
 cudaError_t launch_kv_quantize(const uint16_t* x, int64_t n, int head_dim, uint8_t* codes, float* scale, cudaStream_t st);
 // The rows of a batch of sequences: their sequence, cache slot (prefix + row
 // of the sequence) and rotary position (prefix + depth); rows behind the last
-// sequence get slot -1.
-cudaError_t launch_kv_places(int rows, const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* depth,
+// sequence get slot -1, those of a sequence that does not fit places that
+// launch_kv_write refuses.
+cudaError_t launch_kv_places(int rows, int max_context, const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* depth,
                              int32_t* seq, int32_t* slot, int32_t* pos, cudaStream_t st);
 cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int rows, int q_heads,
                                   const int32_t* row_start, int batch, const int32_t* prefix, const int32_t* cache_seq,

@@ -611,7 +611,7 @@ int nf_stack_verify(nf_stack* s, const int32_t* tokens, const int32_t* depth, co
     int prev = 0;
     cudaGetDevice(&prev);
     cudaSetDevice(s->device);
-    const cudaError_t e = launch_kv_places(rows, row_start, batch, prefix, depth, s->row_seq, s->row_slot, s->row_pos,
+    const cudaError_t e = launch_kv_places(rows, s->d.max_context, row_start, batch, prefix, depth, s->row_seq, s->row_slot, s->row_pos,
                                            static_cast<cudaStream_t>(stream));
     cudaSetDevice(prev);
     if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "verify launch: %s", cudaGetErrorString(e));

@@ -17,6 +17,35 @@ m, wl = nfm(), workload()
 H, V, L = CFG["hidden"], CFG["vocab"], 64
 
 
+class DeviceBytes:
+    """A span of device memory, for torch.as_tensor."""
+
+    def __init__(self, ptr, n):
+        self.__cuda_array_interface__ = dict(shape=(n,), typestr="|u1", data=(ptr, False), version=3)
+
+
+def caches(st):
+    """Copies of every layer's caches (codes and scales) as bytes."""
+    out = []
+    for layer in range(CFG["layers"]):
+        d = st.kv_desc(layer)
+        rows = d.seqs * d.kv_heads * d.max_context
+        for ptr, n in ((d.k, rows * d.head_dim * (1 if d.kind == m.KV_E4M3 else 2)),
+                       (d.v, rows * d.head_dim * (1 if d.kind == m.KV_E4M3 else 2)), (d.k_scale, 4 * rows), (d.v_scale, 4 * rows)):
+            if ptr:
+                out.append(torch.as_tensor(DeviceBytes(ptr, n), device="cuda").clone())
+    return out
+
+
+def changed(st, before):
+    """Which (sequence, position) pairs of any layer's caches differ from their copies."""
+    d = st.kv_desc(0)
+    out = torch.zeros(d.seqs, d.max_context, dtype=torch.bool, device="cuda")
+    for a, b in zip(before, caches(st)):
+        out |= (a != b).view(d.seqs, d.kv_heads, d.max_context, -1).any(-1).any(1)
+    return {(i, p) for i, p in out.nonzero().tolist()}
+
+
 def step(st, tokens, start, prefix, depth=None, rows=None, sync=True):
     rows = len(tokens) if rows is None else rows
     fin = torch.full((rows, H), 3.0, dtype=torch.float32, device="cuda")
@@ -84,4 +113,44 @@ def test_a_step_behind_a_refused_path(model, kv):  # noqa: F811
     with pytest.raises(m.NfError, match="outside the cache"):
         st.sync()
     close(got, fin, "behind a refused path")
+    st.close()
+
+
+@pytest.mark.parametrize("kv", ["e4m3", "bf16"])
+@pytest.mark.parametrize("prefix, depth", [
+    (-1, None), (-2, None), (-(2 ** 31), None), (L - 1, None), (L - 2, None), (L, None), (2 ** 31 - 1, None),
+    (5, [0, -6, 1]), (5, [0, 1, 2 ** 31 - 1])])
+def test_a_refused_sequence_writes_nothing(model, kv, prefix, depth):  # noqa: F811
+    """A sequence of three rows whose prefix, rows or positions lie outside changes no cache, becomes NaN and is reported;
+    the sequences beside it get what they get beside a sequence that fits."""
+    tokens = np.random.default_rng(1).integers(0, V, 7)
+    start = [0, 2, 5, 7]
+    st = make_stack(model, 8, L, kv)
+    st.fill_kv(3)
+    fin, _ = step(st, tokens, start, [10, 5, 20], depth=None if depth is None else [0, 1, 0, 1, 2, 0, 1])
+    st.fill_kv(3)
+    before = caches(st)
+    got, _ = step(st, tokens, start, [10, prefix, 20], depth=None if depth is None else [0, 1] + depth + [0, 1], sync=False)
+    with pytest.raises(m.NfError, match="outside the cache"):
+        st.sync()
+    assert changed(st, before) == {(0, 10), (0, 11), (2, 20), (2, 21)}
+    assert got[2:5].isnan().all()
+    close(got[:2], fin[:2], "the sequence before")
+    close(got[5:], fin[5:], "the sequence behind")
+    st.close()
+
+
+@pytest.mark.parametrize("kv", ["e4m3", "bf16"])
+@pytest.mark.parametrize("start", [[-3, 3, 5], [-(2 ** 31), 3, 5], [0, 3, 99], [-1, 3, 2 ** 31 - 1]])
+def test_row_starts_outside_are_clamped(model, kv, start):  # noqa: F811
+    """Row starts below 0 and behind the rows count as 0 and as the number of rows, in the caches as in the attention."""
+    tokens = np.random.default_rng(2).integers(0, V, 5)
+    st = make_stack(model, 8, L, kv)
+    st.fill_kv(4)
+    fin, _ = step(st, tokens, [0, 3, 5], [10, 20])
+    st.fill_kv(4)
+    before = caches(st)
+    got, _ = step(st, tokens, start, [10, 20])
+    assert changed(st, before) == {(0, 10), (0, 11), (0, 12), (1, 20), (1, 21)}
+    close(got, fin, "clamped")
     st.close()
