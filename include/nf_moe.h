@@ -660,7 +660,9 @@ NF_API int nf_stack_kv(nf_stack* stack, int layer, nf_kv_cache* out);
 NF_API int nf_stack_verify(nf_stack* stack, const int32_t* tokens_dev, const int32_t* depth_dev,
                            const int32_t* row_start_dev, const int32_t* prefix_dev, const uint64_t* mask_dev,
                            int mask_words, int rows, int batch, int32_t* next_dev, float* final_dev, void* stream);
-/* nf_token_logprobs of the last step's logits (a step of at least `rows` rows). */
+/* nf_token_logprobs of the last step's logits (a step of at least `rows` rows;
+ * the host cannot tell which of the captured steps ran last, so it refuses only
+ * more rows than both the last step enqueued and the largest captured one). */
 NF_API int nf_stack_logprobs(nf_stack* stack, int rows, const int32_t* target_dev, int top, float* logprob_dev,
                              float* entropy_dev, int32_t* top_idx_dev, float* top_logprob_dev, void* stream);
 /* nf_kv_accept over every layer's caches (sequence i is cache sequence i). */

@@ -102,6 +102,7 @@ struct nf_stack {
     int32_t* iota = nullptr;       // [B + 1] 0, 1, 2, ...
     void* tree_work = nullptr;
     int last_rows = 0;             // rows of the last step enqueued
+    int captured_rows = 0;         // the most rows of a captured step: any of them may have been replayed since
 
     nf_kv_cache cache(int layer) const {
         const StackLayer& l = layers[static_cast<size_t>(layer)];
@@ -578,7 +579,10 @@ static int stack_step(nf_stack* s, const int32_t* tokens, const int32_t* positio
     int tst = nf_tp_linear_bf16(s->head, s->lm_head, d.vocab, H, final_dev ? final_dev : s->fin, T, nullptr, stream);
     if (tst == NF_OK && next) tst = nf_tp_argmax(s->head, T, d.vocab, next, stream);
     if (tst != NF_OK) return s->fail(tst, "lm_head: %s", nf_tp_last_error(s->head));
-    s->last_rows = T;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();
+    if (capture == cudaStreamCaptureStatusActive) s->captured_rows = std::max(s->captured_rows, T);
+    else s->last_rows = T;
     return NF_OK;
 }
 
@@ -623,7 +627,8 @@ int nf_stack_logprobs(nf_stack* s, int rows, const int32_t* target, int top, flo
                       int32_t* top_idx, float* top_lp, void* stream) {
     if (!s) return NF_ERR_INVALID;
     s->msg.clear();
-    if (rows > s->last_rows) return s->fail(NF_ERR_STATE, "the last step had %d rows", s->last_rows);
+    const int had = std::max(s->last_rows, s->captured_rows);
+    if (rows > had) return s->fail(NF_ERR_STATE, "the last step had %d rows", had);
     const int st = nf_tp_logprobs(s->head, rows, s->d.vocab, target, top, logprob, entropy, top_idx, top_lp, stream);
     if (st != NF_OK) return s->fail(st, "lm_head: %s", nf_tp_last_error(s->head));
     return NF_OK;

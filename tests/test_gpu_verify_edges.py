@@ -154,3 +154,39 @@ def test_row_starts_outside_are_clamped(model, kv, start):  # noqa: F811
     assert changed(st, before) == {(0, 10), (0, 11), (0, 12), (1, 20), (1, 21)}
     close(got, fin, "clamped")
     st.close()
+
+
+def test_logprobs_of_replayed_steps(model):  # noqa: F811
+    """Log-probabilities of a replayed step, whichever step was enqueued or captured since."""
+    tokens = np.random.default_rng(5).integers(0, V, 6)
+    st = make_stack(model, 8, L, "e4m3")
+    args = [(ints(tokens[:n]), ints([0, n]), ints([10]), n, torch.empty(n, dtype=torch.int32, device="cuda"),
+             torch.empty(n, H, device="cuda")) for n in (6, 2)]
+
+    def logprobs():
+        lp = torch.zeros(6, device="cuda")
+        st.logprobs(6, ints([7] * 6), lp)
+        st.sync()
+        return lp
+
+    def fresh():
+        st.fill_kv(3)
+        st.verify(*args[0])
+
+    fresh()
+    want = logprobs()
+    s, graphs = torch.cuda.Stream(), []
+    fresh()  # an eager step of 6 rows, then captures that do not run
+    st.sync()
+    for a in args:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            st.verify(*a, stream=torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(logprobs(), want)
+    for i in (1, 0):  # the larger step is replayed last
+        st.fill_kv(3)
+        graphs[i].replay()
+    assert torch.equal(logprobs(), want)
+    with pytest.raises(m.NfError, match="rows"):
+        st.logprobs(7, ints([7] * 7), torch.zeros(7, device="cuda"))
+    st.close()
