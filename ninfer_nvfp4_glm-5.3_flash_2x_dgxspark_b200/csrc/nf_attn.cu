@@ -45,11 +45,16 @@ __device__ __forceinline__ float warp_sum(float v) {
 // Embedding rows (embed_row, src/text_forward.cpp:753-757): x[t] = embed[tok[t]]
 // widened to F32.  A token outside the vocabulary (the reference fails with
 // "prompt token is outside the vocabulary", :626) records an error and
-// writes a NaN row.
+// writes a NaN row.  A row whose cache slot is -1 (padding; slot may be NULL)
+// has no token and becomes zeros.
 // ---------------------------------------------------------------------------
 __global__ void embed_kernel(const uint16_t* __restrict__ table, int64_t vocab, int H, const int32_t* __restrict__ tok,
-                             float* __restrict__ x, int* __restrict__ err) {
+                             const int32_t* __restrict__ slot, float* __restrict__ x, int* __restrict__ err) {
     const int t = blockIdx.x;
+    if (slot && slot[t] == -1) {
+        for (int i = threadIdx.x; i < H; i += blockDim.x) x[static_cast<int64_t>(t) * H + i] = 0.f;
+        return;
+    }
     const int32_t id = tok[t];
     const bool ok = id >= 0 && id < vocab;
     if (!ok && threadIdx.x == 0) atomicCAS(err, 0, NF_DEVERR_BAD_TOKEN);
@@ -449,9 +454,9 @@ cudaError_t launch_fill_bf16_hash(uint16_t* p, int64_t n, uint64_t seed, cudaStr
 }
 
 cudaError_t launch_embed(const uint16_t* table, int64_t vocab, int H, const int32_t* tok, int T, float* x, int* err,
-                         cudaStream_t st) {
+                         cudaStream_t st, const int32_t* slot) {
     if (T <= 0) return cudaSuccess;
-    embed_kernel<<<T, 256, 0, st>>>(table, vocab, H, tok, x, err);
+    embed_kernel<<<T, 256, 0, st>>>(table, vocab, H, tok, slot, x, err);
     return cudaGetLastError();
 }
 

@@ -305,7 +305,7 @@ struct AttnPart {
 };
 constexpr int kAttnMaxSplitsHost = 64;  // splits of the context per (sequence, head)
 cudaError_t launch_embed(const uint16_t* table, int64_t vocab, int H, const int32_t* tok, int T, float* x, int* err,
-                         cudaStream_t st);
+                         cudaStream_t st, const int32_t* slot = nullptr);
 // RMSNorm per row; h = a (+ the sum of b's slices), h_out optional; stash:
 // the rmsnorm_stash form.
 cudaError_t launch_rmsnorm(const float* a, const float* b, int b_slices, int64_t b_stride, float* h_out, const float* w,

@@ -529,7 +529,7 @@ static int stack_step(nf_stack* s, const int32_t* tokens, const int32_t* positio
     cudaSetDevice(s->device);
     // A row or sequence of a tree step that is refused becomes NaN, and the others go on: its indices must not stop the
     // projections.
-    cudaError_t e = launch_embed(s->embed, d.vocab, H, tokens, T, s->x, tree ? s->bad : s->err, st);
+    cudaError_t e = launch_embed(s->embed, d.vocab, H, tokens, T, s->x, tree ? s->bad : s->err, st, tree ? tree->slot : nullptr);
     int status = NF_OK;
     const float eps = d.norm_eps;
     const int splits = attn_splits(T, nkv, L, s->sms);

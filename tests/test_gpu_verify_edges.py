@@ -190,3 +190,20 @@ def test_logprobs_of_replayed_steps(model):  # noqa: F811
     with pytest.raises(m.NfError, match="rows"):
         st.logprobs(7, ints([7] * 7), torch.zeros(7, device="cuda"))
     st.close()
+
+
+@pytest.mark.parametrize("kv", ["e4m3", "bf16"])
+def test_padded_rows_need_no_token(model, kv):  # noqa: F811
+    """Rows behind the last sequence (and in front of the first) may hold any token: nothing is reported, nothing written,
+    and the others' results stand."""
+    tokens = np.random.default_rng(6).integers(0, V, 3)
+    st = make_stack(model, 8, L, kv)
+    st.fill_kv(3)
+    fin, _ = step(st, tokens, [0, 1, 3], [10, 20])
+    for before, behind in ((0, 3), (2, 0), (1, 2)):
+        st.fill_kv(3)
+        old = caches(st)
+        got, _ = step(st, [-1] * before + list(tokens) + [V, -1, 2 ** 31 - 1][:behind], [before, before + 1, before + 3], [10, 20])
+        assert changed(st, old) == {(0, 10), (1, 20), (1, 21)}
+        close(got[before:before + 3], fin, "beside padding")
+    st.close()
