@@ -254,7 +254,29 @@ struct Walk {
     }
 };
 
-// Finds the CTA's share (every thread sums the weights of a run of sequences) and fills the rows of bad sequences with NaN.  A share
+// NaN into `rows` rows of the output from `first` on, 8 values a store; thread `me` of `threads` that share them.
+__device__ __forceinline__ void fill_nan(const TreeArgs& a, int first, int rows, int D, int64_t me, int64_t threads) {
+    const int64_t per_row = static_cast<int64_t>(a.nq) * D;
+    uint4* dst = reinterpret_cast<uint4*>(a.out + first * per_row);
+    const int64_t n = rows * per_row / 8;
+#pragma unroll 1
+    for (int64_t e = me; e < n; e += threads) dst[e] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+}
+// The rows of bad sequences become NaN: all CTAs share every such sequence's rows (4,096 rows of 32 heads of 128: 22 us;
+// by one thread 384 ms).  Not inlined, as it is rare: the roles that follow share the instruction cache.
+template <typename W>
+__device__ __noinline__ void fill_bad(const TreeArgs& a, int D) {
+    W w;
+#pragma unroll 1
+    for (w.i = 0; w.i < a.batch; ++w.i) {
+        w.load(a);
+        if (w.n > 0 && w.bad(a))
+            fill_nan(a, w.first, w.n, D, static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x,
+                     static_cast<int64_t>(gridDim.x) * blockDim.x);
+    }
+}
+
+// Finds the CTA's share (every thread sums the weights of a run of sequences), and fills the rows of bad sequences.  A share
 // is not smaller than LEAST tiles, those that a CTA takes at a time: smaller
 // ones would only make more parts to join, and no share inside an item may be
 // without a tile.  Ends with a __syncthreads.
@@ -265,16 +287,13 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
     const int run = (a.batch + THREADS - 1) / THREADS;
     const int i0 = min(a.batch, static_cast<int>(threadIdx.x) * run), i1 = min(a.batch, i0 + run);
     int64_t mine = 0;
+    bool any_bad = false;
 #pragma unroll 1
     for (w.i = i0; w.i < i1; ++w.i) {
         w.load(a);
         if (w.n == 0) continue;
         if (w.bad(a)) {
-            if (a.status) atomicCAS(a.status, 0, kStatusBad);
-            if (w.i % gridDim.x == blockIdx.x)
-#pragma unroll 1
-                for (int64_t e = 0; e < static_cast<int64_t>(w.n) * a.nq * D; ++e)
-                    a.out[static_cast<int64_t>(w.first) * a.nq * D + e] = 0x7fc0;
+            any_bad = true;
             continue;
         }
         mine += w.head_weight(a) * a.nkv;
@@ -286,7 +305,10 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
         if (lane >= o) before += up;
     }
     if (lane == 31) sh.warp[warp] = before;
-    __syncthreads();
+    if (__builtin_expect(__syncthreads_or(any_bad), 0)) {
+        if (any_bad && a.status) atomicCAS(a.status, 0, kStatusBad);
+        fill_bad<W>(a, D);
+    }
     int64_t total = 0, base = before - mine;
 #pragma unroll 1
     for (int k = 0; k < THREADS / 32; ++k) {
