@@ -583,7 +583,8 @@ NF_API int nf_kv_write(const nf_kv_cache* cache, const nf_rope* rope, const void
  * positions a row sees never reaches the row's result.  Rows behind
  * row_start_dev[batch] stay as they were; the rows of a sequence whose
  * prefix, rows or cache sequence lie outside the buffers become NaN, and
- * *status_dev nonzero (row_start_dev entries are clamped to [0, rows]). */
+ * *status_dev nonzero (row_start_dev entries are clamped to [0, rows]); so do
+ * all rows, should a wait inside the kernels run out (after 10 s). */
 NF_API int64_t nf_tree_attention_workspace(int head_dim);
 NF_API int nf_tree_attention(const nf_kv_cache* cache, const uint16_t* q_dev, int rows, int q_heads,
                              const int32_t* row_start_dev, int batch, const int32_t* prefix_dev,

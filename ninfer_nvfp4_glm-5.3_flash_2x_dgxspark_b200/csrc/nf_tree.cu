@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
         work_at(a.work).join[blockIdx.x].parts = 0;
+        work_at(a.work).gave_up[blockIdx.x] = 0;
     }
     if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
     __syncthreads();
@@ -946,7 +947,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
-    if (threadIdx.x == 0 && *abort_flag && a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
+    if (threadIdx.x == 0 && *abort_flag) {
+        work_at(a.work).gave_up[blockIdx.x] = 1;
+        if (a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
+    }
+}
+
+// After a wait that ran out nothing of the call can be relied on: every row becomes NaN.  Called by all threads of the
+// join's blocks.
+template <int D>
+__device__ __forceinline__ bool waits_ran_out(const TreeArgs& a, const Work& wk) {
+    static_assert(kMaxCtas <= 256);
+    const bool mine = threadIdx.x < gridDim.x && wk.gave_up[threadIdx.x] != 0;
+    if (__builtin_expect(!__syncthreads_or(mine), 1)) return false;
+    const int first = min(max(a.row_start[0], 0), a.rows), end = min(max(a.row_start[a.batch], 0), a.rows);
+    fill_nan(a, first, max(0, end - first), D,
+             (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x,
+             static_cast<int64_t>(gridDim.x) * gridDim.y * blockDim.x);
+    return true;
 }
 
 // Joins the parts of items that several CTAs computed, in their order: two
@@ -958,6 +976,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     const Work wk = work_at(a.work);
     const int b = blockIdx.x;
     const JoinDesc d = wk.join[b];
+    if (waits_ran_out<D>(a, wk)) return;
     const int lane = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * 2;
     if (d.parts == 0 || r0 >= d.rows) return;
     constexpr int E = D / 32;
@@ -1035,6 +1054,7 @@ __global__ void __launch_bounds__(256) tree_join_few_kernel(const __grid_constan
     const Work wk = work_at(a.work);
     const int b = blockIdx.x;
     const JoinDesc d = wk.join[b];
+    if (waits_ran_out<D>(a, wk)) return;
     const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
     if (d.parts == 0 || r >= d.rows) return;
     constexpr int E = D / 32;
@@ -1142,7 +1162,7 @@ extern "C" {
 
 int64_t nf_tree_attention_workspace(int head_dim) {
     if (head_dim != 64 && head_dim != 128) return 0;
-    return kJoinBytes + kMlBytes + 2ll * kMaxCtas * kItemRows * head_dim * 4;
+    return kJoinBytes + kGaveUpBytes + kMlBytes + 2ll * kMaxCtas * kItemRows * head_dim * 4;
 }
 
 int nf_tree_attention(const nf_kv_cache* cache, const uint16_t* q, int rows, int q_heads, const int32_t* row_start,

@@ -37,16 +37,19 @@ struct JoinDesc {
 };
 struct Work {
     JoinDesc* join;  // [kMaxCtas]
+    int32_t* gave_up;  // [kMaxCtas]: a wait of the CTA ran out
     float2* ml;      // [2 kMaxCtas][kItemRows] (m, l)
     float* acc;      // [2 kMaxCtas][kItemRows][D]
 };
 constexpr int64_t kJoinBytes = (kMaxCtas * sizeof(JoinDesc) + 255) / 256 * 256;
+constexpr int64_t kGaveUpBytes = (kMaxCtas * 4 + 255) / 256 * 256;
 constexpr int64_t kMlBytes = 2ll * kMaxCtas * kItemRows * 8;
 
 __host__ __device__ inline Work work_at(void* p) {
     uint8_t* b = static_cast<uint8_t*>(p);
-    return Work{reinterpret_cast<JoinDesc*>(b), reinterpret_cast<float2*>(b + kJoinBytes),
-                reinterpret_cast<float*>(b + kJoinBytes + kMlBytes)};
+    uint8_t* parts = b + kJoinBytes + kGaveUpBytes;
+    return Work{reinterpret_cast<JoinDesc*>(b), reinterpret_cast<int32_t*>(b + kJoinBytes), reinterpret_cast<float2*>(parts),
+                reinterpret_cast<float*>(parts + kMlBytes)};
 }
 
 struct TreeArgs {
