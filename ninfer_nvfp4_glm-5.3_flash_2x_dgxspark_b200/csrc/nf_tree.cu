@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
         work_at(a.work).join[blockIdx.x].parts = 0;
-        work_at(a.work).gave_up[blockIdx.x] = 0;
+        work_at(a.work).marks[blockIdx.x] = 0;
     }
     if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
     __syncthreads();
@@ -948,23 +948,41 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag) {
-        work_at(a.work).gave_up[blockIdx.x] = 1;
+        work_at(a.work).marks[blockIdx.x] = kMarkGaveUp;
         if (a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
     }
 }
 
-// After a wait that ran out nothing of the call can be relied on: every row becomes NaN.  Called by all threads of the
-// join's blocks.
+// NaN into `rows` rows of the output from `first` on, shared by all threads of the grid.
 template <int D>
-__device__ __forceinline__ bool waits_ran_out(const TreeArgs& a, const Work& wk) {
+__device__ __forceinline__ void fill_nan(const TreeArgs& a, int first, int rows) {
+    const int64_t per_row = static_cast<int64_t>(a.nq) * D, n = rows * per_row / 8;
+    uint4* dst = reinterpret_cast<uint4*>(a.out + first * per_row);
+    const int64_t threads = static_cast<int64_t>(gridDim.x) * gridDim.y * blockDim.x;
+    int64_t e = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;
+#pragma unroll 1
+    for (; e < n; e += threads) dst[e] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+}
+// What the join does beside joining, with all threads of its grid: the rows of refused sequences become NaN (4,096 rows of
+// 32 heads of 128: 24 us; one thread of the attention's took 384 ms), and after a wait that ran out, when nothing of
+// the call can be relied on, every row does.  Returns whether that is so.
+template <int D>
+__device__ __forceinline__ bool rows_without_result(const TreeArgs& a, const Work& wk) {
     static_assert(kMaxCtas <= 256);
-    const bool mine = threadIdx.x < gridDim.x && wk.gave_up[threadIdx.x] != 0;
-    if (__builtin_expect(!__syncthreads_or(mine), 1)) return false;
-    const int first = min(max(a.row_start[0], 0), a.rows), end = min(max(a.row_start[a.batch], 0), a.rows);
-    fill_nan(a, first, max(0, end - first), D,
-             (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x,
-             static_cast<int64_t>(gridDim.x) * gridDim.y * blockDim.x);
-    return true;
+    const int mark = threadIdx.x < gridDim.x ? wk.marks[threadIdx.x] : 0;
+    if (__builtin_expect(!__syncthreads_or(mark), 1)) return false;
+    if (__syncthreads_or(mark == kMarkGaveUp)) {
+        const int first = min(max(a.row_start[0], 0), a.rows), end = min(max(a.row_start[a.batch], 0), a.rows);
+        fill_nan<D>(a, first, max(0, end - first));
+        return true;
+    }
+    Walk<kItemRows, kKeys, 0, 1, 1> w;  // (for its view of a sequence)
+#pragma unroll 1
+    for (w.i = 0; w.i < a.batch; ++w.i) {
+        w.load(a);
+        if (w.n > 0 && w.bad(a)) fill_nan<D>(a, w.first, w.n);
+    }
+    return false;
 }
 
 // Joins the parts of items that several CTAs computed, in their order: two
@@ -976,7 +994,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     const Work wk = work_at(a.work);
     const int b = blockIdx.x;
     const JoinDesc d = wk.join[b];
-    if (waits_ran_out<D>(a, wk)) return;
+    if (rows_without_result<D>(a, wk)) return;
     const int lane = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * 2;
     if (d.parts == 0 || r0 >= d.rows) return;
     constexpr int E = D / 32;
@@ -1054,7 +1072,7 @@ __global__ void __launch_bounds__(256) tree_join_few_kernel(const __grid_constan
     const Work wk = work_at(a.work);
     const int b = blockIdx.x;
     const JoinDesc d = wk.join[b];
-    if (waits_ran_out<D>(a, wk)) return;
+    if (rows_without_result<D>(a, wk)) return;
     const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
     if (d.parts == 0 || r >= d.rows) return;
     constexpr int E = D / 32;
@@ -1162,7 +1180,7 @@ extern "C" {
 
 int64_t nf_tree_attention_workspace(int head_dim) {
     if (head_dim != 64 && head_dim != 128) return 0;
-    return kJoinBytes + kGaveUpBytes + kMlBytes + 2ll * kMaxCtas * kItemRows * head_dim * 4;
+    return kJoinBytes + kMarkBytes + kMlBytes + 2ll * kMaxCtas * kItemRows * head_dim * 4;
 }
 
 int nf_tree_attention(const nf_kv_cache* cache, const uint16_t* q, int rows, int q_heads, const int32_t* row_start,

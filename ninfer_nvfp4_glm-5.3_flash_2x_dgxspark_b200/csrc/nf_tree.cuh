@@ -35,19 +35,20 @@ struct JoinDesc {
     int32_t head;    // KV head
     int32_t pad[3];
 };
+enum : int32_t { kMarkGaveUp = 1, kMarkRefused = 2 };  // a wait of the CTA ran out; some sequence is refused
 struct Work {
     JoinDesc* join;  // [kMaxCtas]
-    int32_t* gave_up;  // [kMaxCtas]: a wait of the CTA ran out
+    int32_t* marks;  // [kMaxCtas]: what the join has to know of every CTA
     float2* ml;      // [2 kMaxCtas][kItemRows] (m, l)
     float* acc;      // [2 kMaxCtas][kItemRows][D]
 };
 constexpr int64_t kJoinBytes = (kMaxCtas * sizeof(JoinDesc) + 255) / 256 * 256;
-constexpr int64_t kGaveUpBytes = (kMaxCtas * 4 + 255) / 256 * 256;
+constexpr int64_t kMarkBytes = (kMaxCtas * 4 + 255) / 256 * 256;
 constexpr int64_t kMlBytes = 2ll * kMaxCtas * kItemRows * 8;
 
 __host__ __device__ inline Work work_at(void* p) {
     uint8_t* b = static_cast<uint8_t*>(p);
-    uint8_t* parts = b + kJoinBytes + kGaveUpBytes;
+    uint8_t* parts = b + kJoinBytes + kMarkBytes;
     return Work{reinterpret_cast<JoinDesc*>(b), reinterpret_cast<int32_t*>(b + kJoinBytes), reinterpret_cast<float2*>(parts),
                 reinterpret_cast<float*>(parts + kMlBytes)};
 }
@@ -257,29 +258,7 @@ struct Walk {
     }
 };
 
-// NaN into `rows` rows of the output from `first` on, 8 values a store; thread `me` of `threads` that share them.
-__device__ __forceinline__ void fill_nan(const TreeArgs& a, int first, int rows, int D, int64_t me, int64_t threads) {
-    const int64_t per_row = static_cast<int64_t>(a.nq) * D;
-    uint4* dst = reinterpret_cast<uint4*>(a.out + first * per_row);
-    const int64_t n = rows * per_row / 8;
-#pragma unroll 1
-    for (int64_t e = me; e < n; e += threads) dst[e] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-}
-// The rows of bad sequences become NaN: all CTAs share every such sequence's rows (4,096 rows of 32 heads of 128: 22 us;
-// by one thread 384 ms).  Not inlined, as it is rare: the roles that follow share the instruction cache.
-template <typename W>
-__device__ __noinline__ void fill_bad(const TreeArgs& a, int D) {
-    W w;
-#pragma unroll 1
-    for (w.i = 0; w.i < a.batch; ++w.i) {
-        w.load(a);
-        if (w.n > 0 && w.bad(a))
-            fill_nan(a, w.first, w.n, D, static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x,
-                     static_cast<int64_t>(gridDim.x) * blockDim.x);
-    }
-}
-
-// Finds the CTA's share (every thread sums the weights of a run of sequences), and fills the rows of bad sequences.  A share
+// Finds the CTA's share (every thread sums the weights of a run of sequences) and marks bad sequences for the join.  A share
 // is not smaller than LEAST tiles, those that a CTA takes at a time: smaller
 // ones would only make more parts to join, and no share inside an item may be
 // without a tile.  Ends with a __syncthreads.
@@ -290,13 +269,13 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
     const int run = (a.batch + THREADS - 1) / THREADS;
     const int i0 = min(a.batch, static_cast<int>(threadIdx.x) * run), i1 = min(a.batch, i0 + run);
     int64_t mine = 0;
-    bool any_bad = false;
 #pragma unroll 1
     for (w.i = i0; w.i < i1; ++w.i) {
         w.load(a);
         if (w.n == 0) continue;
         if (w.bad(a)) {
-            any_bad = true;
+            if (a.status) atomicCAS(a.status, 0, kStatusBad);
+            work_at(a.work).marks[blockIdx.x] = kMarkRefused;
             continue;
         }
         mine += w.head_weight(a) * a.nkv;
@@ -308,10 +287,7 @@ __device__ __forceinline__ Share find_share(const TreeArgs& a, ShareScratch& sh)
         if (lane >= o) before += up;
     }
     if (lane == 31) sh.warp[warp] = before;
-    if (__builtin_expect(__syncthreads_or(any_bad), 0)) {
-        if (any_bad && a.status) atomicCAS(a.status, 0, kStatusBad);
-        fill_bad<W>(a, D);
-    }
+    __syncthreads();
     int64_t total = 0, base = before - mine;
 #pragma unroll 1
     for (int k = 0; k < THREADS / 32; ++k) {

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
         work_at(a.work).join[blockIdx.x].parts = 0;
-        work_at(a.work).gave_up[blockIdx.x] = 0;
+        work_at(a.work).marks[blockIdx.x] = 0;
     }
     __syncthreads();
     pdl_trigger();  // the join's blocks may wait for this grid beside it
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
     }
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) {
-        work_at(a.work).gave_up[blockIdx.x] = 1;
+        work_at(a.work).marks[blockIdx.x] = kMarkGaveUp;
         if (a.status) atomicCAS(a.status, 0, NF_DEVERR_WAIT_FULL);
     }
 }
