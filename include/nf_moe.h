@@ -622,7 +622,8 @@ NF_API int nf_token_logprobs(const void* logits_dev, int logits_type, int64_t ro
  * [batch][max_path]: nodes in rising order, as a child's index is above its
  * parent's.  A sequence with indices outside the cache, or a path that does
  * not rise, is left as it was and sets *status_dev.  No two entries of a call
- * may name the same cache sequence. */
+ * may name the same cache sequence.  2 kv_heads (head_dim / 8 + 1) must be
+ * below 2^31. */
 NF_API int nf_kv_accept(const nf_kv_cache* caches, int layers, const int32_t* prefix_dev, const int32_t* path_dev,
                         int max_path, const int32_t* path_len_dev, const int32_t* cache_seq_dev, int batch,
                         int32_t* status_dev, void* stream);

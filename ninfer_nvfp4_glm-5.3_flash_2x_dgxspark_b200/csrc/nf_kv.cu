@@ -610,6 +610,8 @@ int nf_kv_accept(const nf_kv_cache* caches, int layers, const int32_t* prefix, c
             caches[l].head_dim != caches[0].head_dim)
             return kv_fail(NF_ERR_SHAPE, "the cache of layer %d has another kind or shape than layer 0's", l);
     }
+    if (layers > 0 && static_cast<int64_t>(caches[0].kv_heads) * 2 * (caches[0].head_dim / 8 + 1) > 0x7fffffffll)
+        return kv_fail(NF_ERR_CAPACITY, "a position's rows of %d KV heads: 16-byte pieces must be below 2^31", caches[0].kv_heads);
     if (layers == 0 || batch == 0 || max_path == 0) return NF_OK;
     if (!prefix || !path || !path_len) return kv_fail(NF_ERR_INVALID, "null prefix, path or length pointer");
     const cudaError_t e = launch_kv_accept(caches, layers, prefix, path, max_path, path_len, cache_seq, batch, status,
