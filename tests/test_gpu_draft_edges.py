@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from helpers import nfm
-from test_gpu_draft_ops import check_attention, ints, make_cache
+from test_gpu_draft_ops import check_attention, check_logprobs, ints, logits, make_cache
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -62,3 +62,47 @@ def test_a_refused_sequence_takes_no_longer_than_a_good_one(rows):
     refused = best_us(lambda: m.tree_attention(c, q, start, bad, out, work))
     assert out[:rows].isnan().all()
     assert refused <= 2 * fine + 20, (refused, fine)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("singles, chunk", [(40, 200), (40, 100), (70, 100), (150, 60), (3, 300)])
+def test_attention_of_a_chunk_among_single_rows(kind, singles, chunk):
+    """One long chunk among decoding sequences, on both sides of the average that chooses the kernel."""
+    rng = np.random.default_rng(singles + chunk)
+    rows, at = [1] * (singles + 1), int(rng.integers(singles + 1))
+    rows[at] = chunk
+    prefix = rng.integers(0, 300, singles + 1).tolist()
+    check_attention(chunk, rows, prefix, 8, 1, 64, kind, seq=rng.permutation(singles + 1).tolist(), context=300 + chunk)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_attention_of_a_batch_with_many_empty_places(kind):
+    """A batch of fixed places of which few hold rows."""
+    rows = [0] * 200
+    rows[0], rows[77], rows[78], rows[199] = 1, 9, 1, 2
+    prefix = [5 * i for i in range(200)]
+    check_attention(3, rows, prefix, 8, 2, 64, kind, seq=[i % 7 for i in range(200)], seqs=7, context=1000)
+
+
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("vocab", [20000, 40001, 151552])
+def test_logprobs_of_masked_rows_over_several_ctas(wide, vocab):
+    """Rows of which a grammar leaves a few tokens, and rows without a distribution, where several CTAs share a row: the top
+    tokens go on with -infinity and then NaN, the lower index first."""
+    rng = np.random.default_rng(vocab)
+    x = logits(rng, 8, vocab, wide, pad=3)
+    inf = float("inf")
+    for r, left in enumerate((1, 3, 20, 33)):
+        keep = torch.from_numpy(rng.choice(vocab, left, replace=False)).cuda()
+        old = x[r, keep].clone()
+        x[r] = -inf
+        x[r, keep] = old
+    x[4] = -inf
+    x[5, vocab // 2:] = float("nan")
+    x[6] = float("nan")
+    x[7, :-1] = -inf
+    target = torch.from_numpy(rng.integers(0, vocab, 8)).int().cuda()
+    target[0] = int(x[0].float().argmax())
+    for rows in (8, 1):  # eight and fewer CTAs a row
+        for top in (32, 5, 1):
+            check_logprobs(x[:rows], target[:rows], top)
