@@ -27,6 +27,7 @@ int kv_fail(int status, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(g_kv_error, sizeof(g_kv_error), fmt, ap);
     va_end(ap);
+    if (status == NF_ERR_CUDA) cudaGetLastError();  // told here, and no later launch's failure
     return status;
 }
 

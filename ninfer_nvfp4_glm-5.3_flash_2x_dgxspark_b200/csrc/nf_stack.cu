@@ -479,7 +479,10 @@ int nf_stack_load_kv(nf_stack* s, int layer, const uint16_t* k_host, const uint1
         cudaFree(wide);
     }
     cudaSetDevice(prev);
-    if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "cache upload: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // an allocation's failure is no later launch's
+        return s->fail(NF_ERR_CUDA, "cache upload: %s", cudaGetErrorString(e));
+    }
     return NF_OK;
 }
 
@@ -505,7 +508,10 @@ int nf_stack_fill_kv(nf_stack* s, uint64_t seed) {
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     cudaFree(wide);
     cudaSetDevice(prev);
-    if (e != cudaSuccess) return s->fail(NF_ERR_CUDA, "cache fill: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // an allocation's failure is no later launch's
+        return s->fail(NF_ERR_CUDA, "cache fill: %s", cudaGetErrorString(e));
+    }
     return NF_OK;
 }
 

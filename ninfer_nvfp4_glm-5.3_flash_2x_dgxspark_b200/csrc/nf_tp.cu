@@ -653,7 +653,10 @@ int nf_tp_logprobs(nf_tp* h, int tokens, int64_t rows, const int32_t* target, in
     const cudaError_t e = launch_token_logprobs(h->mbox + kFlagsBytes, NF_DTYPE_F32, rows, tokens, rows, target, top, logprob,
                                                 entropy, top_idx, top_lp, static_cast<cudaStream_t>(stream), h->epoch, h->cap);
     cudaSetDevice(prev);
-    if (e != cudaSuccess) return h->fail(NF_ERR_CUDA, "log-probability launch: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return h->fail(NF_ERR_CUDA, "log-probability launch: %s", cudaGetErrorString(e));
+    }
     return NF_OK;
 }
 

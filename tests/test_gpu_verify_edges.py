@@ -208,3 +208,20 @@ def test_padded_rows_need_no_token(model, kv):  # noqa: F811
         assert changed(st, old) == {(0, 10), (1, 20), (1, 21)}
         close(got[before:before + 3], fin, "beside padding")
     st.close()
+
+
+def test_a_step_after_a_fill_without_memory(model):  # noqa: F811
+    """An E4M3 cache is filled through a buffer of BF16 rows.  Without memory for that the call fails, and the next step
+    does not."""
+    context = 1 << 17
+    st = make_stack(model, 8, context, "e4m3")
+    need = 2 * 8 * context * CFG["kv_heads"] * 128
+    torch.cuda.empty_cache()
+    hold = torch.empty(torch.cuda.mem_get_info()[0] - need // 2, dtype=torch.uint8, device="cuda")
+    with pytest.raises(m.NfError, match="memory"):
+        st.fill_kv(3)
+    del hold
+    torch.cuda.empty_cache()
+    fin, _ = step(st, [1, 2, 3], [0, 1, 3], [0, 0])
+    assert not fin.isnan().any()
+    st.close()
