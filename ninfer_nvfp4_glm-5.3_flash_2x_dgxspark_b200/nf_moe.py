@@ -994,9 +994,22 @@ def _kv_check(st: int) -> None:
 
 def _dim(a, axis: int, name: str, rank: int) -> int:
     """A tensor's extent; the tensor must have `rank` axes."""
-    if len(a.shape) != rank:
-        raise NfError(2, f"{name} has {len(a.shape)} axes; expected {rank}")
-    return a.shape[axis]
+    try:
+        shape = a.shape
+    except AttributeError:
+        raise NfError(1, f"{name} is not a tensor") from None
+    if len(shape) != rank:
+        raise NfError(2, f"{name} has {len(shape)} axes; expected {rank}")
+    return shape[axis]
+
+
+def _workspace(a, device: int) -> tuple[int | None, int]:
+    """A workspace's address and bytes, as the library checks them."""
+    if a is None:
+        return None, 0
+    if not hasattr(a, "numel"):
+        raise NfError(1, "workspace is not a tensor")
+    return _buf(a, 0, _K.u8, "workspace", device), a.numel()
 
 
 def _top(top_idx, top_logprob) -> int:
@@ -1118,7 +1131,7 @@ def tree_attention(cache: KvCache, q, row_start, prefix, out, workspace, *, cach
         _buf(row_start, batch + 1, _K.i32, "row_start", dv), batch, _buf(prefix, batch, _K.i32, "prefix", dv),
         _buf(cache_seq, batch, _K.i32, "cache_seq", dv), _buf(mask, rows * words, _K.u64, "mask", dv), words,
         dim ** -0.5 if scale is None else scale, _buf(out, rows * heads * dim, _K.bf16, "out", dv),
-        _buf(workspace, 0, _K.u8, "workspace", dv), workspace.numel(), _buf(status, 1, _K.i32, "status", dv),
+        *_workspace(workspace, dv), _buf(status, 1, _K.i32, "status", dv),
         stream or None))
 
 
@@ -1147,7 +1160,7 @@ def token_logprobs(logits, targets, logprob, entropy, top_idx, top_logprob, work
         logits.stride(0) if rows > 1 else max(1, vocab), rows, vocab, _buf(targets, rows, _K.i32, "targets", dv), top,
         _buf(logprob, rows, _K.f32, "logprob", dv), _buf(entropy, rows, _K.f32, "entropy", dv),
         _buf(top_idx, rows * top, _K.i32, "top_idx", dv), _buf(top_logprob, rows * top, _K.f32, "top_logprob", dv),
-        _buf(workspace, 0, _K.u8, "workspace", dv), workspace.numel(), stream or None))
+        *_workspace(workspace, dv), stream or None))
 
 
 def kv_accept(caches: KvCaches, prefix, path, path_len, *, cache_seq=None, status=None, stream=0) -> None:

@@ -106,3 +106,23 @@ def test_logprobs_of_masked_rows_over_several_ctas(wide, vocab):
     for rows in (8, 1):  # eight and fewer CTAs a row
         for top in (32, 5, 1):
             check_logprobs(x[:rows], target[:rows], top)
+
+
+def test_what_is_missing_is_refused_by_name():
+    """None, a number or a list in a tensor's place is refused as the binding refuses other arguments."""
+    c, _, _ = make_cache(np.random.default_rng(1), "bf16", 2, 1, 8, 64)
+    q = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    w = torch.empty(m.tree_attention_workspace(64), dtype=torch.uint8, device="cuda")
+    s, p, lg, f = ints([0, 1, 2]), ints([0, 0]), torch.zeros(2, 9, device="cuda"), torch.zeros(2, device="cuda")
+    for word, call in (("workspace", lambda: m.tree_attention(c, q, s, p, q, None)), ("workspace", lambda: m.tree_attention(c, q, s, p, q, 5)),
+                       ("q ", lambda: m.tree_attention(c, None, s, p, q, w)), ("row_start", lambda: m.tree_attention(c, q, [0, 2], p, q, w)),
+                       ("prefix", lambda: m.tree_attention(c, q, s, None, q, w)), ("output", lambda: m.tree_attention(c, q, s, p, None, w)),
+                       ("workspace", lambda: m.token_logprobs(lg, None, None, f, None, None, None)),
+                       ("logits", lambda: m.token_logprobs(None, None, None, f, None, None, w)),
+                       ("qkv", lambda: m.kv_write(c, m.Rope(64), None, 2, p, q)),
+                       ("position", lambda: m.kv_write(c, m.Rope(64), torch.zeros(2, 256, device="cuda"), 2, None, q)),
+                       ("path", lambda: m.kv_accept(m.KvCaches([c]), p, None, p)),
+                       ("null", lambda: m.kv_accept(m.KvCaches([c]), p, p.view(2, 1), None))):
+        with pytest.raises(m.NfError, match=word):
+            call()
+    m.tree_attention(c, q, s, p, torch.empty_like(q), w.view(-1, 64))  # a workspace of any shape will do
