@@ -527,7 +527,9 @@ enum {
     NF_ROPE_PLAIN = 0,
     NF_ROPE_LINEAR = 1, /* f_i / factor */
     NF_ROPE_YARN = 2    /* with r_i = original_context f_i / (2 pi) and g_i = clamp((r_i - slow) / (fast - slow), 0, 1):
-                           g_i f_i + (1 - g_i) f_i / factor, the rotated dims multiplied by 0.1 ln(factor) + 1 */
+                           g_i f_i + (1 - g_i) f_i / factor, the rotated dims multiplied by 0.1 ln(factor) + 1.  The ramp
+                           is linear in the turns r_i; a model whose ramp is linear in i between two pairs, or that has
+                           frequencies or a factor of its own, sets turn[] and magnitude itself */
 };
 typedef struct nf_rope {
     int32_t head_dim, rotary_dim, layout;
@@ -580,7 +582,8 @@ NF_API int nf_kv_write(const nf_kv_cache* cache, const nf_rope* rope, const void
  * BF16, with the rest as a second BF16 term in E4M3 tiles that hold new rows,
  * or, with an E4M3 cache and few rows, to F16 (one below 2^-22 of the row's
  * largest by up to 2^-32 of that one).  What the cache holds outside the
- * positions a row sees never reaches the row's result.  Rows behind
+ * positions a row sees never reaches the row's result; a row that sees a new
+ * row's value that is infinite or NaN becomes NaN.  Rows behind
  * row_start_dev[batch] stay as they were; the rows of a sequence whose
  * prefix, rows or cache sequence lie outside the buffers become NaN, and
  * *status_dev nonzero (row_start_dev entries are clamped to [0, rows]); so do
@@ -638,7 +641,10 @@ NF_API int nf_tp_logprobs(nf_tp* handle, int tokens, int64_t rows, const int32_t
  * nf_stack_create with the caches' kind (nf_stack_create: NF_KV_BF16).  With
  * NF_KV_E4M3 the caches take half the bytes; nf_stack_decode, _load_kv and
  * _fill_kv work the same (the latter two quantise their BF16 rows), and
- * nf_stack_kv_cache returns NF_ERR_UNSUPPORTED. */
+ * nf_stack_kv_cache returns NF_ERR_UNSUPPORTED.  nf_stack_verify, and decode
+ * over E4M3 caches, hold q in BF16 and take exact angles; decode over BF16
+ * caches holds q in F32 and takes the reference's F32 angles, which are off by
+ * some position x 10^-7 radians. */
 NF_API int nf_stack_create_kv(const nf_stack_desc* desc, int kv_kind, int device, nf_stack** out);
 /* A layer's caches as the calls above take them (device pointers). */
 NF_API int nf_stack_kv(nf_stack* stack, int layer, nf_kv_cache* out);

@@ -158,6 +158,10 @@ __device__ __forceinline__ int rank_of(uint64_t v, const uint64_t* s, int n) {
 // 256 rows of 151,552 F32 logits, top 5: 34.9 us, 4.45 TB/s; 4,001 rows of
 // 32,003 BF16 logits: 63.5 us, 4.0 TB/s.  The CTAs an SM holds matter: F32 with
 // 76 registers, so three, 48.2 us; BF16 with four 71.6, with five 66.4.
+// Where a CTA's share holds fewer than `top` threads with a logit above
+// -infinity, every logit is a candidate, and the CTA reads its share once more
+// for every top token: with 1, 3 or 20 tokens left in each of the 256 rows, 384,
+// 383 and 178 us at top 5 and 1,244 at top 20, against 37.
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, BF16 ? 6 : 4) token_logprobs_kernel(const void* __restrict__ logits,
                                                                   const uint32_t* __restrict__ epoch,

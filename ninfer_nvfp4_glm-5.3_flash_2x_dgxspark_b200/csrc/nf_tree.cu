@@ -18,9 +18,10 @@
 // task ahead) took 20% longer, twice the softmax warps 8%.
 // The softmax subtracts the maxima that the tiles before had: no weight gets
 // beyond 2^8 with them, or they rise (227 to 223 us).
-// 4 sequences of 64 nodes, 8 rows a node, on up to 65,000 E4M3 keys: 223 us,
-// 590 TFLOP/s; 24 of 16 nodes on 8,191 BF16 keys, where a tile of 128 rows
-// waits for its 64 KB more than for the products: 77 us, 4.0 TB/s.
+// 4 sequences of 64 nodes, 8 rows a node, on up to 65,000 E4M3 keys: 224 us,
+// 588 TFLOP/s; 24 of 16 nodes on 8,191 BF16 keys, where a tile of 128 rows
+// waits for its 64 KB more than for the products: 76 to 84 us from run to run,
+// 3.6 to 4.0 TB/s.
 #include "nf_tree.cuh"
 
 #include <algorithm>
@@ -264,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     using ItemWalk = Walk<kItemRows, kKeys, 10, 2, 3>;
     // Weights in units of about 2,070 cycles, from the CTAs' times: a tile with two row tiles 6,200, with one 4,200, an
     // item's start and end 17,000 to 24,000.  With tiles alone a few CTAs took 1.5 times the others' (287 us above).
+    // Taken from BF16 and E4M3 caches of D 128 and used for D 64 too, whose tiles are half as long.
     const Share share = find_share<D, kThreads, 1, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;
     const uint32_t tmem = *s_tmem;
@@ -1160,6 +1162,10 @@ cudaError_t launch_tree_attention(const nf_kv_cache& c, const uint16_t* q, int r
     //   BF16  50.2 52.2 60.4  58.4 54.3 62.4  74.8 62.5 62.5  97.3 72.7 62.5  175 114 64.5
     // and one sequence on 65,000 keys: E4M3, 32 rows: 62.5 64.5 72.7; BF16, 24 rows: 80.9 68.6 70.7.  E4M3's keys take
     // longer to convert than a second look at them in the L2.
+    // The average serves a batch of one length.  255 sequences of one row on 1,000 to 2,000 keys and a chunk behind 32,768
+    // less its rows, in one call and apart: a chunk of 512 rows (all in items of 8 or 16 rows) E4M3 2,510 against 85 + 423,
+    // BF16 2,040 against 133 + 315; of 1,024 (E4M3 and BF16 in the kernel for many) 1,110 against 85 + 822, 785 against
+    // 133 + 587.  A caller with such a batch does better with two calls.
     const int64_t all = static_cast<int64_t>(rows) * a.G;
     const int nt = all <= (fp8 ? 32ll : 8ll) * batch ? 1 : !fp8 && all <= 24ll * batch ? 2 : 0;
     cudaError_t e = nt    ? launch_tree_few(c, a, nt, grid, st)

@@ -1,8 +1,8 @@
 // nf_tree_few.cu -- nf_tree_attention's kernel for few rows of a sequence and
 // KV head (decode, and trees of a node or two): warp-level tensor-core tiles.
 //
-// The work is the cache's bytes: 8 rows do 16 (BF16) or 32 (E4M3) flops a
-// byte, a fraction of what the tensor cores could.  So the keys only have to
+// The work is the cache's bytes: 8 rows do 8 (BF16) or 16 (E4M3) flops a
+// byte (a row 4 D flops on a key of 4 D or 2 D bytes), a fraction of what the tensor cores could.  So the keys only have to
 // stream: one warp issues TMA tiles of 64 keys into a ring, and eight warps
 // take 32 keys of a tile each (pairs of warps take tiles in turn), with their
 // own running maximum, sum and output in registers.  Two more warps bring the
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
     }
     __syncthreads();
     pdl_trigger();  // the join's blocks may wait for this grid beside it
-    // an item's start and end take the time of about eight tiles: 83 us above, without that weight 90
+    // an item's start and end take the time of about eight tiles (E4M3, D 128): 83 us above, without that weight 90
     using ItemWalk = Walk<kRows, kKeys, 8, 1, 1>;
     const Share share = find_share<D, G_::kThreads, G_::kGroups, ItemWalk>(a, s_share);
     const bool idle = share.lo >= share.hi;

@@ -1059,7 +1059,9 @@ class KvCaches:
 
 class Rope:
     """Rotary positions (nf_rope): layout "half" or "interleaved"; scaling
-    "none", "linear" or "yarn" (factor, original_context, fast, slow)."""
+    "none", "linear" or "yarn" (factor, original_context, fast, slow).  A model
+    with frequencies of its own sets desc.turn (turns a position, as 64-bit
+    fractions) and desc.magnitude afterwards."""
 
     def __init__(self, head_dim: int, *, rotary_dim: int | None = None, layout: str = "half", theta: float = 10000.0,
                  scaling: str = "none", factor: float = 1.0, original_context: float = 0.0, fast: float = 32.0,
