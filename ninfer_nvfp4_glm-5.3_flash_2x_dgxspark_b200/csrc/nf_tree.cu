@@ -978,11 +978,23 @@ __device__ __forceinline__ bool rows_without_result(const TreeArgs& a, const Wor
         fill_nan<D>(a, first, max(0, end - first));
         return true;
     }
-    Walk<kItemRows, kKeys, 0, 1, 1> w;  // (for its view of a sequence)
+    // a block looks at 256 sequences at a time, a thread each, and then takes its share of every bad one's rows
+    __shared__ int2 s_rows[256];
+    __shared__ int s_n;
 #pragma unroll 1
-    for (w.i = 0; w.i < a.batch; ++w.i) {
-        w.load(a);
-        if (w.n > 0 && w.bad(a)) fill_nan<D>(a, w.first, w.n);
+    for (int i0 = 0; i0 < a.batch; i0 += 256) {
+        __syncthreads();
+        if (threadIdx.x == 0) s_n = 0;
+        __syncthreads();
+        Walk<kItemRows, kKeys, 0, 1, 1> w;  // (for its view of a sequence)
+        w.i = i0 + static_cast<int>(threadIdx.x);
+        if (w.i < a.batch) {
+            w.load(a);
+            if (w.n > 0 && w.bad(a)) s_rows[atomicAdd(&s_n, 1)] = make_int2(w.first, w.n);
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int k = 0; k < s_n; ++k) fill_nan<D>(a, s_rows[k].x, s_rows[k].y);
     }
     return false;
 }
