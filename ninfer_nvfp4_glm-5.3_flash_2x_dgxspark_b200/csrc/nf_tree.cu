@@ -866,10 +866,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             __syncwarp();
             const float mr = s_ml[s * kTileRows + r].x;
             float lr = s_ml[s * kTileRows + r].y;
-            if (s_bad[idx % kBadRing] != 0 && r < rows && poisoned<D, FP8>(a, w.z, p0, n, w.first, node)) {
-                lr = NAN;
-                s_ml[s * kTileRows + r].y = lr;
-            }
+            if (__any_sync(0xffffffffu, s_bad[idx % kBadRing] != 0))
+                if (poisoned<D, FP8>(a, w.z, p0, n, w.first, node, r < rows)) {
+                    lr = NAN;
+                    s_ml[s * kTileRows + r].y = lr;
+                }
             __syncwarp();
             const bool whole = w.kind == 3;
             const int slot = 2 * blockIdx.x + (w.kind & 1), cnt = t1 - w.t0;

@@ -233,6 +233,11 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                 const bool whole = w.kind == 3;
                 const int slot = 2 * blockIdx.x + (w.kind & 1);
                 const Work wk = work_at(a.work);
+                uint32_t nan_rows = 0;
+                if (__any_sync(0xffffffffu, s_bad[at & 3] != 0)) {  // a lane a row
+                    const int node = (w.row0 + min(lane, rows - 1)) / a.G;
+                    nan_rows = __ballot_sync(0xffffffffu, poisoned<D, FP8>(a, w.z, w.p0, w.n, w.first, node, lane < rows));
+                }
 #pragma unroll 1
                 for (int e = tid; e < rows * (D / 4); e += kCount) {
                     const int r = e / (D / 4), d = e % (D / 4) * 4;
@@ -256,7 +261,7 @@ __global__ void __launch_bounds__(Geo<D, FP8, NT>::kThreads, 1) tree_few_kernel(
                         acc.w += g == 0.f ? 0.f : x.w * g;
                     }
                     const int row = w.row0 + r, nd = row / a.G;
-                    if (s_bad[at & 3] && poisoned<D, FP8>(a, w.z, w.p0, w.n, w.first, nd)) lt = NAN;
+                    if ((nan_rows >> r) & 1u) lt = NAN;
                     if (whole) {
                         const float iv = lt == 0.f ? 0.f : 1.f / lt;
                         uint16_t* dst = a.out + (static_cast<int64_t>(w.first + nd) * a.nq + w.g * a.G + (row - nd * a.G)) * D + d;

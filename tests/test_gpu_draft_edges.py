@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from helpers import nfm
-from test_gpu_draft_ops import check_attention, check_logprobs, ints, logits, make_cache
+from test_gpu_draft_ops import check_attention, check_logprobs, exact_attention, ints, logits, make_cache, tree_words
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -143,3 +143,50 @@ def test_what_is_missing_is_refused_by_name():
         with pytest.raises(m.NfError, match=word):
             call()
     m.tree_attention(c, q, s, p, torch.empty_like(q), w.view(-1, 64))  # a workspace of any shape will do
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("mask", [None, "any", "tree"])
+@pytest.mark.parametrize("rows", [[200] + [1] * 150, [3, 150, 70], [7, 2, 9]])
+def test_values_that_are_not_finite_in_a_long_sequence(kind, dim, mask, rows):
+    """A NaN and an infinity in new rows' values reach the rows that see them, in every kernel, and take no row that does
+    not; looking for those rows takes a small part of a call (65 ms where each thread looks for itself)."""
+    rng = np.random.default_rng(len(rows) + dim)
+    nq, nkv = 8, 1
+    long, n = int(np.argmax(rows)), max(rows)
+    prefix = rng.integers(0, 200, len(rows)).tolist()
+    c, k, v = make_cache(rng, kind, len(rows), nkv, 450, dim)
+    words = (n + 63) // 64
+    start = np.concatenate([[0], np.cumsum(rows)])
+    pairs = [tree_words(rng, r, words, mask) for r in rows] if mask else None
+    bits = torch.from_numpy(np.concatenate([p[0] for p in pairs])).cuda() if mask else None
+    q = torch.from_numpy(rng.standard_normal((int(start[-1]), nq, dim)).astype(np.float32)).bfloat16()
+    out, work = torch.empty_like(q, device="cuda"), torch.empty(m.tree_attention_workspace(dim), dtype=torch.uint8, device="cuda")
+    args = (c, q.cuda(), ints(start), ints(prefix), out, work)
+    fine = best_us(lambda: m.tree_attention(*args, mask=bits))
+    bad_rows = sorted({n - 1, n // 2})
+    for i, j in enumerate(bad_rows):
+        at = (long, 0, prefix[long] + j, 5 + 20 * i)
+        if kind == "bf16":
+            c.tensors[1][at] = float("nan") if i else float("inf")
+        elif i:
+            c.tensors[1].view(torch.uint8)[at] = 0xff
+        else:
+            c.tensors[3][at[:3]] = float("inf")
+    took = best_us(lambda: m.tree_attention(*args, mask=bits))
+    got = out.double().cpu().numpy()
+    qd = q.double().numpy()
+    for r in range(n):
+        vis = np.ones(prefix[long] + n, bool)
+        vis[prefix[long]:] = np.arange(n) <= r if mask is None else pairs[long][1][r][:n]
+        mine = got[start[long] + r]
+        if vis[prefix[long]:][bad_rows].any():
+            assert np.isnan(mine).all(), r
+        else:
+            want, tol = exact_attention(qd[start[long] + r], k[long, 0, :len(vis)], v[long, 0, :len(vis)], vis, dim ** -0.5)
+            assert np.all(np.abs(mine - want) <= tol), r
+    rest = np.ones(len(got), bool)
+    rest[start[long]:start[long + 1]] = False
+    assert not np.isnan(got[rest]).any()
+    assert took <= 4 * fine + 50, (took, fine)
