@@ -658,8 +658,9 @@ NF_API int nf_stack_kv(nf_stack* stack, int layer, nf_kv_cache* out);
  * optional) receives every row's greedy token, final_dev (F32 [rows, H],
  * optional) the final norm's output; nf_stack_logprobs reads the step's
  * logits.  Rows behind row_start_dev[batch] write nothing to the caches; their
- * tokens are not looked at and their outputs mean nothing.  The caches' positions from prefix on hold the rows of
- * the step until the next one writes there: nf_stack_accept keeps a path.
+ * tokens are not looked at and their outputs mean nothing.  The caches'
+ * positions from prefix on hold the rows of the step until the next one writes
+ * there: nf_stack_accept keeps a path.
  * A row whose token lies outside the vocabulary becomes NaN; a sequence that
  * nf_tree_attention refuses, or with a position below 0 or from 2^31 on,
  * becomes NaN as a whole and writes nothing.  nf_stack_sync reports both, and
